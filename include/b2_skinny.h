@@ -12,6 +12,10 @@
  *     of the decoder layer                                        (b2_w4_gemm_allreduce_rmsnorm)
  *   - a load-time repack of the W4 weights and the three W4 entry points above on it
  *     (b2_w4_repack, b2_w4_gemm_packed, b2_w4_gemm_allreduce(_rmsnorm)_packed)
+ *   - what a verify step runs between these products: rotary positions (b2_rope), the same with
+ *     the write to a paged cache (b2_rope_cache), attention of the rows over that cache, a long
+ *     prefix shared by all requests read once (b2_prefix_attn), and the logit processors between
+ *     the lm_head and the sampler (b2_logits_process)
  * Every compute entry point launches on the caller's stream, never synchronises and never
  * allocates, so it can be captured in a CUDA graph.
  *
@@ -50,9 +54,10 @@ extern "C" {
 #define B2_ERR_TIMEOUT 5     /* a bounded device-side wait gave up (peer never arrived)      */
 #define B2_ERR_STATE 6       /* bad handle, or an all-reduce handle that is not connected    */
 
-/* Element types for the all-reduce. */
+/* Element types. The all-reduce takes the first two. */
 #define B2_DTYPE_F16 0
 #define B2_DTYPE_F32 1
+#define B2_DTYPE_BF16 2 /* rotary, attention and logit operators only */
 
 /* Short text for a status code (static storage). */
 const char* b2_status_string(int status);
@@ -289,6 +294,95 @@ int b2_w4_gemm_allreduce_emulated(b2_nvar* const* handles, int ranks, const void
                                   const void* const* norm_weight, float eps, void* const* y, int M,
                                   int K, int N, int group_size, void* const* ws, size_t ws_bytes,
                                   void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions, and the same with the cache write
+ *
+ * For every query and key head of row r, pair i < rot_dim / 2 and t = positions[r] * inv_freq[i]
+ * (the product in fp64):  a' = scale * (a cos t - b sin t),  b' = scale * (b cos t + a sin t),
+ * with the pair (x[i], x[i + rot_dim/2]), or (x[2i], x[2i+1]) when `interleaved` is non-zero.
+ * Dimensions from rot_dim on are copied. Arithmetic in fp32, one rounding to the type.
+ *
+ * q [rows, q_heads, head_dim] and k [rows, kv_heads, head_dim] may be views: *_strides holds the
+ * {row, head} strides in elements, dimensions are contiguous. positions holds int32, or int64 when
+ * positions_64 is non-zero. q_out and k_out are contiguous; each may be its own input where that
+ * is contiguous. head_dim 2..1024, rot_dim even and <= head_dim. Types: fp16, bf16, fp32. Heads of
+ * 16-bit types whose pointers, strides and dimensions allow 16-byte accesses (head_dim % 8 == 0,
+ * rot_dim % 16 == 0) take the fast path.
+ * ---------------------------------------------------------------------------------------- */
+int b2_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+            const void* positions, int positions_64, const float* inv_freq, void* q_out,
+            void* k_out, int rows, int q_heads, int kv_heads, int head_dim, int rot_dim,
+            float scale, int interleaved, int dtype, void* stream);
+/* b2_rope on q (into q_out); the turned k and the plain v go to the rows' slots of the caches
+ * [pages, page_size, kv_heads, head_dim], whose {page, token, head} strides in elements are given.
+ * slots[r] = page * page_size + place in the page. A slot outside [0, pages * page_size) writes
+ * nothing (padding rows use -1). The slots of one call must differ: of two rows with one slot,
+ * either may be stored, element by element. */
+int b2_rope_cache(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                  const void* v, const int64_t* v_strides, const void* positions, int positions_64,
+                  const float* inv_freq, const int64_t* slots, void* q_out, void* k_cache,
+                  const int64_t* k_cache_strides, void* v_cache, const int64_t* v_cache_strides,
+                  int pages, int page_size, int rows, int q_heads, int kv_heads, int head_dim,
+                  int rot_dim, float scale, int interleaved, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention of a step's rows over a paged cache with a shared prefix
+ *
+ * Request b owns the rows row_start[b] .. row_start[b+1] (n_b of them; row_start never decreases).
+ * Its rows see the *prefix_len tokens of the prefix, stored in the pages prefix_pages[], and of
+ * its own own_lens[b] tokens (pages[b * pages_stride ...]; the cache already holds the step's
+ * rows, which are the last n_b of them) row i sees all up to its own place, own_lens[b] - n_b + i.
+ * With `tree` (int64 [rows], may be NULL), row t sees the tokens before the last n_b, and of
+ * those the m-th when bit m of tree[t] is set (m < 64).
+ *   out[t,h] = softmax_j(scale * q[t,h] . k_j) v_j,   lse[t,h] = log sum_j exp(scale * q[t,h] . k_j)
+ * A row that sees nothing, and a row of no request, gets out = 0 and lse = -inf. Tokens a row does
+ * not see do not reach it, whatever they hold (NaN, infinities); neither do places of a page
+ * behind a length. Tokens on a page whose id is outside [0, total_pages) are left out; lengths are
+ * cut at what the tables can hold.
+ *
+ * Lengths, tables and row starts are read on the device: a captured call follows them. Query head
+ * h reads KV head h / (q_heads / kv_heads). q [rows, q_heads, head_dim] with {row, head} strides
+ * (even); caches [total_pages, page_size, kv_heads, head_dim] with {page, token, head} strides
+ * (multiples of 8); out [rows, q_heads, head_dim] and lse (fp32, [rows, q_heads]) contiguous.
+ * head_dim a multiple of 8 up to 256, at most 1024 requests and 4096 rows, fp16 or bf16.
+ * Scores, statistics and sums are fp32; the weights are rounded to the type for the second product.
+ * ws: b2_prefix_attn_workspace() bytes, 16-byte aligned, no initialisation; calls that overlap on
+ * the GPU need one each. Equal calls give equal bits.
+ * ---------------------------------------------------------------------------------------- */
+size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, int kv_heads, int head_dim);
+int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
+                   const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,
+                   int total_pages, int page_size, const int32_t* prefix_pages, int n_prefix_pages,
+                   const int32_t* prefix_len, const int32_t* pages, int64_t pages_stride,
+                   int max_pages, const int32_t* own_lens, const int32_t* row_start,
+                   const int64_t* tree, int requests, int rows, int q_heads, int kv_heads,
+                   int head_dim, float scale, int dtype, void* out, float* lse, void* ws,
+                   size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Logit processors: out (fp32 [rows, vocab], contiguous) from logits [rows, vocab] (fp16, bf16 or
+ * fp32, rows `row_stride` elements apart). Column c stands for token vocab_start + c (one rank's
+ * shard of the vocabulary). Row r's history is the first total_lens[r] tokens of
+ * tokens[row_seq[r]] (row_seq NULL: r), of which the first prompt_lens[r] are the prompt: rows of
+ * one request share a history and see it up to their own drafted tokens.
+ * In this order, in fp32, with n = occurrences of the token behind the prompt:
+ *   token anywhere in the history:  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   n > 0:                          x = x - frequency[r] * n - presence[r]
+ *   biases (n_bias per row; id < 0 is unused; entries of one token add up):  x = x + bias
+ *   bit (token & 31) of mask[r * mask_stride + token / 32] clear:            x = -inf
+ * repetition, frequency, presence, biases and mask may be NULL. tokens holds int32, or int64 when
+ * tokens_64 is non-zero, rows tokens_stride apart; ids outside the shard are skipped, a row_seq
+ * outside [0, n_seqs) means no history. At most 2^20 - 1 tokens of history and 2047 biases a row.
+ * `out` may be `logits` where those are fp32 and contiguous. Results do not depend on timing.
+ * ---------------------------------------------------------------------------------------- */
+int b2_logits_process(const void* logits, int64_t row_stride, int dtype, float* out, int rows,
+                      int vocab, int vocab_start, const void* tokens, int tokens_64,
+                      int64_t tokens_stride, int n_seqs, int max_tokens, const int32_t* row_seq,
+                      const int32_t* prompt_lens, const int32_t* total_lens,
+                      const float* repetition, const float* frequency, const float* presence,
+                      const int32_t* bias_ids, const float* bias_values, int n_bias,
+                      const uint32_t* mask, int64_t mask_stride, int mask_words, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Tuning (process-wide; for measurement sweeps). B2_TUNE="key=value,..." in the environment

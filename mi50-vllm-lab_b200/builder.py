@@ -31,7 +31,8 @@ CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-CU_SOURCES = ["b2_runtime.cu", "b2_gemm_f16.cu", "b2_w4.cu", "b2_nvar.cu"]
+CU_SOURCES = ["b2_runtime.cu", "b2_gemm_f16.cu", "b2_w4.cu", "b2_nvar.cu", "b2_rope.cu",
+              "b2_attn.cu", "b2_logits.cu"]
 HEADERS = ["b2_device.cuh", "b2_internal.h", "b2_nvar.cuh"]
 
 CAPI_LIB = HERE / "libb2skinny.so"

@@ -25,6 +25,7 @@ B2_ERR_TIMEOUT = 5
 B2_ERR_STATE = 6
 B2_DTYPE_F16 = 0
 B2_DTYPE_F32 = 1
+B2_DTYPE_BF16 = 2
 B2_BLOB_BYTES = 64
 B2_TUNE_CTAS_PER_SM = 1
 B2_TUNE_MIN_UNITS = 2
@@ -38,6 +39,8 @@ B2_TUNE_NORM_NO_COOP = 9
 B2_TUNE_NORM_IN_LAUNCH = 10
 
 _vp, _i, _sz, _u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
+_i64, _f = C.c_int64, C.c_float
+_strides = C.POINTER(_i64)
 _SIGS = {
     "b2_status_string": (C.c_char_p, [_i]),
     "b2_last_error": (C.c_char_p, []),
@@ -81,6 +84,16 @@ _SIGS = {
                                            C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),
                                            C.POINTER(_vp), C.c_float, C.POINTER(_vp), _i, _i, _i,
                                            _i, C.POINTER(_vp), _sz, _vp]),
+    "b2_rope": (_i, [_vp, _strides, _vp, _strides, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f,
+                     _i, _i, _vp]),
+    "b2_rope_cache": (_i, [_vp, _strides, _vp, _strides, _vp, _strides, _vp, _i, _vp, _vp, _vp, _vp,
+                           _strides, _vp, _strides, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp]),
+    "b2_prefix_attn_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "b2_prefix_attn": (_i, [_vp, _strides, _vp, _strides, _vp, _strides, _i, _i, _vp, _i, _vp, _vp,
+                            _i64, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _sz,
+                            _vp]),
+    "b2_logits_process": (_i, [_vp, _i64, _i, _vp, _i, _i, _i, _vp, _i, _i64, _i, _i, _vp, _vp, _vp,
+                               _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
     "b2_set_tuning": (_i, [_i, _i]),
     "b2_get_tuning": (_i, [_i]),
     "b2_w4_plan": (_i, [_i, _i, _i, _i, _i, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),
@@ -133,6 +146,11 @@ def w4_plan(M: int, K: int, N: int, G: int, fused: bool = False) -> dict:
                            C.byref(ctas)), "b2_w4_plan")
     kernel = "w4c_kernel" if path.value == 2 else "w4_kernel"
     return {"kernel": kernel, "path": path.value, "cluster": cs.value, "ctas": ctas.value}
+
+
+def strides(*values: int) -> "C.Array":
+    """A C array of int64 strides in elements (for the entry points that take strided tensors)."""
+    return (_i64 * len(values))(*values)
 
 
 def ptr_array(ptrs) -> "C.Array":

@@ -21,7 +21,9 @@
 #include <torch/library.h>
 
 #include <mutex>
+#include <optional>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "b2_skinny.h"
@@ -405,6 +407,334 @@ at::Tensor w4gemm_ar_rmsnorm_packed(const at::Tensor& a, const at::Tensor& packe
   return y;
 }
 
+// ------------------------------------------------------------------------------------------------
+// What a verify step runs between its products (no counterpart in the reference's library):
+// rope, rope_cache, prefix_attn, logits_process.
+// ------------------------------------------------------------------------------------------------
+int dtype_code(const at::Tensor& t, const char* op, const char* name, bool f32) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return B2_DTYPE_F16;
+    case at::kBFloat16: return B2_DTYPE_BF16;
+    case at::kFloat:
+      if (f32) return B2_DTYPE_F32;
+      break;
+    default: break;
+  }
+  TORCH_CHECK(false, op, ": ", name, " must be float16", f32 ? ", bfloat16 or float32" : " or bfloat16",
+              "; got ", t.scalar_type());
+}
+
+// A tensor of type `type` on the same device as `like`.
+void check_like(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, const char* op,
+                const char* name) {
+  TORCH_CHECK(t.device() == like.device(), op, ": ", name, " must be on ", like.device(), "; got ",
+              t.device());
+  TORCH_CHECK(t.scalar_type() == type, op, ": ", name, " must be ", type, "; got ", t.scalar_type());
+}
+
+// The stride of dimension `dim`; a dimension of one element has any.
+int64_t stride_of(const at::Tensor& t, int64_t dim, int64_t dense) {
+  return t.size(dim) <= 1 ? dense : t.stride(dim);
+}
+
+struct Heads {  // [rows, heads, dim] with contiguous dim
+  int64_t rows, heads, dim, strides[2];
+};
+Heads check_heads(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 3, op, ": ", name, " must be [rows, heads, head_dim]; got ", t.sizes());
+  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, op, ": ", name, " must be contiguous in its last dimension");
+  const int64_t d = t.size(2), h = t.size(1);
+  TORCH_CHECK(t.size(0) <= INT32_MAX && h >= 1 && h <= 65536 && d >= 1 && d <= 65536, op, ": ", name,
+              " has sizes ", t.sizes());
+  return {t.size(0), h, d, {stride_of(t, 0, h * d), stride_of(t, 1, d)}};
+}
+
+struct Cache {  // [pages, page_size, heads, dim] with contiguous dim
+  int64_t strides[3];
+};
+Cache check_cache(const at::Tensor& t, const at::Tensor& like, int64_t heads, int64_t dim,
+                  const char* op, const char* name) {
+  check_like(t, like, like.scalar_type(), op, name);
+  TORCH_CHECK(t.dim() == 4 && t.size(2) == heads && t.size(3) == dim, op, ": ", name,
+              " must be [pages, page_size, ", heads, ", ", dim, "]; got ", t.sizes());
+  TORCH_CHECK(t.size(0) >= 1 && t.size(0) <= INT32_MAX && t.size(1) >= 1 && t.size(1) <= INT32_MAX, op,
+              ": ", name, " has sizes ", t.sizes());
+  TORCH_CHECK(dim <= 1 || t.stride(3) == 1, op, ": ", name, " must be contiguous in its last dimension");
+  return {{stride_of(t, 0, t.size(1) * heads * dim), stride_of(t, 1, heads * dim), stride_of(t, 2, dim)}};
+}
+
+// The arguments that rope and rope_cache share.
+struct Rope {
+  Heads q, k;
+  int dtype, pos64, rot;
+};
+Rope check_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                const at::Tensor& inv_freq, const char* op) {
+  Rope r;
+  r.q = check_heads(q, op, "q");
+  r.k = check_heads(k, op, "k");
+  r.dtype = dtype_code(q, op, "q", true);
+  check_like(k, q, q.scalar_type(), op, "k");
+  TORCH_CHECK(r.k.rows == r.q.rows && r.k.dim == r.q.dim, op, ": q ", q.sizes(), " and k ", k.sizes(),
+              " differ in rows or head_dim");
+  TORCH_CHECK(positions.device() == q.device() && positions.dim() == 1 &&
+                  positions.size(0) == r.q.rows && positions.is_contiguous() &&
+                  (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong),
+              op, ": positions must be contiguous int32 or int64 [", r.q.rows, "] on ", q.device());
+  r.pos64 = positions.scalar_type() == at::kLong;
+  check_like(inv_freq, q, at::kFloat, op, "inv_freq");
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.is_contiguous() && inv_freq.numel() >= 1 &&
+                  2 * inv_freq.numel() <= r.q.dim,
+              op, ": inv_freq must be contiguous float32 [rot_dim / 2] with rot_dim <= ", r.q.dim,
+              "; got ", inv_freq.sizes());
+  r.rot = (int)(2 * inv_freq.numel());
+  return r;
+}
+
+std::tuple<at::Tensor, at::Tensor> rope(const at::Tensor& q, const at::Tensor& k,
+                                        const at::Tensor& positions, const at::Tensor& inv_freq,
+                                        double scale, bool interleaved) {
+  const Rope r = check_rope(q, k, positions, inv_freq, "rope");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto q_out = at::empty(q.sizes(), q.options());
+  auto k_out = at::empty(k.sizes(), k.options());
+  const int rc = b2_rope(q.data_ptr(), r.q.strides, k.data_ptr(), r.k.strides, positions.data_ptr(),
+                         r.pos64, inv_freq.data_ptr<float>(), q_out.data_ptr(), k_out.data_ptr(),
+                         (int)r.q.rows, (int)r.q.heads, (int)r.k.heads, (int)r.q.dim, r.rot,
+                         (float)scale, interleaved ? 1 : 0, r.dtype,
+                         c10::cuda::getCurrentCUDAStream(q.get_device()).stream());
+  TORCH_CHECK(rc == B2_OK, "gfx906_skinny.rope: ", detail(rc));
+  return {q_out, k_out};
+}
+
+std::tuple<at::Tensor, at::Tensor> rope_meta(const at::Tensor& q, const at::Tensor& k,
+                                             const at::Tensor& positions, const at::Tensor& inv_freq,
+                                             double scale, bool interleaved) {
+  (void)positions, (void)inv_freq, (void)scale, (void)interleaved;
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
+}
+
+at::Tensor rope_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                      const at::Tensor& positions, const at::Tensor& inv_freq,
+                      const at::Tensor& slots, at::Tensor& k_cache, at::Tensor& v_cache, double scale,
+                      bool interleaved) {
+  const char* op = "rope_cache";
+  const Rope r = check_rope(q, k, positions, inv_freq, op);
+  const Heads hv = check_heads(v, op, "v");
+  check_like(v, q, q.scalar_type(), op, "v");
+  TORCH_CHECK(v.sizes() == k.sizes(), op, ": k ", k.sizes(), " and v ", v.sizes(), " differ");
+  check_like(slots, q, at::kLong, op, "slots");
+  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == r.q.rows && slots.is_contiguous(), op,
+              ": slots must be contiguous [", r.q.rows, "]; got ", slots.sizes());
+  const Cache kc = check_cache(k_cache, q, r.k.heads, r.k.dim, op, "k_cache");
+  const Cache vc = check_cache(v_cache, q, r.k.heads, r.k.dim, op, "v_cache");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), op, ": caches of sizes ", k_cache.sizes(), " and ",
+              v_cache.sizes());
+  c10::cuda::CUDAGuard guard(q.device());
+  auto q_out = at::empty(q.sizes(), q.options());
+  const int rc = b2_rope_cache(
+      q.data_ptr(), r.q.strides, k.data_ptr(), r.k.strides, v.data_ptr(), hv.strides,
+      positions.data_ptr(), r.pos64, inv_freq.data_ptr<float>(), slots.data_ptr<int64_t>(),
+      q_out.data_ptr(), k_cache.data_ptr(), kc.strides, v_cache.data_ptr(), vc.strides,
+      (int)k_cache.size(0), (int)k_cache.size(1), (int)r.q.rows, (int)r.q.heads, (int)r.k.heads,
+      (int)r.q.dim, r.rot, (float)scale, interleaved ? 1 : 0, r.dtype,
+      c10::cuda::getCurrentCUDAStream(q.get_device()).stream());
+  TORCH_CHECK(rc == B2_OK, "gfx906_skinny.rope_cache: ", detail(rc));
+  return q_out;
+}
+
+at::Tensor rope_cache_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                           const at::Tensor& positions, const at::Tensor& inv_freq,
+                           const at::Tensor& slots, at::Tensor& k_cache, at::Tensor& v_cache,
+                           double scale, bool interleaved) {
+  (void)k, (void)v, (void)positions, (void)inv_freq, (void)slots, (void)k_cache, (void)v_cache;
+  (void)scale, (void)interleaved;
+  return at::empty(q.sizes(), q.options());
+}
+
+// A contiguous one-dimensional int32 tensor of `n` elements.
+const int32_t* check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* op,
+                          const char* name) {
+  check_like(t, like, at::kInt, op, name);
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), op, ": ", name,
+              " must be contiguous int32 [", n, "]; got ", t.sizes());
+  return t.data_ptr<int32_t>();
+}
+
+std::tuple<at::Tensor, at::Tensor> prefix_attn(const at::Tensor& q, const at::Tensor& k_cache,
+                                               const at::Tensor& v_cache,
+                                               const at::Tensor& prefix_pages,
+                                               const at::Tensor& prefix_len, const at::Tensor& pages,
+                                               const at::Tensor& own_lens, const at::Tensor& row_start,
+                                               double scale, const std::optional<at::Tensor>& tree) {
+  const char* op = "prefix_attn";
+  const Heads h = check_heads(q, op, "q");
+  const int dt = dtype_code(q, op, "q", false);
+  TORCH_CHECK(k_cache.dim() == 4, op, ": k_cache must be [pages, page_size, kv_heads, head_dim]; got ",
+              k_cache.sizes());
+  const int64_t hk = k_cache.size(2);
+  TORCH_CHECK(hk >= 1 && h.heads % hk == 0, op, ": ", h.heads, " query heads on ", hk, " KV heads");
+  const Cache kc = check_cache(k_cache, q, hk, h.dim, op, "k_cache");
+  const Cache vc = check_cache(v_cache, q, hk, h.dim, op, "v_cache");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), op, ": caches of sizes ", k_cache.sizes(), " and ",
+              v_cache.sizes());
+  check_like(pages, q, at::kInt, op, "pages");
+  TORCH_CHECK(pages.dim() == 2 && (pages.size(1) <= 1 || pages.stride(1) == 1), op,
+              ": pages must be int32 [requests, max_pages], contiguous in its last dimension; got ",
+              pages.sizes());
+  const int64_t b = pages.size(0);
+  TORCH_CHECK(b <= INT32_MAX && pages.size(1) <= INT32_MAX, op, ": pages has sizes ", pages.sizes());
+  TORCH_CHECK(prefix_pages.dim() == 1 && prefix_pages.size(0) <= INT32_MAX, op,
+              ": prefix_pages must be one-dimensional; got ", prefix_pages.sizes());
+  const int32_t* pp = check_ints(prefix_pages, q, prefix_pages.size(0), op, "prefix_pages");
+  const int32_t* pl = check_ints(prefix_len, q, 1, op, "prefix_len");
+  const int32_t* ol = check_ints(own_lens, q, b, op, "own_lens");
+  const int32_t* rs = check_ints(row_start, q, b + 1, op, "row_start");
+  const int64_t* tr = nullptr;
+  if (tree.has_value()) {
+    check_like(*tree, q, at::kLong, op, "tree");
+    TORCH_CHECK(tree->dim() == 1 && tree->size(0) == h.rows && tree->is_contiguous(), op,
+                ": tree must be contiguous int64 [", h.rows, "]; got ", tree->sizes());
+    tr = tree->data_ptr<int64_t>();
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  auto out = at::empty(q.sizes(), q.options());
+  auto lse = at::empty({h.rows, h.heads}, q.options().dtype(at::kFloat));
+  if (h.rows == 0) return {out, lse};
+  const size_t bytes = b2_prefix_attn_workspace((int)b, (int)h.rows, (int)h.heads, (int)hk, (int)h.dim);
+  TORCH_CHECK(bytes > 0, "gfx906_skinny.prefix_attn: ", b2_last_error());
+  // The workspace comes from torch's allocator: it belongs to this stream, or to the graph that is
+  // being captured, so calls on two streams and two graphs share nothing.
+  auto ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  const int rc = b2_prefix_attn(
+      q.data_ptr(), h.strides, k_cache.data_ptr(), kc.strides, v_cache.data_ptr(), vc.strides,
+      (int)k_cache.size(0), (int)k_cache.size(1), pp, (int)prefix_pages.size(0), pl,
+      pages.data_ptr<int32_t>(), stride_of(pages, 0, pages.size(1)), (int)pages.size(1), ol, rs, tr,
+      (int)b, (int)h.rows, (int)h.heads, (int)hk, (int)h.dim, (float)scale, dt, out.data_ptr(),
+      lse.data_ptr<float>(), ws.data_ptr(), bytes,
+      c10::cuda::getCurrentCUDAStream(q.get_device()).stream());
+  TORCH_CHECK(rc == B2_OK, "gfx906_skinny.prefix_attn: ", detail(rc));
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> prefix_attn_meta(
+    const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& prefix_pages, const at::Tensor& prefix_len, const at::Tensor& pages,
+    const at::Tensor& own_lens, const at::Tensor& row_start, double scale,
+    const std::optional<at::Tensor>& tree) {
+  (void)k_cache, (void)v_cache, (void)prefix_pages, (void)prefix_len, (void)pages, (void)own_lens;
+  (void)row_start, (void)scale, (void)tree;
+  return {at::empty(q.sizes(), q.options()),
+          at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
+}
+
+// A row parameter of logits_process: contiguous [rows], or nothing.
+template <typename T>
+const T* row_parameter(const std::optional<at::Tensor>& t, const at::Tensor& like, at::ScalarType type,
+                       const char* op, const char* name) {
+  if (!t.has_value()) return nullptr;
+  check_like(*t, like, type, op, name);
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == like.size(0) && t->is_contiguous(), op, ": ", name,
+              " must be contiguous [", like.size(0), "]; got ", t->sizes());
+  return t->data_ptr<T>();
+}
+
+at::Tensor logits_process(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                          const std::optional<at::Tensor>& row_seq,
+                          const std::optional<at::Tensor>& prompt_lens,
+                          const std::optional<at::Tensor>& total_lens,
+                          const std::optional<at::Tensor>& repetition,
+                          const std::optional<at::Tensor>& frequency,
+                          const std::optional<at::Tensor>& presence,
+                          const std::optional<at::Tensor>& bias_ids,
+                          const std::optional<at::Tensor>& bias_values,
+                          const std::optional<at::Tensor>& mask, int64_t vocab_start) {
+  const char* op = "logits_process";
+  TORCH_CHECK(logits.is_cuda(), op, ": logits must be a CUDA tensor");
+  const int dt = dtype_code(logits, op, "logits", true);
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(0) <= INT32_MAX &&
+                  logits.size(1) <= INT32_MAX,
+              op, ": logits must be [rows, vocab]; got ", logits.sizes());
+  TORCH_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, op,
+              ": logits must be contiguous in their last dimension");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  TORCH_CHECK(vocab_start >= 0 && vocab_start <= INT32_MAX, op, ": vocab_start=", vocab_start);
+  const void* tok = nullptr;
+  int tok64 = 0;
+  int64_t tok_stride = 0, seqs = 0, most = 0;
+  if (tokens.has_value()) {
+    TORCH_CHECK(tokens->device() == logits.device() && tokens->dim() == 2 &&
+                    (tokens->scalar_type() == at::kInt || tokens->scalar_type() == at::kLong) &&
+                    (tokens->size(1) <= 1 || tokens->stride(1) == 1),
+                op, ": tokens must be int32 or int64 [requests, length] on ", logits.device(),
+                ", contiguous in its last dimension");
+    seqs = tokens->size(0), most = tokens->size(1);
+    TORCH_CHECK(seqs <= INT32_MAX && most <= INT32_MAX, op, ": tokens has sizes ", tokens->sizes());
+    tok64 = tokens->scalar_type() == at::kLong;
+    tok_stride = stride_of(*tokens, 0, most);
+    tok = tokens->data_ptr();
+    TORCH_CHECK(prompt_lens.has_value() && total_lens.has_value(), op,
+                ": tokens need prompt_lens and total_lens");
+    TORCH_CHECK(row_seq.has_value() || seqs >= rows, op, ": ", seqs, " histories for ", rows,
+                " rows and no row_seq");
+  } else {
+    TORCH_CHECK(!repetition.has_value() && !frequency.has_value() && !presence.has_value(), op,
+                ": penalties need tokens, prompt_lens and total_lens");
+  }
+  const int32_t* seq = row_parameter<int32_t>(row_seq, logits, at::kInt, op, "row_seq");
+  const int32_t* prompt = row_parameter<int32_t>(prompt_lens, logits, at::kInt, op, "prompt_lens");
+  const int32_t* total = row_parameter<int32_t>(total_lens, logits, at::kInt, op, "total_lens");
+  const float* rep = row_parameter<float>(repetition, logits, at::kFloat, op, "repetition");
+  const float* freq = row_parameter<float>(frequency, logits, at::kFloat, op, "frequency");
+  const float* pres = row_parameter<float>(presence, logits, at::kFloat, op, "presence");
+  TORCH_CHECK(bias_ids.has_value() == bias_values.has_value(), op,
+              ": bias_ids and bias_values come together");
+  int64_t n_bias = 0;
+  if (bias_ids.has_value()) {
+    check_like(*bias_ids, logits, at::kInt, op, "bias_ids");
+    check_like(*bias_values, logits, at::kFloat, op, "bias_values");
+    TORCH_CHECK(bias_ids->dim() == 2 && bias_ids->size(0) == rows && bias_ids->is_contiguous() &&
+                    bias_values->sizes() == bias_ids->sizes() && bias_values->is_contiguous(),
+                op, ": bias_ids and bias_values must be contiguous [", rows, ", biases]; got ",
+                bias_ids->sizes(), " and ", bias_values->sizes());
+    n_bias = bias_ids->size(1);
+    TORCH_CHECK(n_bias <= 2047, op, ": ", n_bias, " biases per row (at most 2047)");
+  }
+  const uint32_t* words = nullptr;
+  int64_t mask_stride = 0, mask_words = 0;
+  if (mask.has_value()) {
+    check_like(*mask, logits, at::kInt, op, "mask");
+    TORCH_CHECK(mask->dim() == 2 && mask->size(0) == rows && (mask->size(1) <= 1 || mask->stride(1) == 1),
+                op, ": mask must be int32 [", rows, ", words], contiguous in its last dimension; got ",
+                mask->sizes());
+    mask_words = mask->size(1);
+    TORCH_CHECK(mask_words <= INT32_MAX && mask_words * 32 >= vocab_start + vocab, op, ": mask of ",
+                mask_words, " words for tokens up to ", vocab_start + vocab);
+    mask_stride = stride_of(*mask, 0, mask_words);
+    words = reinterpret_cast<const uint32_t*>(mask->data_ptr<int32_t>());
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto out = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));
+  const int rc = b2_logits_process(
+      logits.data_ptr(), stride_of(logits, 0, vocab), dt, out.data_ptr<float>(), (int)rows, (int)vocab,
+      (int)vocab_start, tok, tok64, tok_stride, (int)seqs, (int)most, seq, prompt, total, rep, freq,
+      pres, n_bias ? bias_ids->data_ptr<int32_t>() : nullptr,
+      n_bias ? bias_values->data_ptr<float>() : nullptr, (int)n_bias, words, mask_stride,
+      (int)mask_words, c10::cuda::getCurrentCUDAStream(logits.get_device()).stream());
+  TORCH_CHECK(rc == B2_OK, "gfx906_skinny.logits_process: ", detail(rc));
+  return out;
+}
+
+at::Tensor logits_process_meta(const at::Tensor& logits, const std::optional<at::Tensor>&,
+                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+                               const std::optional<at::Tensor>&, int64_t) {
+  return at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
+}
+
 int64_t nvar_status(int64_t handle, bool clear) {
   ArEntry* e;
   {
@@ -463,6 +793,17 @@ TORCH_LIBRARY(gfx906_skinny, m) {
   m.def("w4gemm_ar_packed(Tensor a, Tensor packed, int N, int group_size, int handle) -> Tensor");
   m.def("w4gemm_ar_rmsnorm_packed(Tensor a, Tensor packed, int N, int group_size, int handle, "
         "Tensor(a!) residual, Tensor weight, float eps) -> Tensor");
+  m.def("rope(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, float scale=1.0, "
+        "bool interleaved=False) -> (Tensor, Tensor)");
+  m.def("rope_cache(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor inv_freq, Tensor slots, "
+        "Tensor(a!) k_cache, Tensor(b!) v_cache, float scale=1.0, bool interleaved=False) -> Tensor");
+  m.def("prefix_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_pages, "
+        "Tensor prefix_len, Tensor pages, Tensor own_lens, Tensor row_start, float scale, "
+        "Tensor? tree=None) -> (Tensor, Tensor)");
+  m.def("logits_process(Tensor logits, Tensor? tokens=None, Tensor? row_seq=None, "
+        "Tensor? prompt_lens=None, Tensor? total_lens=None, Tensor? repetition=None, "
+        "Tensor? frequency=None, Tensor? presence=None, Tensor? bias_ids=None, "
+        "Tensor? bias_values=None, Tensor? mask=None, int vocab_start=0) -> Tensor");
   m.def("nvar_status(int handle, bool clear=False) -> int");
   m.def("nvar_set_timeout_ms(int handle, int ms) -> ()");
   m.def("workspace_status(bool clear=False) -> int");
@@ -480,6 +821,10 @@ TORCH_LIBRARY_IMPL(gfx906_skinny, CUDA, m) {
   m.impl("w4gemm_ar_rmsnorm", &w4gemm_ar_rmsnorm);
   m.impl("w4gemm_ar_packed", &w4gemm_ar_packed);
   m.impl("w4gemm_ar_rmsnorm_packed", &w4gemm_ar_rmsnorm_packed);
+  m.impl("rope", &rope);
+  m.impl("rope_cache", &rope_cache);
+  m.impl("prefix_attn", &prefix_attn);
+  m.impl("logits_process", &logits_process);
 }
 
 TORCH_LIBRARY_IMPL(gfx906_skinny, Meta, m) {
@@ -487,6 +832,10 @@ TORCH_LIBRARY_IMPL(gfx906_skinny, Meta, m) {
   m.impl("w4gemm", &w4_gemm_meta);
   m.impl("w4_repack", &w4_repack_meta);
   m.impl("w4gemm_packed", &w4_gemm_packed_meta);
+  m.impl("rope", &rope_meta);
+  m.impl("rope_cache", &rope_cache_meta);
+  m.impl("prefix_attn", &prefix_attn_meta);
+  m.impl("logits_process", &logits_process_meta);
 }
 
 TORCH_LIBRARY_IMPL(gfx906_skinny, CompositeExplicitAutograd, m) {

@@ -7,6 +7,9 @@ check and to time its kernels:
   kernels/check_w4.py:11-21, the fp16 GEMM reference of kernels/bench_skinny.py:44, the fixed
   rank-order all-reduce of kernels/hostar.cu:107, seeded input generators for the configurations
   of the benchmark, and the tolerance check.
+* ``step_oracle``: the operators between a verify step's products (rotary positions, cache write,
+  attention on a shared prefix, logit processors) in 64 bits, with error bounds for their kernels;
+  these have no counterpart on the reference's skinny-GEMM path.
 * ``cpu_baseline``: the reference's torch dequantize-then-matmul on the host cores, timed.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` / ``--impl reference`` legs of
