@@ -29,8 +29,10 @@ namespace {
 
 constexpr int kMaxRequests = 1024;
 constexpr int kMaxRows = 4096;
-constexpr int kAttnWarps = 8;
-constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kSoftWarps = 4;      // one thread per row of a block
+constexpr int kLoadThreads = 128;
+constexpr int kAttnThreads = kSoftWarps * 32 + 32 + kLoadThreads;
+constexpr int kBlockRows = 128;
 constexpr int kJoinThreads = 128;
 constexpr int kMaxCtas = 160;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -50,6 +52,7 @@ struct AttnArgs {
   int total_pages, page_size, n_prefix_pages, max_pages;
   int requests, rows, q_heads, kv_heads, group, dim;
   int slots;
+  int q_vec;  // queries allow 16-byte loads
   float scale_log2;
 };
 
@@ -65,28 +68,19 @@ struct Pair;
 template <>
 struct Pair<__half> {
   static constexpr uint32_t kExp = 0x7c00u;  // exponent bits: all set in infinities and NaN
+  static constexpr uint32_t kFormat = 0;     // operand format of the instruction descriptor
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    mma_16816(c, a[0], a[1], a[2], a[3], b0, b1);
   }
 };
 template <>
 struct Pair<__nv_bfloat16> {
   static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr uint32_t kFormat = 1;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
@@ -101,38 +95,90 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   constexpr uint32_t e = Pair<T>::kExp;
   return ((w & e) == e ? 0u : w & 0xffffu) | (((w >> 16) & e) == e ? 0u : w & 0xffff0000u);
 }
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
 // 16 bytes from global to shared memory; `bytes` = 16, or 0 to write zeros without reading.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One arrival on `bar` once this thread's copies so far have landed (counted in its init).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------------------
+// tcgen05: one CTA, accumulators and the A operand in tensor memory, B in 128-byte-swizzled shared
+// memory. Addresses: lane << 16 | column.
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)),
+               "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns)
+               : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Arrive on `bar` when every tcgen05.mma this thread has issued has completed.
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(bar))
+               : "memory");
+}
+// D[128, N] (+)= A[128, 16] B[16, N]: A in tensor memory, B through a shared-memory descriptor.
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc,
+                                       bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// Shared-memory descriptor, 128-byte swizzle; byte offsets between repeats of the 8-row pattern.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(leading >> 4) << 16 |
+         (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: fp32 accumulator, M = 128, N columns, B with K or N contiguous.
+template <typename T>
+__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_n_major) {
+  return 1u << 4 | Pair<T>::kFormat << 7 | Pair<T>::kFormat << 10 | (b_n_major ? 1u << 16 : 0u) |
+         (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+// 32 columns of this warp's 32 lanes, one lane per thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -141,7 +187,7 @@ __device__ __forceinline__ void cp_async_wait() {
 struct Plan {
   int units_end[kMaxRequests + 1];   // running sum of units up to and with segment s
   int groups_end[kMaxRequests + 1];  // running sum of groups
-  int warp_sum[2][kAttnWarps];
+  int warp_sum[2][kAttnThreads / 32];
 };
 
 // Rows [first, first + count) of a request, and how many of its own tokens are stored.
@@ -252,359 +298,481 @@ struct Cursor {
 };
 
 // ------------------------------------------------------------------------------------------------
-// Main kernel. kDim: head dimension rounded up (64, 128, 256). kRowWarps groups of 16 rows; the
-// other kAttnWarps / kRowWarps warps split a tile's tokens, each with its own running maximum and
-// sum, and are joined at the end of a piece.
+// Main kernel. kDim: head dimension rounded up (64, 128, 256), the rest of it zero.
+//
+// Per tile: S[128 rows, kTok] = Q K^T and O[128 rows, kDim] += P V on the tensor cores, with Q, S,
+// P and O in tensor memory (P takes the place of its S), K and V in a ring of shared-memory stages.
+// K is the product's B operand with the dimension contiguous, V its B operand with N contiguous:
+// both lie as loaded, [token][64 dimensions] rows of 128 bytes, swizzled.
+//   warps 0-3  softmax: a thread owns a row (its lane of tensor memory), so the running maximum and
+//              sum need no exchange between threads; they also bring Q in and take O out
+//   warp 4     one thread issues the products: those of tile i + 1 before tile i's second one, so
+//              that the tensor cores work while the softmax of tile i runs
+//   warps 5-8  copy K and V, 16 bytes per cp.async, page by page, for any page size and strides
+// O is rescaled only when a row's maximum has grown by more than 2^8 over the one its weights refer
+// to (the weights stay below 2^8, in range of fp16, with the same relative rounding); the sum l and
+// the partial refer to the same maximum, so nothing is approximated.
 // ------------------------------------------------------------------------------------------------
 template <int kDim>
 struct Shape {
   static constexpr int kTok = kDim == 64 ? 128 : 64;  // tokens per tile
   static constexpr int kStages = kDim == 256 ? 3 : 6;
-  static constexpr int kHalfBytes = kTok * kDim * 2;  // K or V of a stage
-  static constexpr int kRing = kStages * 2 * kHalfBytes;
-  static constexpr int kJoinCols = 32;  // columns of O joined per round
+  static constexpr int kSub = kTok * 128;              // [token][64 dimensions] of K or V
+  static constexpr int kHalf = kSub * (kDim / 64);     // K or V of a stage
+  static constexpr int kRing = kStages * 2 * kHalf;
+  static constexpr int kS = kDim, kQ = kDim + 2 * kTok;  // columns of tensor memory; O at 0
+  static constexpr int kColumns = 512;
+  static_assert(kQ + kDim / 2 <= kColumns, "tensor memory of an SM");
 };
 
-template <int kDim, int kRowWarps>
+struct Control {
+  uint64_t full[6], empty[6];
+  uint64_t s_full[2], p_full[2], o_done[2], q_full, o_free, sync, drain;
+  uint32_t tmem;
+  int abort;
+  int bad_unit[6];  // per stage: 1 + the unit, if any, for which a page id outside the cache was met
+  int bad_value;    // 1 + the unit for which a value that is no number was met in a masked tile
+  unsigned char bad_token[128];
+};
+
+template <int kDim>
 constexpr size_t attn_smem() {
-  return Shape<kDim>::kRing +
-         sizeof(float) * ((kAttnWarps / kRowWarps) * kRowWarps * 16 * (Shape<kDim>::kJoinCols + 4)) +
-         sizeof(float2) * kAttnWarps * 16 + sizeof(Plan) + 64;
+  return 1024 + Shape<kDim>::kRing + sizeof(Plan) + sizeof(Control) + 16;
 }
 
-template <typename T, int kDim, int kRowWarps>
+__device__ int g_attn_status;
+
+template <typename T, int kDim>
 __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p) {
   using S = Shape<kDim>;
   constexpr int kTok = S::kTok, kStages = S::kStages;
-  constexpr int kTokWarps = kAttnWarps / kRowWarps;
-  constexpr int kWarpTok = kTok / kTokWarps;  // tokens of a tile per warp
-  constexpr int kBlockRows = kRowWarps * 16;
-  constexpr int kChunks = kDim / 8;           // 16-byte chunks per token
-  constexpr int kCols = S::kJoinCols;
-  static_assert(kWarpTok % 16 == 0, "a warp takes whole k-steps of the second product");
-
-  extern __shared__ __align__(128) uint8_t smem[];
-  float* s_join = reinterpret_cast<float*>(smem + S::kRing);  // [tokwarp][row][kCols + 4]
-  float2* s_ml = reinterpret_cast<float2*>(s_join + kTokWarps * kBlockRows * (kCols + 4));
-  Plan& plan = *reinterpret_cast<Plan*>(s_ml + kAttnWarps * 16);
-  // per stage: 1 + the unit, if any, for which a page id outside the cache was met there
-  volatile int* s_bad = reinterpret_cast<volatile int*>(&plan + 1);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  Control& c = *reinterpret_cast<Control*>(smem + S::kRing);
+  Plan& plan = *reinterpret_cast<Plan*>((reinterpret_cast<uintptr_t>(&c + 1) + 15) & ~(uintptr_t)15);
+  volatile int* s_abort = &c.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rw = warp % kRowWarps, tw = warp / kRowWarps;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&c.full[s], kLoadThreads + kLoadThreads / 32);
+      mbar_init(&c.empty[s], 1);
+      c.bad_unit[s] = 0;
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&c.s_full[b], 1);
+      mbar_init(&c.p_full[b], kSoftWarps);
+      mbar_init(&c.o_done[b], 1);
+    }
+    mbar_init(&c.q_full, kSoftWarps);
+    mbar_init(&c.o_free, kSoftWarps);
+    mbar_init(&c.sync, kSoftWarps);
+    mbar_init(&c.drain, 1);
+    c.abort = 0;
+    c.bad_value = 0;
+    mbar_fence_init();
+  }
+  if (warp == kSoftWarps) tmem_alloc(&c.tmem, S::kColumns);
   grid_dep_wait();
   grid_dep_launch();
-  make_plan<kAttnWarps>(p, kTok, kBlockRows, plan);
+  make_plan<kAttnThreads / 32>(p, kTok, kBlockRows, plan);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = c.tmem;
   const int units = plan.units_end[p.requests];
-  if (units == 0) return;
   const int ctas = plan_ctas(units, gridDim.x);
-  if ((int)blockIdx.x >= ctas) return;
-  const int u_lo = plan_begin(units, ctas, blockIdx.x), u_hi = plan_begin(units, ctas, blockIdx.x + 1);
-
+  const bool idle = (int)blockIdx.x >= ctas;
+  const int u_lo = idle ? 0 : plan_begin(units, ctas, blockIdx.x);
+  const int u_hi = idle ? 0 : plan_begin(units, ctas, blockIdx.x + 1);
   const uint32_t ring = smem_u32(smem);
-  const T* kc = static_cast<const T*>(p.k);
-  const T* vc = static_cast<const T*>(p.v);
+  const int stage_bytes = 2 * S::kHalf;
 
-  // ---- loads: this thread's chunk column and rows of every tile
-  Cursor lc;
-  lc.seek(p, plan, u_lo, kTok, kBlockRows);
-  int lu = u_lo;
-  const int chunk = threadIdx.x % kChunks;
-  const bool chunk_in = chunk * 8 < p.dim;
-  auto fill = [&](int stage) {
-    if (lu < u_hi) {
-      const int head = lc.group / lc.blocks;
-      const int32_t* table = lc.seg ? p.pages + (int64_t)(lc.seg - 1) * p.pages_stride : p.prefix_pages;
-      const uint32_t kb = ring + stage * 2 * S::kHalfBytes, vb = kb + S::kHalfBytes;
-#pragma unroll
-      for (int i = 0; i < kTok / (kAttnThreads / kChunks); ++i) {
-        const int r = threadIdx.x / kChunks + i * (kAttnThreads / kChunks);
-        const int tok = lc.tile * kTok + r;
-        const T *ks = kc, *vs = vc;
-        int bytes = 0;
-        if (tok < lc.len) {
-          const int pg = tok / p.page_size;
-          const int id = table[pg];
-          if (id >= 0 && id < p.total_pages) {
-            const int at = tok - pg * p.page_size;
-            ks = kc + id * p.ks[0] + at * p.ks[1] + head * p.ks[2] + chunk * 8;
-            vs = vc + id * p.vs[0] + at * p.vs[1] + head * p.vs[2] + chunk * 8;
-            bytes = chunk_in ? 16 : 0;
-          } else {
-            s_bad[stage] = lu + 1;
-          }
-        }
-        if (!bytes) ks = kc, vs = vc;
-        const uint32_t off = r * (kDim * 2) + ((chunk ^ (r & 7)) << 4);
-        cp_async16(kb + off, ks, bytes);
-        cp_async16(vb + off, vs, bytes);
+  Cursor cur;
+  if (!idle) cur.seek(p, plan, u_lo, kTok, kBlockRows);
+
+  if (warp > kSoftWarps) {
+    // ------------------------------------------------------------------------------ loaders
+    constexpr int kChunks = kDim / 8;               // 16-byte chunks per token
+    constexpr int kWarpRows = 32 / kChunks;         // tokens per warp and copy
+    constexpr int kLoadWarps = kLoadThreads / 32;
+    constexpr int kIters = kTok / (kWarpRows * kLoadWarps);
+    const int lw = warp - kSoftWarps - 1;
+    const int chunk = lane % kChunks;
+    const bool chunk_in = chunk * 8 < p.dim;
+    // this lane looks up the page of one of the warp's tokens; shuffles hand it out
+    const int my_row = (lane / kWarpRows) * (kWarpRows * kLoadWarps) + lw * kWarpRows + lane % kWarpRows;
+    auto look_up = [&](int& id, int& at) {
+      id = -1;
+      at = 0;
+      const int tok = cur.tile * kTok + my_row;
+      if (my_row < kTok && tok < cur.len) {
+        const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
+        const int pg = tok / p.page_size;
+        id = table[pg];
+        at = tok - pg * p.page_size;
+        if (id < 0 || id >= p.total_pages) id = -2;
       }
-      lc.next(p, plan, kTok, kBlockRows);
-      ++lu;
+    };
+    int id = -1, at = 0;
+    if (!idle) look_up(id, at);
+    for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
+      const int stage = i % kStages;
+      const int head = cur.group / cur.blocks;
+      const int tile_id = id, tile_at = at;
+      const T* kc = static_cast<const T*>(p.k) + head * p.ks[2] + chunk * 8;
+      const T* vc = static_cast<const T*>(p.v) + head * p.vs[2] + chunk * 8;
+      cur.next(p, plan, kTok, kBlockRows);
+      if (u + 1 < u_hi) look_up(id, at);  // its latency passes behind this tile's wait and copies
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort);
+      ok = __shfl_sync(~0u, ok, 0);
+      if (!ok) break;
+      if (tile_id == -2) c.bad_unit[stage] = u + 1;
+      const uint32_t kb = ring + stage * stage_bytes + (chunk >> 3) * S::kSub;
+#pragma unroll
+      for (int j = 0; j < kIters; ++j) {
+        const int src = j * kWarpRows + lane / kChunks;
+        const int pid = __shfl_sync(~0u, tile_id, src), pat = __shfl_sync(~0u, tile_at, src);
+        const int r = j * (kWarpRows * kLoadWarps) + lw * kWarpRows + lane / kChunks;
+        const bool have = pid >= 0 && chunk_in;
+        const T* ks = have ? kc + pid * p.ks[0] + pat * p.ks[1] : static_cast<const T*>(p.k);
+        const T* vs = have ? vc + pid * p.vs[0] + pat * p.vs[1] : static_cast<const T*>(p.v);
+        const uint32_t dst = kb + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+        cp_async16(dst, ks, have ? 16 : 0);
+        cp_async16(dst + S::kHalf, vs, have ? 16 : 0);
+      }
+      cp_async_arrive(&c.full[stage]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.full[stage]);  // orders bad_unit before the stage is full
     }
-    cp_async_commit();
-  };
-  if (threadIdx.x < kStages) s_bad[threadIdx.x] = 0;
-  __syncthreads();  // the flags are cleared before a fill sets one
+    cp_async_wait_all();
+  } else if (warp == kSoftWarps) {
+    // ------------------------------------------------------------------------------ products
+    if (lane == 0 && !idle) {
+      constexpr uint32_t kIdescS = instr_desc<T>(kTok, false), kIdescO = instr_desc<T>(kDim, true);
+      int pieces = 0;         // pieces whose second product has begun
+      bool first[2] = {};     // tile i (by parity) opens its piece
+      bool ok = true;
+      auto second = [&](int i) {  // O += P V of tile i
+        ok = ok && mbar_wait(&c.p_full[i & 1], (i >> 1) & 1, s_abort);
+        if (first[i & 1]) {
+          if (pieces > 0) ok = ok && mbar_wait(&c.o_free, (pieces - 1) & 1, s_abort);
+          ++pieces;
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t vb = ring + (i % kStages) * stage_bytes + S::kHalf;
+        const uint32_t pa = tmem + S::kS + (i & 1) * kTok;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) fill(s);
-
-  // ---- compute
-  Cursor cc;
-  cc.seek(p, plan, u_lo, kTok, kBlockRows);
-  const int g4 = lane >> 2, t4 = lane & 3;
-  uint32_t qf[kDim / 16][4];
-  float o[kDim / 8][4];
-  float m[2] = {}, l[2] = {};
-  int seen[2] = {};             // tokens of the segment the lane's two rows see
-  unsigned long long branch[2] = {};
-  int base = 0;                 // first new token of the request
-  bool piece_start = true;
-  int stage = 0;
-
-  for (int u = u_lo; u < u_hi; ++u) {
-    const int head = cc.group / cc.blocks, block = cc.group - head * cc.blocks;
-    const int row_lim = cc.count * p.group;  // rows of the segment
-    const int my_rows = row_lim - block * kBlockRows - rw * 16;  // of this warp's 16
-    if (piece_start) {
+        for (int ks = 0; ks < kTok / 16; ++ks)
+          tc_mma(tmem, pa + ks * 8, smem_desc(vb + ks * 2048, S::kSub, 1024), kIdescO,
+                 !(first[i & 1] && ks == 0));
+        tc_commit(&c.empty[i % kStages]);
+        tc_commit(&c.o_done[i & 1]);
+      };
+      int starts = 0;
+      int n = 0;
+      for (int u = u_lo; u < u_hi && ok; ++u, ++n) {
+        const bool start = n == 0 || cur.tile == 0;
+        // A new piece's queries arrive after the last weights of the old one: take those first.
+        if (start && n > 0) second(n - 1);
+        if (start) {
+          ok = ok && mbar_wait(&c.q_full, starts & 1, s_abort);
+          ++starts;
+        }
+        ok = ok && mbar_wait(&c.full[n % kStages], (n / kStages) & 1, s_abort);
+        if (!ok) break;
+        fence_proxy_async_smem();  // the copies wrote through the generic proxy
+        tc_fence_after();
+        const uint32_t kb = ring + (n % kStages) * stage_bytes;
+        const uint32_t sd = tmem + S::kS + (n & 1) * kTok;
 #pragma unroll
-      for (int j = 0; j < kDim / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-      base = cc.len - cc.count;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[e] = neg_inf();
-        l[e] = 0.f;
-        const int r = g4 + 8 * e;
-        const int f = block * kBlockRows + rw * 16 + r;
-        const bool act = r < my_rows;
-        const int local = act ? f / p.group : 0;
-        const int t = cc.first + local;
-        const T* src = static_cast<const T*>(p.q) + t * p.q_row +
+        for (int ks = 0; ks < kDim / 16; ++ks)
+          tc_mma(sd, tmem + S::kQ + ks * 8, smem_desc(kb + (ks / 4) * S::kSub + (ks % 4) * 32, 16, 1024),
+                 kIdescS, ks > 0);
+        tc_commit(&c.s_full[n & 1]);
+        if (!start) second(n - 1);
+        first[n & 1] = start;
+        cur.next(p, plan, kTok, kBlockRows);
+      }
+      if (ok && n > 0) second(n - 1);
+      if (!ok) {  // let what is in flight land before the tensor memory is freed
+        tc_commit(&c.drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_test(&c.drain, 0) && globaltimer_ns() - t0 < kPipeWaitNs) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------------------ softmax
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const uint32_t t_o = tmem + lanes, t_q = tmem + lanes + S::kQ;
+    bool ok = !idle;
+    // The rows of a piece and what they see.
+    int rows_here = 0, base = 0, seen = 0;
+    unsigned long long branch = 0;
+    // Queries of the piece at the cursor into tensor memory.
+    auto open_piece = [&] {
+      const int head = cur.group / cur.blocks, block = cur.group - head * cur.blocks;
+      rows_here = min(kBlockRows, cur.count * p.group - block * kBlockRows);
+      base = cur.len - cur.count;
+      const int f = block * kBlockRows + threadIdx.x;
+      const bool act = (int)threadIdx.x < rows_here;
+      const int local = act ? f / p.group : 0;
+      const int t = cur.first + local;
+      seen = !act ? 0x7fffffff : cur.seg == 0 ? cur.len : min(cur.len, base + local + 1);
+      branch = 0;
+      if (p.tree && cur.seg && act) {
+        branch = (unsigned long long)p.tree[t];
+        seen = min(cur.len, base);
+      }
+      if (warp * 32 < rows_here) {
+        const T* src = static_cast<const T*>(p.q) + (int64_t)t * p.q_row +
                        (int64_t)(head * p.group + (act ? f - local * p.group : 0)) * p.q_head;
-        seen[e] = !act ? 0x7fffffff : cc.seg == 0 ? cc.len : min(cc.len, base + local + 1);
-        branch[e] = 0;
-        if (p.tree && cc.seg && act) {
-          branch[e] = (unsigned long long)p.tree[t];
-          seen[e] = min(cc.len, base);
-        }
 #pragma unroll
-        for (int ks = 0; ks < kDim / 16; ++ks) {
-          const int d = ks * 16 + t4 * 2;
-          qf[ks][e] = act && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-          qf[ks][2 + e] = act && d + 8 < p.dim ? *reinterpret_cast<const uint32_t*>(src + d + 8) : 0u;
+        for (int c0 = 0; c0 < kDim / 2; c0 += 32) {
+          uint32_t w[32];
+          if (p.q_vec) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int d = (c0 + 4 * j) * 2;
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (act && d < p.dim) v = *reinterpret_cast<const uint4*>(src + d);
+              w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int d = (c0 + j) * 2;
+              w[j] = act && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+            }
+          }
+          tmem_st32(t_q + c0, w);
         }
+        tc_wait_st();
       }
-      piece_start = false;
-    }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.q_full);
+    };
+    if (ok) open_piece();
+    // A barrier of the softmax warps whose wait is bounded like the others.
+    int syncs = 0;
+    auto sync_rows = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.sync);
+      ok = mbar_wait(&c.sync, syncs++ & 1, s_abort) && ok;
+      __syncwarp();
+    };
 
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    fill(stage == 0 ? kStages - 1 : stage - 1);  // the stage that every warp has left behind
-
-    if (my_rows > 0) {
-      const uint32_t kb = ring + stage * 2 * S::kHalfBytes, vb = kb + S::kHalfBytes;
-      const int tok0 = tw * kWarpTok;
-      float s[kWarpTok / 8][4];
-#pragma unroll
-      for (int j = 0; j < kWarpTok / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
-      // S = Q K^T. One ldmatrix.x4 = two 8-token groups x two 8-element chunks.
-      const int lr = (lane & 7) + ((lane >> 4) << 3), lch = (lane >> 3) & 1;
-#pragma unroll
-      for (int ks = 0; ks < kDim / 16; ++ks) {
-#pragma unroll
-        for (int j = 0; j < kWarpTok / 16; ++j) {
-          const int r = tok0 + j * 16 + lr;
-          uint32_t b[4];
-          ldsm4(b, kb + r * (kDim * 2) + (((ks * 2 + lch) ^ (r & 7)) << 4));
-          Pair<T>::mma(s[2 * j], qf[ks], b[0], b[1]);
-          Pair<T>::mma(s[2 * j + 1], qf[ks], b[2], b[3]);
-        }
+    float m_ref = neg_inf(), l = 0.f;  // the maximum the weights refer to, and their sum
+    bool piece_start = true;
+    for (int u = u_lo, i = 0; u < u_hi && ok; ++u, ++i) {
+      const int b = i & 1, stage = i % kStages;
+      const bool act_warp = warp * 32 < rows_here;
+      const uint32_t t_s = tmem + lanes + S::kS + b * kTok;
+      const int tile0 = cur.tile * kTok;
+      if (piece_start) {
+        m_ref = neg_inf();
+        l = 0.f;
       }
-      const int tile0 = cc.tile * kTok;
-      const bool masked = tile0 + kTok > min(seen[0], seen[1]) || s_bad[stage] == u + 1;
-#pragma unroll
-      for (int j = 0; j < kWarpTok / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] *= p.scale_log2;
-      const int32_t* table = cc.seg ? p.pages + (int64_t)(cc.seg - 1) * p.pages_stride : p.prefix_pages;
-      auto sees = [&](int e, int tok) {
-        bool see = tok < seen[e];
-        if (!see && branch[e]) {
+      ok = mbar_wait(&c.s_full[b], (i >> 1) & 1, s_abort);
+      // already complete: S was computed from this stage. Makes its flags and values visible here.
+      ok = ok && mbar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
+      if (!__all_sync(~0u, ok)) break;
+      tc_fence_after();
+      const bool bad_page = *const_cast<volatile int*>(&c.bad_unit[stage]) == u + 1;
+      const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
+      auto sees = [&](int tok) {
+        bool see = tok < seen;
+        if (!see && branch) {
           const int n = tok - base;
-          see = n >= 0 && n < 64 && tok < cc.len && ((branch[e] >> n) & 1);
+          see = n >= 0 && n < 64 && tok < cur.len && ((branch >> n) & 1);
         }
-        if (see && s_bad[stage] == u + 1) {
+        if (see && bad_page) {
           const int id = table[tok / p.page_size];
           see = id >= 0 && id < p.total_pages;
         }
         return see;
       };
-      bool bad_v = false;  // a masked tile holds values that are no numbers
-      if (__any_sync(~0u, masked)) {
+      // Some row of the block may not see a token of this tile (uniform over the block).
+      const int sure = cur.seg == 0 ? cur.len : min(cur.len, p.tree ? base : base + 1);
+      const bool masked = tile0 + kTok > sure || bad_page;
+      if (act_warp) {
+        // 64 scores at a time. Of a tile of 128 the second half is read twice: holding both would
+        // cost the registers that the rest needs.
+        uint32_t s[64];
+        const bool plain = !masked && p.scale_log2 > 0.f;
+        const float mul = plain ? p.scale_log2 : 1.f;
+        auto scores = [&](int h) {
 #pragma unroll
-        for (int j = 0; j < kWarpTok / 8; ++j)
+          for (int j = 0; j < 64; j += 32)
+            tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[j]), t_s + h * 64 + j);
+          tc_wait_ld();
+          if (!plain) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!sees(e >> 1, tile0 + tok0 + j * 8 + t4 * 2 + (e & 1))) s[j][e] = neg_inf();
-        for (int i = lane; i < kWarpTok * kChunks; i += 32) {
-          const uint4 w = lds128(vb + tok0 * (kDim * 2) + i * 16);
-          bad_v |= non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
-        }
-        bad_v = __any_sync(~0u, bad_v);
-      }
-      float mx[2] = {neg_inf(), neg_inf()};
-#pragma unroll
-      for (int j = 0; j < kWarpTok / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-      float corr[2], ms[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(~0u, mx[e], 1));
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(~0u, mx[e], 2));
-        const float nm = fmaxf(m[e], mx[e]);
-        ms[e] = nm == neg_inf() ? 0.f : nm;
-        corr[e] = ex2(m[e] - ms[e]);
-        m[e] = nm;
-        l[e] *= corr[e];
-      }
-#pragma unroll
-      for (int j = 0; j < kWarpTok / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[j][e] = ex2(s[j][e] - ms[e >> 1]);
-          l[e >> 1] += s[j][e];
-        }
-#pragma unroll
-      for (int j = 0; j < kDim / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] *= corr[e >> 1];
-      // O += P V. P is rounded to the cache's type for the tensor cores; its sum l is not.
-      auto weigh = [&](auto clean) {
-#pragma unroll
-        for (int kt = 0; kt < kWarpTok / 16; ++kt) {
-          const uint32_t a[4] = {Pair<T>::pack(s[2 * kt][0], s[2 * kt][1]),
-                                 Pair<T>::pack(s[2 * kt][2], s[2 * kt][3]),
-                                 Pair<T>::pack(s[2 * kt + 1][0], s[2 * kt + 1][1]),
-                                 Pair<T>::pack(s[2 * kt + 1][2], s[2 * kt + 1][3])};
-          const int r = tok0 + kt * 16 + (lane & 15);
-          const uint32_t rb = vb + r * (kDim * 2);
-#pragma unroll
-          for (int j = 0; j < kDim / 16; ++j) {
-            uint32_t b[4];
-            ldsm4_t(b, rb + (((2 * j + (lane >> 4)) ^ (r & 7)) << 4));
-            if constexpr (decltype(clean)::value) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) b[i] = finite_or_zero<T>(b[i]);
+            for (int j = 0; j < 64; ++j) {
+              const float x = __uint_as_float(s[j]) * p.scale_log2;
+              s[j] = __float_as_uint(!masked || sees(tile0 + h * 64 + j) ? x : neg_inf());
             }
-            Pair<T>::mma(o[2 * j], a, b[0], b[1]);
-            Pair<T>::mma(o[2 * j + 1], a, b[2], b[3]);
+            __syncwarp();
           }
-        }
-      };
-      if (!bad_v) {
-        weigh(std::false_type{});
-      } else {
-        // 0 * NaN would reach rows that do not see the token: the product runs on the numbers, and
-        // what is none is added to the rows that see it (whose result it makes inf or NaN).
-        weigh(std::true_type{});
-        for (int r = tok0; r < tok0 + kWarpTok; ++r) {
-          const bool s0 = sees(0, tile0 + r), s1 = sees(1, tile0 + r);
+        };
+        float mx4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-          for (int j = 0; j < kDim / 8; ++j) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                smem + stage * 2 * S::kHalfBytes + S::kHalfBytes + r * (kDim * 2) +
-                ((j ^ (r & 7)) << 4) + t4 * 4);
-            if (!non_finite<T>(w)) continue;
-            const float2 v = unpack2<T>(w);
-            if (!isfinite(v.x)) {
-              if (s0) o[j][0] += v.x;
-              if (s1) o[j][2] += v.x;
-            }
-            if (!isfinite(v.y)) {
-              if (s0) o[j][1] += v.y;
-              if (s1) o[j][3] += v.y;
+        for (int h = kTok / 64 - 1; h >= 0; --h) {
+          scores(h);
+#pragma unroll
+          for (int j = 0; j < 64; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+        const bool grow = mx > m_ref + 8.f || (m_ref == neg_inf() && mx > neg_inf());
+        if (__any_sync(~0u, grow)) {
+          const float f = grow ? ex2(m_ref - mx) : 1.f;
+          if (grow) m_ref = mx;
+          l *= f;
+          if (!piece_start) {
+            ok = mbar_wait(&c.o_done[b ^ 1], ((i - 1) >> 1) & 1, s_abort);
+            tc_fence_after();
+            __syncwarp();
+#pragma unroll 1
+            for (int c0 = 0; c0 < kDim; c0 += 32) {
+              uint32_t w[32];
+              tmem_ld32(w, t_o + c0);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * f);
+              tmem_st32(t_o + c0, w);
             }
           }
         }
+        const float ref = m_ref == neg_inf() ? 0.f : m_ref;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < kTok / 64; ++h) {
+          if (h > 0) scores(h);
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const float x = ex2(fmaf(__uint_as_float(s[j]), mul, -ref));
+            const float y = ex2(fmaf(__uint_as_float(s[j + 1]), mul, -ref));
+            sum[j & 2] += x;
+            sum[(j & 2) + 1] += y;
+            s[j / 2] = Pair<T>::pack(x, y);
+          }
+          // over scores that have been read: weights take half the columns
+          tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_wait_st();
       }
-    }
+      // A masked tile of a request's own tokens may hold infinities or NaN that some rows do not
+      // see; 0 * NaN would carry them into those rows. They are replaced by zeros before the second
+      // product, and added afterwards to the rows that see them.
+      bool poisoned = false;
+      if (masked && cur.seg) {
+        uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
+        bool found = false;
+        for (int x = threadIdx.x; x < S::kHalf / 16; x += kSoftWarps * 32) {
+          const uint4 w = *reinterpret_cast<const uint4*>(vt + x * 16);
+          found |= non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
+        }
+        if (found) *const_cast<volatile int*>(&c.bad_value) = u + 1;
+        sync_rows();
+        poisoned = *const_cast<volatile int*>(&c.bad_value) == u + 1;
+        if (poisoned) {
+          for (int x = threadIdx.x; x < kTok; x += kSoftWarps * 32) c.bad_token[x] = 0;
+          sync_rows();
+          for (int x = threadIdx.x; x < S::kHalf / 16; x += kSoftWarps * 32) {
+            uint4 w = *reinterpret_cast<const uint4*>(vt + x * 16);
+            if (!(non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w))) continue;
+            *const_cast<volatile unsigned char*>(&c.bad_token[(x / 8) % kTok]) = 1;
+            w = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z),
+                           finite_or_zero<T>(w.w));
+            *reinterpret_cast<uint4*>(vt + x * 16) = w;
+          }
+          fence_proxy_async_smem();
+          sync_rows();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.p_full[b]);
+      if (poisoned) {
+        ok = ok && mbar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
+        tc_fence_after();
+        __syncwarp();
+        const int head = cur.group / cur.blocks;
+        for (int x = 0; x < kTok && act_warp; ++x) {
+          if (!*const_cast<volatile unsigned char*>(&c.bad_token[x])) continue;
+          const int tok = tile0 + x, pg = tok / p.page_size;
+          const bool see = (int)threadIdx.x < rows_here && sees(tok);
+          const T* v = static_cast<const T*>(p.v) + table[pg] * p.vs[0] +
+                       (tok - pg * p.page_size) * p.vs[1] + head * p.vs[2];
+#pragma unroll 1
+          for (int c0 = 0; c0 < kDim; c0 += 32) {
+            uint32_t w[32];
+            tmem_ld32(w, t_o + c0);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (c0 + j >= p.dim || !see) continue;
+              const float y = (float)v[c0 + j];
+              if (!isfinite(y)) w[j] = __float_as_uint(__uint_as_float(w[j]) + y);
+            }
+            tmem_st32(t_o + c0, w);
+          }
+          tc_wait_st();
+        }
+        tc_fence_before();
+        sync_rows();  // bad_token is free again
+      }
 
-    // ---- end of a piece: join the token warps and write the partial
-    const bool piece_end = cc.tile + 1 == cc.tiles || u + 1 == u_hi;
-    if (piece_end) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l[e] += __shfl_xor_sync(~0u, l[e], 1);
-        l[e] += __shfl_xor_sync(~0u, l[e], 2);
+      const bool piece_end = cur.tile + 1 == cur.tiles || u + 1 == u_hi;
+      piece_start = piece_end;
+      if (!piece_end) {
+        ++cur.tile;
+        continue;
       }
-      if (t4 == 0) {
-        s_ml[tw * kBlockRows + rw * 16 + g4] = make_float2(m[0], l[0]);
-        s_ml[tw * kBlockRows + rw * 16 + g4 + 8] = make_float2(m[1], l[1]);
-      }
-      __syncthreads();
-      float f[2];
+      // ---- end of a piece: the next one's queries first, then O out
+      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.group;
+      const int done_rows = rows_here;
+      cur.next(p, plan, kTok, kBlockRows);
+      if (u + 1 < u_hi) open_piece();
+      ok = ok && mbar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
+      tc_fence_after();
+      __syncwarp();
+      if (warp * 32 < done_rows) {
+        const bool act = (int)threadIdx.x < done_rows && slot >= 0 && slot < p.slots;
+        const int64_t at = (int64_t)slot * kBlockRows + threadIdx.x;
+        float* dst = p.part_o + at * p.dim;
+#pragma unroll 1
+        for (int c0 = 0; c0 < p.dim; c0 += 32) {
+          uint32_t w[32];
+          tmem_ld32(w, t_o + c0);
+          tc_wait_ld();
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = neg_inf();
-#pragma unroll
-        for (int w = 0; w < kTokWarps; ++w)
-          top = fmaxf(top, s_ml[w * kBlockRows + rw * 16 + g4 + 8 * e].x);
-        f[e] = ex2(m[e] - (top == neg_inf() ? 0.f : top));
-      }
-      const int slot = (int)blockIdx.x + (cc.seg ? plan.groups_end[cc.seg - 1] : 0) + cc.group;
-      const int rows_here = min(kBlockRows, row_lim - block * kBlockRows);
-      const bool room = slot >= 0 && slot < p.slots;
-      if (room && (int)threadIdx.x < rows_here) {
-        float top = neg_inf(), sum = 0.f;
-        for (int w = 0; w < kTokWarps; ++w) top = fmaxf(top, s_ml[w * kBlockRows + threadIdx.x].x);
-        const float safe = top == neg_inf() ? 0.f : top;
-        for (int w = 0; w < kTokWarps; ++w) {
-          const float2 ml = s_ml[w * kBlockRows + threadIdx.x];
-          sum += ml.y * ex2(ml.x - safe);
+          for (int j = 0; j < 32; j += 4)
+            if (act && c0 + j < p.dim)
+              *reinterpret_cast<uint4*>(dst + c0 + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
         }
-        p.part_ml[(int64_t)slot * kBlockRows + threadIdx.x] = make_float2(top, sum);
+        if (act) p.part_ml[at] = make_float2(m_ref, l);
       }
-      float* dst = p.part_o + (int64_t)slot * kBlockRows * p.dim;
-#pragma unroll
-      for (int c0 = 0; c0 < kDim; c0 += kCols) {
-        if (c0 < p.dim) {
-#pragma unroll
-          for (int j = 0; j < kCols / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float* to = s_join + (tw * kBlockRows + rw * 16 + g4 + 8 * e) * (kCols + 4) + j * 8 + t4 * 2;
-              to[0] = o[c0 / 8 + j][2 * e] * f[e];
-              to[1] = o[c0 / 8 + j][2 * e + 1] * f[e];
-            }
-        }
-        __syncthreads();
-        if (c0 < p.dim && room) {
-          for (int i = threadIdx.x; i < rows_here * (kCols / 4); i += kAttnThreads) {
-            const int r = i / (kCols / 4), c = (i % (kCols / 4)) * 4;
-            if (c0 + c >= p.dim) continue;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kTokWarps; ++w) {
-              const float4 x = *reinterpret_cast<const float4*>(
-                  s_join + (w * kBlockRows + r) * (kCols + 4) + c);
-              v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
-            *reinterpret_cast<float4*>(dst + (int64_t)r * p.dim + c0 + c) = v;
-          }
-        }
-        __syncthreads();
-      }
-      piece_start = true;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.o_free);
     }
-    cc.next(p, plan, kTok, kBlockRows);
-    if (++stage == kStages) stage = 0;
   }
-  cp_async_wait<0>();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free(tmem, S::kColumns);
+  }
+  if (threadIdx.x == 0 && *s_abort) atomicCAS(&g_attn_status, 0, B2_ERR_TIMEOUT);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -612,8 +780,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
 // its request's own group, each from a run of CTAs; they are added in that order.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, int tok, int block_rows,
-                                                            int grid) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, int tok, int grid) {
+  constexpr int block_rows = kBlockRows;
   __shared__ Plan plan;
   __shared__ int s_seg;
   const int t = blockIdx.x / p.q_heads, h = blockIdx.x - t * p.q_heads;
@@ -679,18 +847,16 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, in
 }
 
 int round_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Rows of a block: 32 where no group has more, else 64.
-int block_rows_for(int rows, int group) { return (int64_t)rows * group <= 32 ? 32 : 64; }
-int64_t slots_for(int requests, int rows, int group, int kv_heads, int block_rows, int ctas) {
-  const int64_t blocks = ((int64_t)rows * group + block_rows - 1) / block_rows;
-  return ctas + kv_heads * (2 * blocks + requests);
+int64_t slots_for(int requests, int rows, int group, int kv_heads) {
+  const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
+  return kMaxCtas + kv_heads * (2 * blocks + requests);
 }
 
-template <typename T, int kDim, int kRowWarps>
+template <typename T, int kDim>
 int launch_typed(const AttnArgs& p, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = attn_smem<kDim, kRowWarps>();
+  constexpr size_t smem = attn_smem<kDim>();
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  auto kernel = attn_kernel<T, kDim, kRowWarps>;
+  auto kernel = attn_kernel<T, kDim>;
   static bool configured[64] = {};
   int dev = 0;
   B2_CUDA_TRY(cudaGetDevice(&dev));
@@ -701,18 +867,15 @@ int launch_typed(const AttnArgs& p, int ctas, cudaStream_t stream) {
   int rc = launch_kernel(kernel, ctas, kAttnThreads, smem, stream, /*early=*/true, p);
   if (rc) return rc;
   return launch_kernel(join_kernel<T>, p.rows * p.q_heads, kJoinThreads, 0, stream, /*early=*/true,
-                       p, Shape<kDim>::kTok, kRowWarps * 16, ctas);
+                       p, Shape<kDim>::kTok, ctas);
 }
 
 template <typename T>
-int launch_dim(const AttnArgs& p, int block_rows, int ctas, cudaStream_t stream) {
-  switch (round_dim(p.dim) + block_rows) {
-    case 64 + 32: return launch_typed<T, 64, 2>(p, ctas, stream);
-    case 64 + 64: return launch_typed<T, 64, 4>(p, ctas, stream);
-    case 128 + 32: return launch_typed<T, 128, 2>(p, ctas, stream);
-    case 128 + 64: return launch_typed<T, 128, 4>(p, ctas, stream);
-    case 256 + 32: return launch_typed<T, 256, 2>(p, ctas, stream);
-    default: return launch_typed<T, 256, 4>(p, ctas, stream);
+int launch_dim(const AttnArgs& p, int ctas, cudaStream_t stream) {
+  switch (round_dim(p.dim)) {
+    case 64: return launch_typed<T, 64>(p, ctas, stream);
+    case 128: return launch_typed<T, 128>(p, ctas, stream);
+    default: return launch_typed<T, 256>(p, ctas, stream);
   }
 }
 
@@ -736,9 +899,8 @@ extern "C" size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, 
                                            int head_dim) {
   using namespace b2;
   if (check_shape(requests, rows, q_heads, kv_heads, head_dim)) return 0;
-  const int group = q_heads / kv_heads, br = block_rows_for(rows, group);
-  const int64_t slots = slots_for(requests, rows, group, kv_heads, br, kMaxCtas);
-  return (size_t)slots * br * (head_dim * sizeof(float) + sizeof(float2)) + 256;
+  const int64_t slots = slots_for(requests, rows, q_heads / kv_heads, kv_heads);
+  return (size_t)slots * kBlockRows * (head_dim * sizeof(float) + sizeof(float2)) + 256;
 }
 
 extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
@@ -778,10 +940,10 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   const size_t need = b2_prefix_attn_workspace(requests, rows, q_heads, kv_heads, head_dim);
   if (!ws || ws_bytes < need || !aligned16(ws))
     return fail(B2_ERR_WORKSPACE, "%s: workspace of %zu B, need %zu B", op, ws_bytes, need);
-  const int group = q_heads / kv_heads, br = block_rows_for(rows, group);
+  const int group = q_heads / kv_heads;
   const int tok = round_dim(head_dim) == 64 ? 128 : 64;
   // units are counted in 32 bits
-  const int64_t blocks = ((int64_t)rows * group + br - 1) / br;
+  const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
   const int64_t tiles = ((int64_t)std::max(n_prefix_pages, max_pages) * page_size + tok - 1) / tok;
   if ((2 * blocks + requests) * kv_heads * tiles > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "%s: tables too long for %d rows", op, rows);
@@ -796,17 +958,18 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.prefix_pages = prefix_pages, p.prefix_len = prefix_len, p.pages = pages, p.own_lens = own_lens;
   p.row_start = row_start, p.tree = tree;
   p.out = out, p.lse = lse;
+  p.q_vec = aligned16(q) && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0;
   p.pages_stride = pages_stride;
   p.total_pages = total_pages, p.page_size = page_size;
   p.n_prefix_pages = n_prefix_pages, p.max_pages = max_pages;
   p.requests = requests, p.rows = rows, p.q_heads = q_heads, p.kv_heads = kv_heads, p.group = group;
   p.dim = head_dim;
-  p.slots = (int)slots_for(requests, rows, group, kv_heads, br, kMaxCtas);
+  p.slots = (int)slots_for(requests, rows, group, kv_heads);
   p.scale_log2 = scale * kLog2e;
   p.part_ml = static_cast<float2*>(ws);
-  const size_t ml_bytes = ((size_t)p.slots * br * sizeof(float2) + 255) & ~(size_t)255;
+  const size_t ml_bytes = ((size_t)p.slots * kBlockRows * sizeof(float2) + 255) & ~(size_t)255;
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + ml_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == B2_DTYPE_F16 ? launch_dim<__half>(p, br, ctas, s)
-                               : launch_dim<__nv_bfloat16>(p, br, ctas, s);
+  return dtype == B2_DTYPE_F16 ? launch_dim<__half>(p, ctas, s)
+                               : launch_dim<__nv_bfloat16>(p, ctas, s);
 }
