@@ -350,6 +350,10 @@ int b2_rope_cache(const void* q, const int64_t* q_strides, const void* k, const 
  * ws: b2_prefix_attn_workspace() bytes, 16-byte aligned, no initialisation; calls that overlap on
  * the GPU need one each. Equal calls give equal bits.
  * ---------------------------------------------------------------------------------------- */
+/* A device-side wait that gave up (a fault of the library or the device; outputs of that call are
+ * undefined) is recorded per device: 0 or B2_ERR_TIMEOUT, cleared when `clear` is non-zero.
+ * Synchronises the device. */
+int b2_prefix_attn_status(int clear, int* device_status);
 size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, int kv_heads, int head_dim);
 int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
                    const int64_t* k_strides, const void* v_cache, const int64_t* v_strides,

@@ -88,6 +88,7 @@ _SIGS = {
                      _i, _i, _vp]),
     "b2_rope_cache": (_i, [_vp, _strides, _vp, _strides, _vp, _strides, _vp, _i, _vp, _vp, _vp, _vp,
                            _strides, _vp, _strides, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp]),
+    "b2_prefix_attn_status": (_i, [_i, C.POINTER(_i)]),
     "b2_prefix_attn_workspace": (_sz, [_i, _i, _i, _i, _i]),
     "b2_prefix_attn": (_i, [_vp, _strides, _vp, _strides, _vp, _strides, _i, _i, _vp, _i, _vp, _vp,
                             _i64, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _sz,

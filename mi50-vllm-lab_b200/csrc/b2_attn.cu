@@ -31,12 +31,21 @@ constexpr int kMaxRequests = 1024;
 constexpr int kMaxRows = 4096;
 constexpr int kSoftWarps = 4;      // one thread per row of a block
 constexpr int kLoadThreads = 128;
-constexpr int kAttnThreads = kSoftWarps * 32 + 32 + kLoadThreads;
 constexpr int kBlockRows = 128;
 constexpr int kJoinThreads = 128;
 constexpr int kMaxCtas = 160;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Where the partials of a row are: written by the main launch, read by the one that joins them.
+struct RowPlan {
+  int units;                        // of the whole call
+  int prefix_tiles, prefix_blocks, prefix_first;
+  int tiles, blocks, first;         // of the row's request; tiles = 0: none
+  int unit0, group0;                // units and groups before the request's
+  int owned;                        // the row belongs to a request
+  int pad[2];
+};
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -46,13 +55,15 @@ struct AttnArgs {
   const int64_t* tree;
   void* out;
   float* lse;
-  float* part_o;   // [slots][rows per block][dim]
-  float2* part_ml; // [slots][rows per block]
+  float* part_o;    // [slots][rows per block][dim]
+  float2* part_ml;  // [slots][rows per block]
+  RowPlan* row_plan;  // [rows]
   int64_t pages_stride;
   int total_pages, page_size, n_prefix_pages, max_pages;
   int requests, rows, q_heads, kv_heads, group, dim;
   int slots;
-  int q_vec;  // queries allow 16-byte loads
+  int q_vec;     // queries allow 16-byte loads
+  int box_rows;  // tokens per TMA box: a power of two that divides the page size
   float scale_log2;
 };
 
@@ -128,6 +139,12 @@ __device__ __forceinline__ void tc_fence_after() {
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(p));
+  return p != 0;
+}
 // Arrive on `bar` when every tcgen05.mma this thread has issued has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -187,71 +204,76 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 struct Plan {
   int units_end[kMaxRequests + 1];   // running sum of units up to and with segment s
   int groups_end[kMaxRequests + 1];  // running sum of groups
-  int warp_sum[2][kAttnThreads / 32];
+  int first[kMaxRequests + 1];       // first row of the segment
+  int count[kMaxRequests + 1];       // and how many
+  int len[kMaxRequests + 1];         // tokens
 };
 
-// Rows [first, first + count) of a request, and how many of its own tokens are stored.
-__device__ __forceinline__ void request_rows(const AttnArgs& p, int b, int& first, int& count) {
-  first = min(max(p.row_start[b], 0), p.rows);
-  count = max(0, min(max(p.row_start[b + 1], 0), p.rows) - first);
-}
-__device__ __forceinline__ int own_length(const AttnArgs& p, int b) {
-  return (int)min((int64_t)max(p.own_lens[b], 0), (int64_t)p.max_pages * p.page_size);
-}
-__device__ __forceinline__ int prefix_length(const AttnArgs& p) {
-  return (int)min((int64_t)max(*p.prefix_len, 0), (int64_t)p.n_prefix_pages * p.page_size);
-}
-__device__ __forceinline__ void segment_shape(const AttnArgs& p, int s, int tok, int block_rows,
-                                              int& first, int& count, int& len, int& tiles,
-                                              int& blocks) {
-  if (s == 0) {
-    first = min(max(p.row_start[0], 0), p.rows);
-    count = max(0, min(max(p.row_start[p.requests], 0), p.rows) - first);
-    len = prefix_length(p);
-  } else {
-    request_rows(p, s - 1, first, count);
-    len = own_length(p, s - 1);
-  }
-  tiles = (len + tok - 1) / tok;
-  blocks = (count * p.group + block_rows - 1) / block_rows;
+__device__ __forceinline__ int blocks_of(int count, int group) {
+  return (count * group + kBlockRows - 1) / kBlockRows;
 }
 
-// Block-wide scan over the segments; kWarps warps take part. Row starts that decrease are outside
-// the contract: the plan is then empty (every output 0, lse -inf), so that no index leaves its array.
-template <int kWarps>
-__device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, int block_rows, Plan& plan) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int u_base = 0, g_base = 0;
+// Lengths and rows of every segment, cut at the tables and at the rows there are, and the running
+// sums. Row starts that decrease are outside the contract: the plan is then empty (every output 0,
+// lse -inf), so that no index leaves its array. Ends with a block-wide barrier.
+__device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan) {
   int bad = 0;
-  for (int b = threadIdx.x; b < p.requests; b += kWarps * 32) bad |= p.row_start[b + 1] < p.row_start[b];
-  bad = __syncthreads_or(bad);
-  for (int s0 = 0; s0 <= p.requests; s0 += kWarps * 32) {
-    const int s = s0 + threadIdx.x;
-    int u = 0, g = 0;
-    if (s <= p.requests) {
-      int first, count, len, tiles, blocks;
-      segment_shape(p, s, tok, block_rows, first, count, len, tiles, blocks);
-      if (tiles > 0 && !bad) {
-        g = p.kv_heads * blocks;
-        u = g * tiles;
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int uu = __shfl_up_sync(~0u, u, d), gg = __shfl_up_sync(~0u, g, d);
-      if (lane >= d) u += uu, g += gg;
-    }
-    if (lane == 31) plan.warp_sum[0][warp] = u, plan.warp_sum[1][warp] = g;
-    __syncthreads();
-    int ub = u_base, gb = g_base;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) ub += plan.warp_sum[0][w], gb += plan.warp_sum[1][w];
-      u_base += plan.warp_sum[0][w];
-      g_base += plan.warp_sum[1][w];
-    }
-    if (s <= p.requests) plan.units_end[s] = ub + u, plan.groups_end[s] = gb + g;
-    __syncthreads();
+  for (int s = threadIdx.x; s <= p.requests; s += blockDim.x) {
+    const int r0 = p.row_start[s ? s - 1 : 0], r1 = p.row_start[s ? s : p.requests];
+    const int len = s ? p.own_lens[s - 1] : *p.prefix_len;
+    const int64_t room = (int64_t)(s ? p.max_pages : p.n_prefix_pages) * p.page_size;
+    bad |= r1 < r0;
+    const int first = min(max(r0, 0), p.rows);
+    plan.first[s] = first;
+    plan.count[s] = max(0, min(max(r1, 0), p.rows) - first);
+    plan.len[s] = (int)min((int64_t)max(len, 0), room);
   }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x < 32) {
+    int u_base = 0, g_base = 0;
+    for (int s0 = 0; s0 <= p.requests; s0 += 32) {
+      const int s = s0 + threadIdx.x;
+      int u = 0, g = 0;
+      if (s <= p.requests && !bad && plan.len[s] > 0) {
+        g = p.kv_heads * blocks_of(plan.count[s], p.group);
+        u = g * ((plan.len[s] + tok - 1) / tok);
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int uu = __shfl_up_sync(~0u, u, d), gg = __shfl_up_sync(~0u, g, d);
+        if ((int)threadIdx.x >= d) u += uu, g += gg;
+      }
+      u += u_base, g += g_base;
+      if (s <= p.requests) plan.units_end[s] = u, plan.groups_end[s] = g;
+      u_base = __shfl_sync(~0u, u, 31);
+      g_base = __shfl_sync(~0u, g, 31);
+    }
+  }
+  __syncthreads();
+}
+
+// The plan of row t for the launch that joins its partials.
+__device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const Plan& plan, int t) {
+  RowPlan r = {};
+  r.units = plan.units_end[p.requests];
+  r.prefix_tiles = (plan.len[0] + tok - 1) / tok;
+  r.prefix_blocks = blocks_of(plan.count[0], p.group);
+  r.prefix_first = plan.first[0];
+  // the last request that starts at or before t: requests without rows share a start with the next
+  int lo = 0, hi = p.requests;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (plan.first[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  if (r.units > 0 && lo > 0 && t < plan.first[lo] + plan.count[lo]) {
+    r.owned = 1;
+    r.tiles = (plan.len[lo] + tok - 1) / tok;
+    r.blocks = blocks_of(plan.count[lo], p.group);
+    r.first = plan.first[lo];
+    r.unit0 = plan.units_end[lo - 1];
+    r.group0 = plan.groups_end[lo - 1];
+  }
+  p.row_plan[t] = r;
 }
 
 // CTAs that share `units` units: at most `ctas`, none of them empty.
@@ -265,25 +287,26 @@ __device__ __forceinline__ int plan_owner(int units, int ctas, int u) {
 
 // A position in the unit order: segment, group inside it (head-major), tile.
 struct Cursor {
-  int seg, group, tile;              // group = head * blocks + row block
+  int seg, group, tile;  // group = head * blocks + row block
   int first, count, len, tiles, blocks;
-  __device__ __forceinline__ void load(const AttnArgs& p, int tok, int block_rows) {
-    segment_shape(p, seg, tok, block_rows, first, count, len, tiles, blocks);
+  __device__ __forceinline__ void load(const AttnArgs& p, const Plan& plan, int tok) {
+    first = plan.first[seg], count = plan.count[seg], len = plan.len[seg];
+    tiles = (len + tok - 1) / tok;
+    blocks = blocks_of(count, p.group);
   }
-  __device__ __forceinline__ void seek(const AttnArgs& p, const Plan& plan, int u, int tok,
-                                       int block_rows) {
+  __device__ __forceinline__ void seek(const AttnArgs& p, const Plan& plan, int u, int tok) {
     int lo = 0, hi = p.requests;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (plan.units_end[mid] > u) hi = mid; else lo = mid + 1;
     }
     seg = lo;
-    load(p, tok, block_rows);
+    load(p, plan, tok);
     const int local = u - (seg ? plan.units_end[seg - 1] : 0);
     group = local / tiles;
     tile = local - group * tiles;
   }
-  __device__ __forceinline__ void next(const AttnArgs& p, const Plan& plan, int tok, int block_rows) {
+  __device__ __forceinline__ void next(const AttnArgs& p, const Plan& plan, int tok) {
     if (++tile < tiles) return;
     tile = 0;
     if (++group < p.kv_heads * blocks) return;
@@ -292,7 +315,7 @@ struct Cursor {
     while (seg < p.requests && plan.units_end[seg + 1] == done) ++seg;
     if (seg < p.requests) {
       ++seg;
-      load(p, tok, block_rows);
+      load(p, plan, tok);
     }
   }
 };
@@ -306,9 +329,10 @@ struct Cursor {
 // both lie as loaded, [token][64 dimensions] rows of 128 bytes, swizzled.
 //   warps 0-3  softmax: a thread owns a row (its lane of tensor memory), so the running maximum and
 //              sum need no exchange between threads; they also bring Q in and take O out
-//   warp 4     one thread issues the products: those of tile i + 1 before tile i's second one, so
-//              that the tensor cores work while the softmax of tile i runs
-//   warps 5-8  copy K and V, 16 bytes per cp.async, page by page, for any page size and strides
+//   warp 4     issues the products: the first of tile i + 1 before the second of tile i, so that
+//              the tensor cores work while the softmax of tile i runs
+//   warp 5     (kTma) one TMA box per group of tokens of one page and 64 dimensions
+//   warps 5-8  (otherwise) 16 bytes per cp.async, for any page size and strides
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the one its weights refer
 // to (the weights stay below 2^8, in range of fp16, with the same relative rounding); the sum l and
 // the partial refer to the same maximum, so nothing is approximated.
@@ -335,6 +359,8 @@ struct Control {
   unsigned char bad_token[128];
 };
 
+constexpr int attn_threads(bool tma) { return kSoftWarps * 32 + 32 + (tma ? 32 : kLoadThreads); }
+
 template <int kDim>
 constexpr size_t attn_smem() {
   return 1024 + Shape<kDim>::kRing + sizeof(Plan) + sizeof(Control) + 16;
@@ -342,8 +368,25 @@ constexpr size_t attn_smem() {
 
 __device__ int g_attn_status;
 
-template <typename T, int kDim>
-__global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p) {
+// mbar_wait without its suspend-time hint.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_test(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  for (unsigned int it = 1; it < kMaxSpin; ++it) {
+    if (mbar_test(bar, parity)) return true;
+    if ((it & 63u) == 0) {
+      if (*abort) return false;
+      if (globaltimer_ns() - t0 > kPipeWaitNs) break;
+    }
+  }
+  *abort = 1;
+  return false;
+}
+
+template <typename T, int kDim, bool kTma>
+__global__ void __launch_bounds__(attn_threads(kTma), 1)
+    attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const AttnArgs p) {
   using S = Shape<kDim>;
   constexpr int kTok = S::kTok, kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -356,7 +399,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&c.full[s], kLoadThreads + kLoadThreads / 32);
+      mbar_init(&c.full[s], kTma ? 1 : kLoadThreads + kLoadThreads / 32);
       mbar_init(&c.empty[s], 1);
       c.bad_unit[s] = 0;
     }
@@ -376,11 +419,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
   if (warp == kSoftWarps) tmem_alloc(&c.tmem, S::kColumns);
   grid_dep_wait();
   grid_dep_launch();
-  make_plan<kAttnThreads / 32>(p, kTok, kBlockRows, plan);
+  make_plan(p, kTok, plan);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = c.tmem;
+  const uint32_t tmem = __shfl_sync(~0u, c.tmem, 0);
   const int units = plan.units_end[p.requests];
   const int ctas = plan_ctas(units, gridDim.x);
   const bool idle = (int)blockIdx.x >= ctas;
@@ -390,9 +433,65 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
   const int stage_bytes = 2 * S::kHalf;
 
   Cursor cur;
-  if (!idle) cur.seek(p, plan, u_lo, kTok, kBlockRows);
+  if (!idle) cur.seek(p, plan, u_lo, kTok);
 
-  if (warp > kSoftWarps) {
+  if (kTma && warp > kSoftWarps) {
+    // ------------------------------------------------------------------------------ loader (TMA)
+    // Boxes of box_rows tokens x 64 dimensions. A box behind the length, or of a page that does not
+    // exist, is loaded from behind the last page: zeros, without a read.
+    const int groups = kTok / p.box_rows;  // a power of two, at most 16
+    constexpr int kSubs = kDim / 64;
+    const int boxes = groups * kSubs * 2;
+    const int row0 = (lane % groups) * p.box_rows;  // the same for all boxes of a lane
+    int id = -1, at = 0;
+    auto look_up = [&] {
+      const int tok = cur.tile * kTok + row0;
+      id = -1, at = 0;
+      if (tok < cur.len) {
+        const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
+        const int pg = tok / p.page_size;
+        id = table[pg];
+        at = tok - pg * p.page_size;
+      }
+    };
+    if (lane == 0) {
+      tma_prefetch_desc(&map_k);
+      tma_prefetch_desc(&map_v);
+    }
+    const uint64_t once = l2_evict_first_policy(), again = l2_evict_normal_policy();
+    if (!idle) look_up();
+    int issued = 0;
+    for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
+      const int stage = i % kStages;
+      const int head = cur.group / cur.blocks, tok = cur.tile * kTok + row0, len = cur.len;
+      const uint64_t pol = cur.blocks > 1 ? again : once;
+      const int raw = id, tile_at = at;
+      cur.next(p, plan, kTok);
+      if (u + 1 < u_hi) look_up();  // its latency passes behind this tile's wait
+      if (!__all_sync(~0u, bar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort))) break;
+      const bool exists = raw >= 0 && raw < p.total_pages;
+      const int page = tok < len && exists ? raw : p.total_pages;
+      if (tok < len && !exists) *const_cast<volatile int*>(&c.bad_unit[stage]) = u + 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&c.full[stage], stage_bytes);
+      __syncwarp();
+      for (int x = lane; x < boxes; x += 32) {
+        const int sub = (x / groups) % kSubs, is_v = x / (groups * kSubs);
+        uint8_t* dst = smem + stage * stage_bytes + is_v * S::kHalf + sub * S::kSub + row0 * 128;
+        tma_load_4d(dst, is_v ? &map_v : &map_k, &c.full[stage], sub * 64, tile_at, head, page, pol);
+      }
+      __syncwarp();
+      issued = i + 1;
+    }
+    // After an abort: do not retire while copies may still be landing in shared memory.
+    if (*s_abort) {
+      for (int k = max(0, issued - kStages); k < issued; ++k) {
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_test(&c.full[k % kStages], (k / kStages) & 1) && globaltimer_ns() - t0 < kPipeWaitNs) {
+        }
+      }
+    }
+  } else if (warp > kSoftWarps) {
     // ------------------------------------------------------------------------------ loaders
     constexpr int kChunks = kDim / 8;               // 16-byte chunks per token
     constexpr int kWarpRows = 32 / kChunks;         // tokens per warp and copy
@@ -423,10 +522,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
       const int tile_id = id, tile_at = at;
       const T* kc = static_cast<const T*>(p.k) + head * p.ks[2] + chunk * 8;
       const T* vc = static_cast<const T*>(p.v) + head * p.vs[2] + chunk * 8;
-      cur.next(p, plan, kTok, kBlockRows);
+      cur.next(p, plan, kTok);
       if (u + 1 < u_hi) look_up(id, at);  // its latency passes behind this tile's wait and copies
       bool ok = true;
-      if (lane == 0) ok = mbar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort);
+      if (lane == 0) ok = bar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort);
       ok = __shfl_sync(~0u, ok, 0);
       if (!ok) break;
       if (tile_id == -2) c.bad_unit[stage] = u + 1;
@@ -450,56 +549,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
     cp_async_wait_all();
   } else if (warp == kSoftWarps) {
     // ------------------------------------------------------------------------------ products
-    if (lane == 0 && !idle) {
+    // The whole warp runs this loop, so that addresses and descriptors stay in uniform registers;
+    // one elected lane issues.
+    for (int r = blockIdx.x + gridDim.x * lane; r < p.rows; r += gridDim.x * 32)
+      write_row_plan(p, kTok, plan, r);
+    __syncwarp();
+    if (!idle) {
       constexpr uint32_t kIdescS = instr_desc<T>(kTok, false), kIdescO = instr_desc<T>(kDim, true);
-      int pieces = 0;         // pieces whose second product has begun
-      bool first[2] = {};     // tile i (by parity) opens its piece
+      int pieces = 0;  // pieces whose second product has begun
       bool ok = true;
-      auto second = [&](int i) {  // O += P V of tile i
-        ok = ok && mbar_wait(&c.p_full[i & 1], (i >> 1) & 1, s_abort);
-        if (first[i & 1]) {
-          if (pieces > 0) ok = ok && mbar_wait(&c.o_free, (pieces - 1) & 1, s_abort);
+      const bool leader = elect_one();
+      auto second = [&](int i, bool first) {  // O (+)= P V of tile i; `first`: it opens its piece
+        ok = ok && __all_sync(~0u, bar_wait(&c.p_full[i & 1], (i >> 1) & 1, s_abort));
+        if (first) {
+          if (pieces > 0) ok = ok && __all_sync(~0u, bar_wait(&c.o_free, (pieces - 1) & 1, s_abort));
           ++pieces;
         }
         if (!ok) return;
         tc_fence_after();
-        const uint32_t vb = ring + (i % kStages) * stage_bytes + S::kHalf;
+        const int stage = i % kStages;
+        const uint64_t vd = smem_desc(ring + stage * stage_bytes + S::kHalf, S::kSub, 1024);
         const uint32_t pa = tmem + S::kS + (i & 1) * kTok;
+        if (leader) {
 #pragma unroll
-        for (int ks = 0; ks < kTok / 16; ++ks)
-          tc_mma(tmem, pa + ks * 8, smem_desc(vb + ks * 2048, S::kSub, 1024), kIdescO,
-                 !(first[i & 1] && ks == 0));
-        tc_commit(&c.empty[i % kStages]);
-        tc_commit(&c.o_done[i & 1]);
+          for (int ks = 0; ks < kTok / 16; ++ks)
+            tc_mma(tmem, pa + ks * 8, vd + ks * (2048 >> 4), kIdescO, ks > 0 || !first);
+          tc_commit(&c.empty[stage]);
+          tc_commit(&c.o_done[i & 1]);
+        }
+        __syncwarp();
       };
-      int starts = 0;
-      int n = 0;
+      int starts = 0, n = 0;
+      bool before = false;  // the tile before opened its piece
       for (int u = u_lo; u < u_hi && ok; ++u, ++n) {
         const bool start = n == 0 || cur.tile == 0;
         // A new piece's queries arrive after the last weights of the old one: take those first.
-        if (start && n > 0) second(n - 1);
+        if (start && n > 0) second(n - 1, before);
         if (start) {
-          ok = ok && mbar_wait(&c.q_full, starts & 1, s_abort);
+          ok = ok && __all_sync(~0u, bar_wait(&c.q_full, starts & 1, s_abort));
           ++starts;
         }
-        ok = ok && mbar_wait(&c.full[n % kStages], (n / kStages) & 1, s_abort);
+        const int stage = n % kStages;
+        ok = ok && __all_sync(~0u, bar_wait(&c.full[stage], (n / kStages) & 1, s_abort));
         if (!ok) break;
-        fence_proxy_async_smem();  // the copies wrote through the generic proxy
+        if constexpr (!kTma) fence_proxy_async_smem();  // cp.async writes through the generic proxy
         tc_fence_after();
-        const uint32_t kb = ring + (n % kStages) * stage_bytes;
+        const uint64_t kd = smem_desc(ring + stage * stage_bytes, 16, 1024);
         const uint32_t sd = tmem + S::kS + (n & 1) * kTok;
+        if (leader) {
 #pragma unroll
-        for (int ks = 0; ks < kDim / 16; ++ks)
-          tc_mma(sd, tmem + S::kQ + ks * 8, smem_desc(kb + (ks / 4) * S::kSub + (ks % 4) * 32, 16, 1024),
-                 kIdescS, ks > 0);
-        tc_commit(&c.s_full[n & 1]);
-        if (!start) second(n - 1);
-        first[n & 1] = start;
-        cur.next(p, plan, kTok, kBlockRows);
+          for (int ks = 0; ks < kDim / 16; ++ks)
+            tc_mma(sd, tmem + S::kQ + ks * 8, kd + (((ks / 4) * S::kSub + (ks % 4) * 32) >> 4), kIdescS,
+                   ks > 0);
+          tc_commit(&c.s_full[n & 1]);
+        }
+        __syncwarp();
+        if (!start) second(n - 1, before);
+        before = start;
+        cur.next(p, plan, kTok);
       }
-      if (ok && n > 0) second(n - 1);
+      if (ok && n > 0) second(n - 1, before);
       if (!ok) {  // let what is in flight land before the tensor memory is freed
-        tc_commit(&c.drain);
+        if (leader) tc_commit(&c.drain);
         const unsigned long long t0 = globaltimer_ns();
         while (!mbar_test(&c.drain, 0) && globaltimer_ns() - t0 < kPipeWaitNs) {
         }
@@ -564,7 +675,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
     auto sync_rows = [&] {
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.sync);
-      ok = mbar_wait(&c.sync, syncs++ & 1, s_abort) && ok;
+      ok = bar_wait(&c.sync, syncs++ & 1, s_abort) && ok;
       __syncwarp();
     };
 
@@ -579,24 +690,30 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
         m_ref = neg_inf();
         l = 0.f;
       }
-      ok = mbar_wait(&c.s_full[b], (i >> 1) & 1, s_abort);
+      ok = bar_wait(&c.s_full[b], (i >> 1) & 1, s_abort);
       // already complete: S was computed from this stage. Makes its flags and values visible here.
-      ok = ok && mbar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
+      ok = ok && bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
       if (!__all_sync(~0u, ok)) break;
       tc_fence_after();
       const bool bad_page = *const_cast<volatile int*>(&c.bad_unit[stage]) == u + 1;
       const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
-      auto sees = [&](int tok) {
-        bool see = tok < seen;
-        if (!see && branch) {
-          const int n = tok - base;
-          see = n >= 0 && n < 64 && tok < cur.len && ((branch >> n) & 1);
+      // Which of the 64 tokens from t0 on this row sees, one bit each.
+      auto visible = [&](int t0) {
+        auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+        unsigned long long bits = below(seen - t0);
+        if (branch) {
+          const int off = t0 - base;
+          const unsigned long long m = off >= 64 || off <= -64 ? 0ull : off >= 0 ? branch >> off : branch << -off;
+          bits |= m & below(cur.len - t0);
         }
-        if (see && bad_page) {
-          const int id = table[tok / p.page_size];
-          see = id >= 0 && id < p.total_pages;
+        if (bad_page) {
+#pragma unroll 1
+          for (int j = 0; j < 64 && t0 + j < cur.len; ++j) {
+            const int id = table[(t0 + j) / p.page_size];
+            if (id < 0 || id >= p.total_pages) bits &= ~(1ull << j);
+          }
         }
-        return see;
+        return bits;
       };
       // Some row of the block may not see a token of this tile (uniform over the block).
       const int sure = cur.seg == 0 ? cur.len : min(cur.len, p.tree ? base : base + 1);
@@ -613,10 +730,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
             tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[j]), t_s + h * 64 + j);
           tc_wait_ld();
           if (!plain) {
+            const unsigned long long bits = masked ? visible(tile0 + h * 64) : ~0ull;
+            const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
 #pragma unroll
             for (int j = 0; j < 64; ++j) {
               const float x = __uint_as_float(s[j]) * p.scale_log2;
-              s[j] = __float_as_uint(!masked || sees(tile0 + h * 64 + j) ? x : neg_inf());
+              s[j] = __float_as_uint((j < 32 ? lo >> j : hi >> (j - 32)) & 1u ? x : neg_inf());
             }
             __syncwarp();
           }
@@ -635,7 +754,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
           if (grow) m_ref = mx;
           l *= f;
           if (!piece_start) {
-            ok = mbar_wait(&c.o_done[b ^ 1], ((i - 1) >> 1) & 1, s_abort);
+            ok = bar_wait(&c.o_done[b ^ 1], ((i - 1) >> 1) & 1, s_abort);
             tc_fence_after();
             __syncwarp();
 #pragma unroll 1
@@ -668,47 +787,61 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tc_wait_st();
       }
-      // A masked tile of a request's own tokens may hold infinities or NaN that some rows do not
-      // see; 0 * NaN would carry them into those rows. They are replaced by zeros before the second
-      // product, and added afterwards to the rows that see them.
+      // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
+      // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
+      // that only some rows see are searched for infinities and NaN: those are replaced by zeros
+      // before the second product, and added afterwards to the rows that see them.
       bool poisoned = false;
-      if (masked && cur.seg) {
+      if (masked) {
         uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
-        bool found = false;
-        for (int x = threadIdx.x; x < S::kHalf / 16; x += kSoftWarps * 32) {
-          const uint4 w = *reinterpret_cast<const uint4*>(vt + x * 16);
-          found |= non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
-        }
-        if (found) *const_cast<volatile int*>(&c.bad_value) = u + 1;
-        sync_rows();
-        poisoned = *const_cast<volatile int*>(&c.bad_value) == u + 1;
-        if (poisoned) {
-          for (int x = threadIdx.x; x < kTok; x += kSoftWarps * 32) c.bad_token[x] = 0;
-          sync_rows();
-          for (int x = threadIdx.x; x < S::kHalf / 16; x += kSoftWarps * 32) {
-            uint4 w = *reinterpret_cast<const uint4*>(vt + x * 16);
-            if (!(non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w))) continue;
-            *const_cast<volatile unsigned char*>(&c.bad_token[(x / 8) % kTok]) = 1;
-            w = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z),
-                           finite_or_zero<T>(w.w));
-            *reinterpret_cast<uint4*>(vt + x * 16) = w;
-          }
+        const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
+        if (kTma && stored < kTok) {
+          const int n = (stored + p.box_rows - 1) / p.box_rows * p.box_rows - stored;
+          for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32)
+            *reinterpret_cast<uint4*>(vt + (x / 8 / n) * S::kSub + (stored + x / 8 % n) * 128 +
+                                      (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
+        }
+        const int from = max(sure - tile0, 0), n = stored - from;
+        if (n > 0) {
+          auto chunk = [&](int x) {
+            return reinterpret_cast<uint4*>(vt + (x / 8 / n) * S::kSub + (from + x / 8 % n) * 128 + (x & 7) * 16);
+          };
+          auto no_number = [](const uint4& w) {
+            return non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
+          };
+          bool found = false;
+          for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32) found |= no_number(*chunk(x));
+          if (found) *const_cast<volatile int*>(&c.bad_value) = u + 1;
           sync_rows();
+          poisoned = *const_cast<volatile int*>(&c.bad_value) == u + 1;
+          if (poisoned) {
+            for (int x = threadIdx.x; x < kTok; x += kSoftWarps * 32) c.bad_token[x] = 0;
+            sync_rows();
+            for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32) {
+              uint4 w = *chunk(x);
+              if (!no_number(w)) continue;
+              *const_cast<volatile unsigned char*>(&c.bad_token[from + x / 8 % n]) = 1;
+              *chunk(x) = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y),
+                                     finite_or_zero<T>(w.z), finite_or_zero<T>(w.w));
+            }
+            fence_proxy_async_smem();
+            sync_rows();
+          }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.p_full[b]);
       if (poisoned) {
-        ok = ok && mbar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
+        ok = ok && bar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
         tc_fence_after();
         __syncwarp();
         const int head = cur.group / cur.blocks;
         for (int x = 0; x < kTok && act_warp; ++x) {
           if (!*const_cast<volatile unsigned char*>(&c.bad_token[x])) continue;
           const int tok = tile0 + x, pg = tok / p.page_size;
-          const bool see = (int)threadIdx.x < rows_here && sees(tok);
+          const bool see = (int)threadIdx.x < rows_here && (visible(tok) & 1ull);
           const T* v = static_cast<const T*>(p.v) + table[pg] * p.vs[0] +
                        (tok - pg * p.page_size) * p.vs[1] + head * p.vs[2];
 #pragma unroll 1
@@ -739,9 +872,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
       // ---- end of a piece: the next one's queries first, then O out
       const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.group;
       const int done_rows = rows_here;
-      cur.next(p, plan, kTok, kBlockRows);
+      cur.next(p, plan, kTok);
       if (u + 1 < u_hi) open_piece();
-      ok = ok && mbar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
+      ok = ok && bar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
       tc_fence_after();
       __syncwarp();
       if (warp * 32 < done_rows) {
@@ -777,71 +910,83 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_kernel(const AttnArgs p)
 
 // ------------------------------------------------------------------------------------------------
 // Join: one block per (row, query head). The row's partials are those of its prefix group and of
-// its request's own group, each from a run of CTAs; they are added in that order.
+// its request's own group, each from a run of CTAs: partial j lies at slot
+// from + j (j < n0, the prefix's) or from1 + j - n0. Weights first, a thread per partial, then the
+// sum over partials in their order, a thread per dimension with its loads ahead of its sums.
 // ------------------------------------------------------------------------------------------------
+constexpr int kMaxPartials = 2 * kMaxCtas;
+
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, int tok, int grid) {
-  constexpr int block_rows = kBlockRows;
-  __shared__ Plan plan;
-  __shared__ int s_seg;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, int grid) {
+  __shared__ float s_w[kMaxPartials];
+  __shared__ int64_t s_at[kMaxPartials];
+  __shared__ float s_red[2][kJoinThreads / 32];
   const int t = blockIdx.x / p.q_heads, h = blockIdx.x - t * p.q_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_dep_wait();
   grid_dep_launch();
-  make_plan<kJoinThreads / 32>(p, tok, block_rows, plan);
-  if (threadIdx.x == 0) {
-    int seg = -1;
-    for (int b = 0; b < p.requests; ++b) {
-      int first, count;
-      request_rows(p, b, first, count);
-      if (t >= first && t < first + count) {
-        seg = b + 1;
-        break;
-      }
-    }
-    s_seg = seg;
-  }
-  __syncthreads();
-  const int seg = s_seg, units = plan.units_end[p.requests];
-  const int ctas = units > 0 ? plan_ctas(units, grid) : 1;
+  const RowPlan r = p.row_plan[t];
   const int head = h / p.group, g = h - head * p.group;
-  // the two runs of pieces: slots from[i] + 0 .. n[i] - 1, row[i] in each
-  int from[2], n[2], row[2];
+  int from[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0};
+  if (r.owned) {
+    const int ctas = plan_ctas(r.units, grid);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    n[i] = from[i] = row[i] = 0;
-    if (seg < 0) continue;
-    const int s = i == 0 ? 0 : seg;
-    int first, count, len, tiles, blocks;
-    segment_shape(p, s, tok, block_rows, first, count, len, tiles, blocks);
-    if (tiles == 0 || units == 0) continue;
-    const int f = (t - first) * p.group + g;
-    const int group = head * blocks + f / block_rows;
-    row[i] = f % block_rows;
-    const int u0 = (s ? plan.units_end[s - 1] : 0) + group * tiles;
-    const int c0 = plan_owner(units, ctas, u0), c1 = plan_owner(units, ctas, u0 + tiles - 1);
-    from[i] = c0 + (s ? plan.groups_end[s - 1] : 0) + group;
-    n[i] = min(c1 - c0 + 1, max(0, p.slots - from[i]));
-  }
-  float top = neg_inf();
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < n[i]; ++j)
-      top = fmaxf(top, p.part_ml[(int64_t)(from[i] + j) * block_rows + row[i]].x);
-  const float safe = top == neg_inf() ? 0.f : top;
-  float sum = 0.f, acc[2] = {0.f, 0.f};
-  const int d0 = threadIdx.x, d1 = threadIdx.x + kJoinThreads;
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < n[i]; ++j) {
-      const int64_t at = (int64_t)(from[i] + j) * block_rows + row[i];
-      const float2 ml = p.part_ml[at];
-      const float w = ex2(ml.x - safe);
-      sum += ml.y * w;
-      if (d0 < p.dim) acc[0] += p.part_o[at * p.dim + d0] * w;
-      if (d1 < p.dim) acc[1] += p.part_o[at * p.dim + d1] * w;
+    for (int i = 0; i < 2; ++i) {
+      const int tiles = i ? r.tiles : r.prefix_tiles, blocks = i ? r.blocks : r.prefix_blocks;
+      if (tiles == 0) continue;
+      const int f = (t - (i ? r.first : r.prefix_first)) * p.group + g;
+      const int group = head * blocks + f / kBlockRows;
+      row[i] = f % kBlockRows;
+      const int u0 = (i ? r.unit0 : 0) + group * tiles;
+      const int c0 = plan_owner(r.units, ctas, u0), c1 = plan_owner(r.units, ctas, u0 + tiles - 1);
+      from[i] = c0 + (i ? r.group0 : 0) + group;
+      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i]));
     }
+  }
+  const int total = n[0] + n[1];
+  float top = neg_inf();
+  for (int j = threadIdx.x; j < total; j += kJoinThreads) {
+    const int i = j >= n[0];
+    const int64_t at = (int64_t)(from[i] + j - (i ? n[0] : 0)) * kBlockRows + row[i];
+    const float m = p.part_ml[at].x;
+    s_at[j] = at;
+    s_w[j] = m;
+    top = fmaxf(top, m);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  if (lane == 0) s_red[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
+  const float safe = top == neg_inf() ? 0.f : top;
+  float sum = 0.f;
+  for (int j = threadIdx.x; j < total; j += kJoinThreads) {
+    const float w = ex2(s_w[j] - safe);
+    s_w[j] = w;
+    sum += p.part_ml[s_at[j]].y * w;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+  if (lane == 0) s_red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim;
-  if (d0 < p.dim) out[d0] = T(acc[0] * inv);
-  if (d1 < p.dim) out[d1] = T(acc[1] * inv);
+  for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
+    float acc = 0.f;
+    for (int j0 = 0; j0 < total; j0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j0 + j < total ? p.part_o[s_at[j0 + j] * p.dim + d] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < total) acc += x[j] * s_w[j0 + j];
+    }
+    out[d] = T(acc * inv);
+  }
   if (threadIdx.x == 0)
     p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
 }
@@ -852,11 +997,12 @@ int64_t slots_for(int requests, int rows, int group, int kv_heads) {
   return kMaxCtas + kv_heads * (2 * blocks + requests);
 }
 
-template <typename T, int kDim>
-int launch_typed(const AttnArgs& p, int ctas, cudaStream_t stream) {
+template <typename T, int kDim, bool kTma>
+int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& p, int ctas,
+                 cudaStream_t stream) {
   constexpr size_t smem = attn_smem<kDim>();
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  auto kernel = attn_kernel<T, kDim>;
+  auto kernel = attn_kernel<T, kDim, kTma>;
   static bool configured[64] = {};
   int dev = 0;
   B2_CUDA_TRY(cudaGetDevice(&dev));
@@ -864,18 +1010,48 @@ int launch_typed(const AttnArgs& p, int ctas, cudaStream_t stream) {
     B2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured[dev] = true;
   }
-  int rc = launch_kernel(kernel, ctas, kAttnThreads, smem, stream, /*early=*/true, p);
+  int rc = launch_kernel(kernel, ctas, attn_threads(kTma), smem, stream, /*early=*/true, mk, mv, p);
   if (rc) return rc;
   return launch_kernel(join_kernel<T>, p.rows * p.q_heads, kJoinThreads, 0, stream, /*early=*/true,
-                       p, Shape<kDim>::kTok, ctas);
+                       p, ctas);
+}
+
+// A cache as a tensor map (dimension, place in the page, head, page), boxes of box_rows tokens and
+// 64 dimensions. False where TMA cannot take it; the kernel then copies with cp.async.
+template <typename T>
+bool cache_map(CUtensorMap* map, const void* base, const int64_t* s, const AttnArgs& p) {
+  const uint64_t dims[4] = {(uint64_t)p.dim, (uint64_t)p.page_size, (uint64_t)p.kv_heads,
+                            (uint64_t)p.total_pages};
+  uint64_t strides[3] = {(uint64_t)s[1] * 2, (uint64_t)s[2] * 2, (uint64_t)s[0] * 2};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t e = i == 0 ? s[1] : i == 1 ? s[2] : s[0];
+    if (dims[i + 1] == 1) strides[i] = (uint64_t)p.dim * 2;  // never stepped
+    else if (e <= 0 || e >= (int64_t)1 << 38) return false;
+  }
+  const uint32_t box[4] = {64, (uint32_t)p.box_rows, 1, 1};
+  return encode_4d(map, Pair<T>::kFormat == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) == B2_OK;
+}
+
+// TMA where a page holds whole groups of 8 tokens (the rows of one swizzle pattern); a box then
+// never crosses a page.
+template <typename T, int kDim>
+int launch_dim(AttnArgs& p, int ctas, cudaStream_t stream) {
+  CUtensorMap mk = {}, mv = {};
+  p.box_rows = std::min(Shape<kDim>::kTok, p.page_size & -p.page_size);
+  if (p.box_rows >= 8 && p.dim >= 64 && cache_map<T>(&mk, p.k, p.ks, p) &&
+      cache_map<T>(&mv, p.v, p.vs, p))
+    return launch_typed<T, kDim, true>(mk, mv, p, ctas, stream);
+  return launch_typed<T, kDim, false>(mk, mv, p, ctas, stream);
 }
 
 template <typename T>
-int launch_dim(const AttnArgs& p, int ctas, cudaStream_t stream) {
+int launch_type(AttnArgs& p, int ctas, cudaStream_t stream) {
   switch (round_dim(p.dim)) {
-    case 64: return launch_typed<T, 64>(p, ctas, stream);
-    case 128: return launch_typed<T, 128>(p, ctas, stream);
-    default: return launch_typed<T, 256>(p, ctas, stream);
+    case 64: return launch_dim<T, 64>(p, ctas, stream);
+    case 128: return launch_dim<T, 128>(p, ctas, stream);
+    default: return launch_dim<T, 256>(p, ctas, stream);
   }
 }
 
@@ -895,12 +1071,27 @@ int check_shape(int requests, int rows, int q_heads, int kv_heads, int head_dim)
 }  // namespace
 }  // namespace b2
 
+extern "C" int b2_prefix_attn_status(int clear, int* device_status) {
+  using namespace b2;
+  if (!device_status) return fail(B2_ERR_INVALID_ARG, "prefix_attn_status: null output");
+  int v = 0;
+  B2_CUDA_TRY(cudaDeviceSynchronize());
+  B2_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attn_status, sizeof(v)));
+  if (clear && v) {
+    const int zero = 0;
+    B2_CUDA_TRY(cudaMemcpyToSymbol(g_attn_status, &zero, sizeof(zero)));
+  }
+  *device_status = v;
+  return B2_OK;
+}
+
 extern "C" size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, int kv_heads,
                                            int head_dim) {
   using namespace b2;
   if (check_shape(requests, rows, q_heads, kv_heads, head_dim)) return 0;
   const int64_t slots = slots_for(requests, rows, q_heads / kv_heads, kv_heads);
-  return (size_t)slots * kBlockRows * (head_dim * sizeof(float) + sizeof(float2)) + 256;
+  return (size_t)slots * kBlockRows * (head_dim * sizeof(float) + sizeof(float2)) +
+         (size_t)rows * sizeof(RowPlan) + 256;
 }
 
 extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
@@ -966,10 +1157,11 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.dim = head_dim;
   p.slots = (int)slots_for(requests, rows, group, kv_heads);
   p.scale_log2 = scale * kLog2e;
-  p.part_ml = static_cast<float2*>(ws);
-  const size_t ml_bytes = ((size_t)p.slots * kBlockRows * sizeof(float2) + 255) & ~(size_t)255;
+  p.row_plan = static_cast<RowPlan*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(p.row_plan + rows);
+  const size_t ml_bytes = ((size_t)rows * sizeof(RowPlan) + (size_t)p.slots * kBlockRows * sizeof(float2) + 255) & ~(size_t)255;
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + ml_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == B2_DTYPE_F16 ? launch_dim<__half>(p, ctas, s)
-                               : launch_dim<__nv_bfloat16>(p, ctas, s);
+  return dtype == B2_DTYPE_F16 ? launch_type<__half>(p, ctas, s)
+                               : launch_type<__nv_bfloat16>(p, ctas, s);
 }

@@ -39,6 +39,9 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uin
 // any order of size (a middle dimension may step further than the outer one).
 int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[3],
               const uint64_t strides_bytes[2], const uint32_t box[3], CUtensorMapSwizzle swizzle);
+// The same with four dimensions and the strides of dims 1 to 3.
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[4],
+              const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swizzle);
 
 // Workspace layout: [status words][tile counters][partial slots][row sums of the fused RMSNorm,
 // kMaxM floats per CTA].

@@ -81,8 +81,8 @@ namespace {
 struct MapKey {
   const void* base;
   int rank;
-  uint64_t dims[3], strides[2];
-  uint32_t box[3];
+  uint64_t dims[4], strides[3];
+  uint32_t box[4];
   int dtype, swizzle, device;
   bool operator==(const MapKey& o) const {
     if (base != o.base || rank != o.rank || dtype != o.dtype || swizzle != o.swizzle ||
@@ -116,8 +116,8 @@ size_t map_hash(const MapKey& k) {
 int encode_uncached(CUtensorMap* map, const MapKey& k) {
   auto fn = get_encode_fn();
   if (!fn) return fail(B2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[3] = {0, 0, 0}, strides[2] = {0, 0};
-  cuuint32_t box[3] = {0, 0, 0}, estr[3] = {1, 1, 1};
+  cuuint64_t dims[4] = {0, 0, 0, 0}, strides[3] = {0, 0, 0};
+  cuuint32_t box[4] = {0, 0, 0, 0}, estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < k.rank; ++i) {
     dims[i] = k.dims[i];
     box[i] = k.box[i];
@@ -181,6 +181,21 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, con
   }
   k.strides[0] = strides_bytes[0];
   k.strides[1] = strides_bytes[1];
+  k.dtype = (int)dtype;
+  k.swizzle = (int)swizzle;
+  return encode_cached(map, k);
+}
+
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[4],
+              const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swizzle) {
+  MapKey k = {};
+  k.base = base;
+  k.rank = 4;
+  for (int i = 0; i < 4; ++i) {
+    k.dims[i] = dims[i];
+    k.box[i] = box[i];
+    if (i < 3) k.strides[i] = strides_bytes[i];
+  }
   k.dtype = (int)dtype;
   k.swizzle = (int)swizzle;
   return encode_cached(map, k);

@@ -755,15 +755,19 @@ void nvar_set_timeout_ms(int64_t handle, int64_t ms) {
   TORCH_CHECK(rc == B2_OK, "nvar_set_timeout_ms: ", detail(rc));
 }
 
-// Status word of the current device's GEMM workspace (synchronises the device).
+// Status word of the current device's GEMM workspace, or else that of its attention calls
+// (synchronises the device).
 int64_t workspace_status(bool clear) {
   int dev = 0;
   TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess, "workspace_status: no CUDA device");
   void* ws = workspace(dev);
   int st = 0;
-  const int rc = b2_workspace_status(ws, clear ? 1 : 0, &st);
+  int rc = b2_workspace_status(ws, clear ? 1 : 0, &st);
   TORCH_CHECK(rc == B2_OK, "workspace_status: ", detail(rc));
-  return st;
+  int attn = 0;
+  rc = b2_prefix_attn_status(clear ? 1 : 0, &attn);
+  TORCH_CHECK(rc == B2_OK, "workspace_status: ", detail(rc));
+  return st ? st : attn;
 }
 
 void set_tuning(int64_t key, int64_t value) {
