@@ -33,6 +33,7 @@ constexpr int kSoftWarps = 4;      // one thread per row of a block
 constexpr int kLoadThreads = 128;
 constexpr int kBlockRows = 128;
 constexpr int kJoinThreads = 128;
+constexpr unsigned int kMaxPolls = 1u << 20;  // of two barriers in turn, before the wait with a clock
 constexpr int kMaxCtas = 160;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -331,7 +332,8 @@ struct Cursor {
 //              sum need no exchange between threads; they also bring Q in and take O out
 //   warp 4     issues the products: the first of tile i + 1 before the second of tile i, so that
 //              the tensor cores work while the softmax of tile i runs
-//   warp 5     (kTma) one TMA box per group of tokens of one page and 64 dimensions
+//   warps 5, 6 (kTma) K and V: one TMA box per group of tokens of one page and 64 dimensions; two
+//              warps, so that one's look-ups pass behind the other's copies
 //   warps 5-8  (otherwise) 16 bytes per cp.async, for any page size and strides
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the one its weights refer
 // to (the weights stay below 2^8, in range of fp16, with the same relative rounding); the sum l and
@@ -359,7 +361,7 @@ struct Control {
   unsigned char bad_token[128];
 };
 
-constexpr int attn_threads(bool tma) { return kSoftWarps * 32 + 32 + (tma ? 32 : kLoadThreads); }
+constexpr int attn_threads(bool tma) { return kSoftWarps * 32 + 32 + (tma ? 64 : kLoadThreads); }
 
 template <int kDim>
 constexpr size_t attn_smem() {
@@ -368,7 +370,7 @@ constexpr size_t attn_smem() {
 
 __device__ int g_attn_status;
 
-// mbar_wait without its suspend-time hint.
+// mbar_wait without its suspend-time hint: the waits of this kernel are short.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   if (mbar_test(bar, parity)) return true;
   const unsigned long long t0 = globaltimer_ns();
@@ -381,6 +383,18 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
   }
   *abort = 1;
   return false;
+}
+// Has the phase completed? Never suspends the thread.
+__device__ __forceinline__ bool mbar_test_now(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 template <typename T, int kDim, bool kTma>
@@ -397,9 +411,11 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
   volatile int* s_abort = &c.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (kTma && threadIdx.x >= (kSoftWarps + 1) * 32 && lane == 0)
+    tma_prefetch_desc(warp == kSoftWarps + 2 ? &map_v : &map_k);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&c.full[s], kTma ? 1 : kLoadThreads + kLoadThreads / 32);
+      mbar_init(&c.full[s], kTma ? 2 : kLoadThreads + kLoadThreads / 32);
       mbar_init(&c.empty[s], 1);
       c.bad_unit[s] = 0;
     }
@@ -436,12 +452,13 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
   if (!idle) cur.seek(p, plan, u_lo, kTok);
 
   if (kTma && warp > kSoftWarps) {
-    // ------------------------------------------------------------------------------ loader (TMA)
+    // ------------------------------------------------------------------------------ loaders (TMA)
     // Boxes of box_rows tokens x 64 dimensions. A box behind the length, or of a page that does not
     // exist, is loaded from behind the last page: zeros, without a read.
     const int groups = kTok / p.box_rows;  // a power of two, at most 16
-    constexpr int kSubs = kDim / 64;
-    const int boxes = groups * kSubs * 2;
+    const int boxes = groups * (kDim / 64);
+    const bool is_v = warp == kSoftWarps + 2;
+    const CUtensorMap* map = is_v ? &map_v : &map_k;
     const int row0 = (lane % groups) * p.box_rows;  // the same for all boxes of a lane
     int id = -1, at = 0;
     auto look_up = [&] {
@@ -454,10 +471,6 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
         at = tok - pg * p.page_size;
       }
     };
-    if (lane == 0) {
-      tma_prefetch_desc(&map_k);
-      tma_prefetch_desc(&map_v);
-    }
     const uint64_t once = l2_evict_first_policy(), again = l2_evict_normal_policy();
     if (!idle) look_up();
     int issued = 0;
@@ -473,12 +486,12 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       const int page = tok < len && exists ? raw : p.total_pages;
       if (tok < len && !exists) *const_cast<volatile int*>(&c.bad_unit[stage]) = u + 1;
       __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&c.full[stage], stage_bytes);
+      if (lane == 0) mbar_arrive_expect_tx(&c.full[stage], S::kHalf);
       __syncwarp();
+      uint8_t* dst = smem + stage * stage_bytes + (is_v ? S::kHalf : 0) + row0 * 128;
       for (int x = lane; x < boxes; x += 32) {
-        const int sub = (x / groups) % kSubs, is_v = x / (groups * kSubs);
-        uint8_t* dst = smem + stage * stage_bytes + is_v * S::kHalf + sub * S::kSub + row0 * 128;
-        tma_load_4d(dst, is_v ? &map_v : &map_k, &c.full[stage], sub * 64, tile_at, head, page, pol);
+        const int sub = x / groups;
+        tma_load_4d(dst + sub * S::kSub, map, &c.full[stage], sub * 64, tile_at, head, page, pol);
       }
       __syncwarp();
       issued = i + 1;
@@ -590,6 +603,14 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
           ++starts;
         }
         const int stage = n % kStages;
+        // While this tile's keys are on their way, the weights of the one before may be ready.
+        bool pending = !start;
+        for (unsigned int it = 0; pending && it < kMaxPolls; ++it) {
+          if (__any_sync(~0u, mbar_test_now(&c.full[stage], (n / kStages) & 1))) break;
+          if (!__any_sync(~0u, mbar_test_now(&c.p_full[(n - 1) & 1], ((n - 1) >> 1) & 1))) continue;
+          second(n - 1, before);
+          pending = false;
+        }
         ok = ok && __all_sync(~0u, bar_wait(&c.full[stage], (n / kStages) & 1, s_abort));
         if (!ok) break;
         if constexpr (!kTma) fence_proxy_async_smem();  // cp.async writes through the generic proxy
@@ -604,7 +625,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
           tc_commit(&c.s_full[n & 1]);
         }
         __syncwarp();
-        if (!start) second(n - 1, before);
+        if (pending) second(n - 1, before);
         before = start;
         cur.next(p, plan, kTok);
       }
@@ -643,26 +664,23 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       if (warp * 32 < rows_here) {
         const T* src = static_cast<const T*>(p.q) + (int64_t)t * p.q_row +
                        (int64_t)(head * p.group + (act ? f - local * p.group : 0)) * p.q_head;
+        uint32_t w[kDim / 2];  // all loads before the first store
+        if (p.q_vec) {
 #pragma unroll
-        for (int c0 = 0; c0 < kDim / 2; c0 += 32) {
-          uint32_t w[32];
-          if (p.q_vec) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int d = (c0 + 4 * j) * 2;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (act && d < p.dim) v = *reinterpret_cast<const uint4*>(src + d);
-              w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int d = (c0 + j) * 2;
-              w[j] = act && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-            }
+          for (int j = 0; j < kDim / 8; ++j) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (act && 8 * j < p.dim) v = *reinterpret_cast<const uint4*>(src + 8 * j);
+            w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
           }
-          tmem_st32(t_q + c0, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kDim / 2; ++j)
+            w[j] = act && 2 * j < p.dim ? *reinterpret_cast<const uint32_t*>(src + 2 * j) : 0u;
         }
+        __syncwarp();
+#pragma unroll
+        for (int c0 = 0; c0 < kDim / 2; c0 += 32)
+          tmem_st32(t_q + c0, *reinterpret_cast<const uint32_t(*)[32]>(&w[c0]));
         tc_wait_st();
       }
       tc_fence_before();
@@ -795,35 +813,36 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       if (masked) {
         uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
         const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
+        // a thread's chunk column, and every kPass-th token from its first
+        constexpr int kCols = kDim / 8, kPass = kSoftWarps * 32 / kCols;
+        const int col = threadIdx.x % kCols, tok0 = threadIdx.x / kCols;
+        uint8_t* column = vt + (col / 8) * S::kSub + (col & 7) * 16;
         if (kTma && stored < kTok) {
-          const int n = (stored + p.box_rows - 1) / p.box_rows * p.box_rows - stored;
-          for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32)
-            *reinterpret_cast<uint4*>(vt + (x / 8 / n) * S::kSub + (stored + x / 8 % n) * 128 +
-                                      (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+          const int end = (stored + p.box_rows - 1) & -p.box_rows;
+          for (int r = stored + tok0; r < end; r += kPass)
+            *reinterpret_cast<uint4*>(column + r * 128) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
         }
-        const int from = max(sure - tile0, 0), n = stored - from;
-        if (n > 0) {
-          auto chunk = [&](int x) {
-            return reinterpret_cast<uint4*>(vt + (x / 8 / n) * S::kSub + (from + x / 8 % n) * 128 + (x & 7) * 16);
-          };
+        const int from = max(sure - tile0, 0);
+        if (from < stored) {
           auto no_number = [](const uint4& w) {
             return non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
           };
           bool found = false;
-          for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32) found |= no_number(*chunk(x));
+          for (int r = from + tok0; r < stored; r += kPass)
+            found |= no_number(*reinterpret_cast<const uint4*>(column + r * 128));
           if (found) *const_cast<volatile int*>(&c.bad_value) = u + 1;
           sync_rows();
           poisoned = *const_cast<volatile int*>(&c.bad_value) == u + 1;
           if (poisoned) {
             for (int x = threadIdx.x; x < kTok; x += kSoftWarps * 32) c.bad_token[x] = 0;
             sync_rows();
-            for (int x = threadIdx.x; x < n * (kDim / 8); x += kSoftWarps * 32) {
-              uint4 w = *chunk(x);
+            for (int r = from + tok0; r < stored; r += kPass) {
+              uint4& w = *reinterpret_cast<uint4*>(column + r * 128);
               if (!no_number(w)) continue;
-              *const_cast<volatile unsigned char*>(&c.bad_token[from + x / 8 % n]) = 1;
-              *chunk(x) = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y),
-                                     finite_or_zero<T>(w.z), finite_or_zero<T>(w.w));
+              *const_cast<volatile unsigned char*>(&c.bad_token[r]) = 1;
+              w = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z),
+                             finite_or_zero<T>(w.w));
             }
             fence_proxy_async_smem();
             sync_rows();
