@@ -32,7 +32,6 @@ constexpr int kMaxRows = 4096;
 constexpr int kSoftWarps = 4;      // one thread per row of a block
 constexpr int kLoadThreads = 128;
 constexpr int kBlockRows = 128;
-constexpr int kJoinThreads = 128;
 constexpr unsigned int kMaxPolls = 1u << 20;  // of two barriers in turn, before the wait with a clock
 constexpr int kMaxCtas = 160;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -47,6 +46,23 @@ struct RowPlan {
   int owned;                        // the row belongs to a request
   int pad[2];
 };
+
+// Division of 0 <= n < 2^31 by a number fixed for the launch, as a product and a shift (Granlund and
+// Montgomery, Division by Invariant Integers using Multiplication, 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+  }
+};
+FastDiv make_div(int d) {
+  FastDiv f;
+  f.d = (uint32_t)d;
+  f.shift = 0;
+  while ((1ll << f.shift) < d) ++f.shift;
+  f.mul = (uint32_t)((((1ull << f.shift) - (uint64_t)d) << 32) / (uint64_t)d + 1);
+  return f;
+}
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -65,6 +81,7 @@ struct AttnArgs {
   int slots;
   int q_vec;     // queries allow 16-byte loads
   int box_rows;  // tokens per TMA box: a power of two that divides the page size
+  FastDiv by_page, by_group;
   float scale_log2;
 };
 
@@ -106,6 +123,15 @@ template <typename T>
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   constexpr uint32_t e = Pair<T>::kExp;
   return ((w & e) == e ? 0u : w & 0xffffu) | (((w >> 16) & e) == e ? 0u : w & 0xffff0000u);
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+// 32 bytes, a whole sector, in one store.
+__device__ __forceinline__ void st_256(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 // 16 bytes from global to shared memory; `bytes` = 16, or 0 to write zeros without reading.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -286,15 +312,16 @@ __device__ __forceinline__ int plan_owner(int units, int ctas, int u) {
   return (int)((((int64_t)u + 1) * ctas - 1) / units);
 }
 
-// A position in the unit order: segment, group inside it (head-major), tile.
+// A position in the unit order: segment, head, row block, tile. A group is a (head, row block).
 struct Cursor {
-  int seg, group, tile;  // group = head * blocks + row block
+  int seg, head, block, tile;
   int first, count, len, tiles, blocks;
   __device__ __forceinline__ void load(const AttnArgs& p, const Plan& plan, int tok) {
     first = plan.first[seg], count = plan.count[seg], len = plan.len[seg];
     tiles = (len + tok - 1) / tok;
     blocks = blocks_of(count, p.group);
   }
+  __device__ __forceinline__ int group() const { return head * blocks + block; }
   __device__ __forceinline__ void seek(const AttnArgs& p, const Plan& plan, int u, int tok) {
     int lo = 0, hi = p.requests;
     while (lo < hi) {
@@ -303,15 +330,18 @@ struct Cursor {
     }
     seg = lo;
     load(p, plan, tok);
-    const int local = u - (seg ? plan.units_end[seg - 1] : 0);
-    group = local / tiles;
-    tile = local - group * tiles;
+    const int local = u - (seg ? plan.units_end[seg - 1] : 0), g = local / tiles;
+    tile = local - g * tiles;
+    head = blocks == 1 ? g : g / blocks;
+    block = g - head * blocks;
   }
   __device__ __forceinline__ void next(const AttnArgs& p, const Plan& plan, int tok) {
     if (++tile < tiles) return;
     tile = 0;
-    if (++group < p.kv_heads * blocks) return;
-    group = 0;
+    if (++block < blocks) return;
+    block = 0;
+    if (++head < p.kv_heads) return;
+    head = 0;
     const int done = plan.units_end[seg];
     while (seg < p.requests && plan.units_end[seg + 1] == done) ++seg;
     if (seg < p.requests) {
@@ -433,6 +463,12 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     mbar_fence_init();
   }
   if (warp == kSoftWarps) tmem_alloc(&c.tmem, S::kColumns);
+  {  // page tables into L2 behind the plan
+    const int line = 32, step = gridDim.x * blockDim.x * line, at = (blockIdx.x * blockDim.x + threadIdx.x) * line;
+    for (int i = at; i < p.n_prefix_pages; i += step) prefetch_l2(p.prefix_pages + i);
+    const int64_t all = p.requests > 0 ? (p.requests - 1) * p.pages_stride + p.max_pages : 0;
+    for (int64_t i = at; i < all; i += step) prefetch_l2(p.pages + i);
+  }
   grid_dep_wait();
   grid_dep_launch();
   make_plan(p, kTok, plan);
@@ -453,20 +489,21 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
 
   if (kTma && warp > kSoftWarps) {
     // ------------------------------------------------------------------------------ loaders (TMA)
-    // Boxes of box_rows tokens x 64 dimensions. A box behind the length, or of a page that does not
+    // Boxes of box_rows tokens x 64 dimensions, their pages looked up by a lane each. A box behind the length, or of a page that does not
     // exist, is loaded from behind the last page: zeros, without a read.
     const int groups = kTok / p.box_rows;  // a power of two, at most 16
-    const int boxes = groups * (kDim / 64);
+    const int box_bytes = p.box_rows * 128;
+    const bool leader = elect_one();
     const bool is_v = warp == kSoftWarps + 2;
     const CUtensorMap* map = is_v ? &map_v : &map_k;
-    const int row0 = (lane % groups) * p.box_rows;  // the same for all boxes of a lane
+    const int row0 = (lane & (groups - 1)) * p.box_rows;
     int id = -1, at = 0;
     auto look_up = [&] {
       const int tok = cur.tile * kTok + row0;
       id = -1, at = 0;
       if (tok < cur.len) {
         const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
-        const int pg = tok / p.page_size;
+        const int pg = p.by_page.div(tok);
         id = table[pg];
         at = tok - pg * p.page_size;
       }
@@ -476,7 +513,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     int issued = 0;
     for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
       const int stage = i % kStages;
-      const int head = cur.group / cur.blocks, tok = cur.tile * kTok + row0, len = cur.len;
+      const int head = cur.head, tok = cur.tile * kTok + row0, len = cur.len;
       const uint64_t pol = cur.blocks > 1 ? again : once;
       const int raw = id, tile_at = at;
       cur.next(p, plan, kTok);
@@ -486,12 +523,18 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       const int page = tok < len && exists ? raw : p.total_pages;
       if (tok < len && !exists) *const_cast<volatile int*>(&c.bad_unit[stage]) = u + 1;
       __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&c.full[stage], S::kHalf);
-      __syncwarp();
-      uint8_t* dst = smem + stage * stage_bytes + (is_v ? S::kHalf : 0) + row0 * 128;
-      for (int x = lane; x < boxes; x += 32) {
-        const int sub = x / groups;
-        tma_load_4d(dst + sub * S::kSub, map, &c.full[stage], sub * 64, tile_at, head, page, pol);
+      // One lane issues every box, with operands that are the same in the whole warp.
+      const uint32_t dst = ring + stage * stage_bytes + (is_v ? S::kHalf : 0);
+      if (leader) mbar_arrive_expect_tx(&c.full[stage], S::kHalf);
+#pragma unroll 1
+      for (int g = 0; g < groups; ++g) {
+        const int pid = __shfl_sync(~0u, page, g), pat = __shfl_sync(~0u, tile_at, g);
+        if (leader) {
+#pragma unroll
+          for (int sub = 0; sub < kDim / 64; ++sub)
+            tma_load_4d(dst + g * box_bytes + sub * S::kSub, map, &c.full[stage], sub * 64, pat, head,
+                        pid, pol);
+        }
       }
       __syncwarp();
       issued = i + 1;
@@ -521,7 +564,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       const int tok = cur.tile * kTok + my_row;
       if (my_row < kTok && tok < cur.len) {
         const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
-        const int pg = tok / p.page_size;
+        const int pg = p.by_page.div(tok);
         id = table[pg];
         at = tok - pg * p.page_size;
         if (id < 0 || id >= p.total_pages) id = -2;
@@ -531,7 +574,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     if (!idle) look_up(id, at);
     for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
       const int stage = i % kStages;
-      const int head = cur.group / cur.blocks;
+      const int head = cur.head;
       const int tile_id = id, tile_at = at;
       const T* kc = static_cast<const T*>(p.k) + head * p.ks[2] + chunk * 8;
       const T* vc = static_cast<const T*>(p.v) + head * p.vs[2] + chunk * 8;
@@ -648,12 +691,12 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     unsigned long long branch = 0;
     // Queries of the piece at the cursor into tensor memory.
     auto open_piece = [&] {
-      const int head = cur.group / cur.blocks, block = cur.group - head * cur.blocks;
+      const int head = cur.head, block = cur.block;
       rows_here = min(kBlockRows, cur.count * p.group - block * kBlockRows);
       base = cur.len - cur.count;
       const int f = block * kBlockRows + threadIdx.x;
       const bool act = (int)threadIdx.x < rows_here;
-      const int local = act ? f / p.group : 0;
+      const int local = act ? p.by_group.div(f) : 0;
       const int t = cur.first + local;
       seen = !act ? 0x7fffffff : cur.seg == 0 ? cur.len : min(cur.len, base + local + 1);
       branch = 0;
@@ -727,7 +770,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
         if (bad_page) {
 #pragma unroll 1
           for (int j = 0; j < 64 && t0 + j < cur.len; ++j) {
-            const int id = table[(t0 + j) / p.page_size];
+            const int id = table[p.by_page.div(t0 + j)];
             if (id < 0 || id >= p.total_pages) bits &= ~(1ull << j);
           }
         }
@@ -856,10 +899,10 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
         ok = ok && bar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
         tc_fence_after();
         __syncwarp();
-        const int head = cur.group / cur.blocks;
+        const int head = cur.head;
         for (int x = 0; x < kTok && act_warp; ++x) {
           if (!*const_cast<volatile unsigned char*>(&c.bad_token[x])) continue;
-          const int tok = tile0 + x, pg = tok / p.page_size;
+          const int tok = tile0 + x, pg = p.by_page.div(tok);
           const bool see = (int)threadIdx.x < rows_here && (visible(tok) & 1ull);
           const T* v = static_cast<const T*>(p.v) + table[pg] * p.vs[0] +
                        (tok - pg * p.page_size) * p.vs[1] + head * p.vs[2];
@@ -889,7 +932,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
         continue;
       }
       // ---- end of a piece: the next one's queries first, then O out
-      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.group;
+      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.group();
       const int done_rows = rows_here;
       cur.next(p, plan, kTok);
       if (u + 1 < u_hi) open_piece();
@@ -906,9 +949,8 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
           tmem_ld32(w, t_o + c0);
           tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            if (act && c0 + j < p.dim)
-              *reinterpret_cast<uint4*>(dst + c0 + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+          for (int j = 0; j < 32; j += 8)
+            if (act && c0 + j < p.dim) st_256(dst + c0 + j, &w[j]);
         }
         if (act) p.part_ml[at] = make_float2(m_ref, l);
       }
@@ -929,23 +971,27 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
 
 // ------------------------------------------------------------------------------------------------
 // Join: one block per (row, query head). The row's partials are those of its prefix group and of
-// its request's own group, each from a run of CTAs: partial j lies at slot
-// from + j (j < n0, the prefix's) or from1 + j - n0. Weights first, a thread per partial, then the
-// sum over partials in their order, a thread per dimension with its loads ahead of its sums.
+// its request's own group, each from a run of CTAs: partial j lies at slot from[0] + j for the first
+// n[0], at from[1] + j - n[0] for the others. kThreads / kCols threads take the partials in turn, a
+// thread four dimensions of each; the first loads of O are on their way before the weights are
+// known. Sums run over fixed sets in a fixed order.
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxPartials = 2 * kMaxCtas;
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, int grid) {
+template <typename T, int kCols, int kThreads>
+__global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int grid) {
+  constexpr int kWarps = kThreads / 32, kTeams = kThreads / kCols, kAhead = 4;
   __shared__ float s_w[kMaxPartials];
-  __shared__ int64_t s_at[kMaxPartials];
-  __shared__ float s_red[2][kJoinThreads / 32];
+  __shared__ float s_red[2][kWarps];
+  __shared__ float4 s_acc[kThreads];
   const int t = blockIdx.x / p.q_heads, h = blockIdx.x - t * p.q_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = threadIdx.x % kCols, team = threadIdx.x / kCols;
+  const bool col_in = col * 4 < p.dim;
   grid_dep_wait();
   grid_dep_launch();
   const RowPlan r = p.row_plan[t];
-  const int head = h / p.group, g = h - head * p.group;
+  const int head = p.by_group.div(h), g = h - head * p.group;
   int from[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0};
   if (r.owned) {
     const int ctas = plan_ctas(r.units, grid);
@@ -963,27 +1009,45 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, in
     }
   }
   const int total = n[0] + n[1];
+  auto place = [&](int j) {
+    const bool own = j >= n[0];
+    return (int64_t)(own ? from[1] + j - n[0] : from[0] + j) * kBlockRows + (own ? row[1] : row[0]);
+  };
+  float4 x[kAhead];
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = j0 + k * kTeams;
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < total && col_in) x[k] = *reinterpret_cast<const float4*>(p.part_o + place(j) * p.dim + col * 4);
+    }
+  };
+  constexpr int kMine = (kMaxPartials + kThreads - 1) / kThreads;
+  float2 ml[kMine];
   float top = neg_inf();
-  for (int j = threadIdx.x; j < total; j += kJoinThreads) {
-    const int i = j >= n[0];
-    const int64_t at = (int64_t)(from[i] + j - (i ? n[0] : 0)) * kBlockRows + row[i];
-    const float m = p.part_ml[at].x;
-    s_at[j] = at;
-    s_w[j] = m;
-    top = fmaxf(top, m);
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int j = threadIdx.x + k * kThreads;
+    ml[k] = make_float2(neg_inf(), 0.f);
+    if (j < total) ml[k] = p.part_ml[place(j)];
   }
+  fetch(team);
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) top = fmaxf(top, ml[k].x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   if (lane == 0) s_red[0][warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[0][w]);
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_red[0][w]);
   const float safe = top == neg_inf() ? 0.f : top;
   float sum = 0.f;
-  for (int j = threadIdx.x; j < total; j += kJoinThreads) {
-    const float w = ex2(s_w[j] - safe);
-    s_w[j] = w;
-    sum += p.part_ml[s_at[j]].y * w;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int j = threadIdx.x + k * kThreads;
+    const float w = ex2(ml[k].x - safe);
+    if (j < total) s_w[j] = w;
+    sum += ml[k].y * w;
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
@@ -991,20 +1055,28 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs p, in
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[1][w];
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim;
-  for (int d = threadIdx.x; d < p.dim; d += kJoinThreads) {
-    float acc = 0.f;
-    for (int j0 = 0; j0 < total; j0 += 8) {
-      float x[8];
+  for (int w = 0; w < kWarps; ++w) sum += s_red[1][w];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = team; j0 < total; j0 += kAhead * kTeams) {
+    if (j0 != team) fetch(j0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j0 + j < total ? p.part_o[s_at[j0 + j] * p.dim + d] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < total) acc += x[j] * s_w[j0 + j];
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = j0 + k * kTeams;
+      if (j >= total) continue;
+      const float w = s_w[j];
+      acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
     }
-    out[d] = T(acc * inv);
+  }
+  s_acc[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x < kCols && col_in) {
+    for (int k = 1; k < kTeams; ++k) {
+      const float4 y = s_acc[k * kCols + threadIdx.x];
+      acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim + col * 4;
+    out[0] = T(acc.x * inv), out[1] = T(acc.y * inv), out[2] = T(acc.z * inv), out[3] = T(acc.w * inv);
   }
   if (threadIdx.x == 0)
     p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
@@ -1031,8 +1103,12 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& p
   }
   int rc = launch_kernel(kernel, ctas, attn_threads(kTma), smem, stream, /*early=*/true, mk, mv, p);
   if (rc) return rc;
-  return launch_kernel(join_kernel<T>, p.rows * p.q_heads, kJoinThreads, 0, stream, /*early=*/true,
-                       p, ctas);
+  // Partials of a row: about as many as CTAs per group. Few of them: few threads.
+  const int64_t groups = (int64_t)p.kv_heads * (((int64_t)p.rows * p.group + kBlockRows - 1) / kBlockRows);
+  const int grid = p.rows * p.q_heads;
+  if (ctas / groups <= 8)
+    return launch_kernel(join_kernel<T, kDim / 4, 128>, grid, 128, 0, stream, /*early=*/true, p, ctas);
+  return launch_kernel(join_kernel<T, kDim / 4, 512>, grid, 512, 0, stream, /*early=*/true, p, ctas);
 }
 
 // A cache as a tensor map (dimension, place in the page, head, page), boxes of box_rows tokens and
@@ -1148,8 +1224,9 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
       return fail(B2_ERR_INVALID_ARG, "%s: cache strides must be multiples of 8 elements", op);
   const size_t need = b2_prefix_attn_workspace(requests, rows, q_heads, kv_heads, head_dim);
-  if (!ws || ws_bytes < need || !aligned16(ws))
-    return fail(B2_ERR_WORKSPACE, "%s: workspace of %zu B, need %zu B", op, ws_bytes, need);
+  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
+    return fail(B2_ERR_WORKSPACE, "%s: workspace of %zu B, need %zu B, 256-byte aligned", op, ws_bytes,
+                need);
   const int group = q_heads / kv_heads;
   const int tok = round_dim(head_dim) == 64 ? 128 : 64;
   // units are counted in 32 bits
@@ -1171,6 +1248,7 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.q_vec = aligned16(q) && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0;
   p.pages_stride = pages_stride;
   p.total_pages = total_pages, p.page_size = page_size;
+  p.by_page = make_div(page_size), p.by_group = make_div(group);
   p.n_prefix_pages = n_prefix_pages, p.max_pages = max_pages;
   p.requests = requests, p.rows = rows, p.q_heads = q_heads, p.kv_heads = kv_heads, p.group = group;
   p.dim = head_dim;
