@@ -8,12 +8,12 @@
 // A row that sees nothing gives out = 0 and lse = -inf.
 //
 // The rows' queries of one KV head form the M side of the products: T*G rows for the prefix, which
-// is read once for all of them, and n_b*G for a request's own tokens. Work is counted in units of
-// one tile of kTok tokens for one block of rows and one KV head, over all segments (segment 0 =
-// the prefix, segment b+1 = request b's own tokens). A persistent grid takes equal contiguous
-// ranges of units, whatever the lengths on the device say, so a captured graph follows growing
-// lengths. A range's piece of one (segment, head, row block) group ends in an unnormalised fp32
-// partial (O, m, l) in the workspace, at slot cta + group (no two pieces share one); a second
+// is read once for all of them (up to 256; beyond, once per 256), and n_b*G for a request's own
+// tokens. A persistent grid takes equal contiguous ranges of work, counted in tiles of kTok tokens
+// for one group of rows and one KV head over all segments (segment 0 = the prefix, segment b+1 =
+// request b's own tokens), whatever the lengths on the device say, so a captured graph follows
+// growing lengths. A range's piece of one (segment, head, rows) group ends in unnormalised fp32
+// partials (O, m, l) in the workspace, at slot cta + group (no two pieces share one); a second
 // launch joins the partials of each row in a fixed order, so results do not depend on timing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -29,9 +29,8 @@ namespace {
 
 constexpr int kMaxRequests = 1024;
 constexpr int kMaxRows = 4096;
-constexpr int kSoftWarps = 4;      // one thread per row of a block
 constexpr int kLoadThreads = 128;
-constexpr int kBlockRows = 128;
+constexpr int kBlockRows = 128;  // rows of one product: the lanes of tensor memory
 constexpr unsigned int kMaxPolls = 1u << 20;  // of two barriers in turn, before the wait with a clock
 constexpr int kMaxCtas = 160;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -39,11 +38,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // Where the partials of a row are: written by the main launch, read by the one that joins them.
 struct RowPlan {
-  int units;                        // of the whole call
-  int prefix_tiles, prefix_blocks, prefix_first;
-  int tiles, blocks, first;         // of the row's request; tiles = 0: none
-  int unit0, group0;                // units and groups before the request's
-  int owned;                        // the row belongs to a request
+  int cost;                                       // of the whole call
+  int prefix_tiles, prefix_first, prefix_count;   // of the prefix
+  int tiles, first, count;                        // of the row's request; tiles = 0: none
+  int cost0, group0;                              // cost and groups before the request's
+  int owned;                                      // the row belongs to a request
   int pad[2];
 };
 
@@ -72,8 +71,8 @@ struct AttnArgs {
   const int64_t* tree;
   void* out;
   float* lse;
-  float* part_o;    // [slots][rows per block][dim]
-  float2* part_ml;  // [slots][rows per block]
+  float* part_o;    // [slots][chains][rows per block][dim]
+  float2* part_ml;  // [slots][chains][rows per block]
   RowPlan* row_plan;  // [rows]
   int64_t pages_stride;
   int total_pages, page_size, n_prefix_pages, max_pages;
@@ -226,23 +225,37 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 }
 
 // ------------------------------------------------------------------------------------------------
-// The plan: every block derives it from the lengths on the device.
+// The plan: every block derives it from the lengths on the device. A group is kChains blocks of rows
+// of one head and segment. A tile of a segment with more than one block of rows costs 3, any other
+// 2: with two chains the tensor cores and the softmax then take longer than the copies.
 // ------------------------------------------------------------------------------------------------
 struct Plan {
-  int units_end[kMaxRequests + 1];   // running sum of units up to and with segment s
+  int cost_end[kMaxRequests + 1];    // running sum of costs up to and with segment s
   int groups_end[kMaxRequests + 1];  // running sum of groups
   int first[kMaxRequests + 1];       // first row of the segment
   int count[kMaxRequests + 1];       // and how many
   int len[kMaxRequests + 1];         // tokens
 };
+constexpr int kMaxWeight = 3;
 
-__device__ __forceinline__ int blocks_of(int count, int group) {
-  return (count * group + kBlockRows - 1) / kBlockRows;
+template <int kChains>
+__device__ __forceinline__ int groups_of(int count, int group) {
+  return (count * group + kChains * kBlockRows - 1) / (kChains * kBlockRows);
+}
+template <int kChains>
+__device__ __forceinline__ int weight_of(int count, int group) {
+  return kChains > 1 && count * group > kBlockRows ? kMaxWeight : 2;
+}
+// Rows of group g of a segment.
+template <int kChains>
+__device__ __forceinline__ int group_rows(int count, int group, int g) {
+  return min(kChains * kBlockRows, count * group - g * kChains * kBlockRows);
 }
 
 // Lengths and rows of every segment, cut at the tables and at the rows there are, and the running
 // sums. Row starts that decrease are outside the contract: the plan is then empty (every output 0,
 // lse -inf), so that no index leaves its array. Ends with a block-wide barrier.
+template <int kChains>
 __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan) {
   int bad = 0;
   for (int s = threadIdx.x; s <= p.requests; s += blockDim.x) {
@@ -257,22 +270,22 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
   }
   bad = __syncthreads_or(bad);
   if (threadIdx.x < 32) {
-    int u_base = 0, g_base = 0;
+    int c_base = 0, g_base = 0;
     for (int s0 = 0; s0 <= p.requests; s0 += 32) {
       const int s = s0 + threadIdx.x;
-      int u = 0, g = 0;
+      int c = 0, g = 0;
       if (s <= p.requests && !bad && plan.len[s] > 0) {
-        g = p.kv_heads * blocks_of(plan.count[s], p.group);
-        u = g * ((plan.len[s] + tok - 1) / tok);
+        g = p.kv_heads * groups_of<kChains>(plan.count[s], p.group);
+        c = g * ((plan.len[s] + tok - 1) / tok) * weight_of<kChains>(plan.count[s], p.group);
       }
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
-        const int uu = __shfl_up_sync(~0u, u, d), gg = __shfl_up_sync(~0u, g, d);
-        if ((int)threadIdx.x >= d) u += uu, g += gg;
+        const int cc = __shfl_up_sync(~0u, c, d), gg = __shfl_up_sync(~0u, g, d);
+        if ((int)threadIdx.x >= d) c += cc, g += gg;
       }
-      u += u_base, g += g_base;
-      if (s <= p.requests) plan.units_end[s] = u, plan.groups_end[s] = g;
-      u_base = __shfl_sync(~0u, u, 31);
+      c += c_base, g += g_base;
+      if (s <= p.requests) plan.cost_end[s] = c, plan.groups_end[s] = g;
+      c_base = __shfl_sync(~0u, c, 31);
       g_base = __shfl_sync(~0u, g, 31);
     }
   }
@@ -282,72 +295,90 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
 // The plan of row t for the launch that joins its partials.
 __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const Plan& plan, int t) {
   RowPlan r = {};
-  r.units = plan.units_end[p.requests];
+  r.cost = plan.cost_end[p.requests];
   r.prefix_tiles = (plan.len[0] + tok - 1) / tok;
-  r.prefix_blocks = blocks_of(plan.count[0], p.group);
   r.prefix_first = plan.first[0];
+  r.prefix_count = plan.count[0];
   // the last request that starts at or before t: requests without rows share a start with the next
   int lo = 0, hi = p.requests;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (plan.first[mid] <= t) lo = mid; else hi = mid - 1;
   }
-  if (r.units > 0 && lo > 0 && t < plan.first[lo] + plan.count[lo]) {
+  if (r.cost > 0 && lo > 0 && t < plan.first[lo] + plan.count[lo]) {
     r.owned = 1;
     r.tiles = (plan.len[lo] + tok - 1) / tok;
-    r.blocks = blocks_of(plan.count[lo], p.group);
     r.first = plan.first[lo];
-    r.unit0 = plan.units_end[lo - 1];
+    r.count = plan.count[lo];
+    r.cost0 = plan.cost_end[lo - 1];
     r.group0 = plan.groups_end[lo - 1];
   }
   p.row_plan[t] = r;
 }
 
-// CTAs that share `units` units: at most `ctas`, none of them empty.
-__device__ __forceinline__ int plan_ctas(int units, int ctas) { return min(units, ctas); }
-__device__ __forceinline__ int plan_begin(int units, int ctas, int c) {
-  return (int)((int64_t)units * c / ctas);
+// CTAs that share a cost: each range is at least one tile wide, so that the tiles that start in it
+// are at least one. A tile belongs to the CTA in whose range it starts.
+__device__ __forceinline__ int plan_ctas(int cost, int ctas) {
+  return max(1, min(cost / kMaxWeight, ctas));
 }
-__device__ __forceinline__ int plan_owner(int units, int ctas, int u) {
-  return (int)((((int64_t)u + 1) * ctas - 1) / units);
+__device__ __forceinline__ int plan_begin(int cost, int ctas, int c) {
+  return (int)((int64_t)cost * c / ctas);
+}
+__device__ __forceinline__ int plan_owner(int cost, int ctas, int at) {
+  return (int)((((int64_t)at + 1) * ctas - 1) / cost);
 }
 
-// A position in the unit order: segment, head, row block, tile. A group is a (head, row block).
+// A position in the order of tiles: segment, head, group, tile.
+template <int kChains>
 struct Cursor {
-  int seg, head, block, tile;
-  int first, count, len, tiles, blocks;
+  int seg, head, group, tile, at;  // at: the cost before it
+  int first, count, len, tiles, groups, weight;
   __device__ __forceinline__ void load(const AttnArgs& p, const Plan& plan, int tok) {
     first = plan.first[seg], count = plan.count[seg], len = plan.len[seg];
     tiles = (len + tok - 1) / tok;
-    blocks = blocks_of(count, p.group);
+    groups = groups_of<kChains>(count, p.group);
+    weight = weight_of<kChains>(count, p.group);
   }
-  __device__ __forceinline__ int group() const { return head * blocks + block; }
-  __device__ __forceinline__ void seek(const AttnArgs& p, const Plan& plan, int u, int tok) {
+  __device__ __forceinline__ int index() const { return head * groups + group; }  // in the segment
+  __device__ __forceinline__ int rows(const AttnArgs& p) const {
+    return group_rows<kChains>(count, p.group, group);
+  }
+  // The first tile at or behind cost c.
+  __device__ __forceinline__ void seek(const AttnArgs& p, const Plan& plan, int c, int tok) {
     int lo = 0, hi = p.requests;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (plan.units_end[mid] > u) hi = mid; else lo = mid + 1;
+      if (plan.cost_end[mid] > c) hi = mid; else lo = mid + 1;
     }
     seg = lo;
     load(p, plan, tok);
-    const int local = u - (seg ? plan.units_end[seg - 1] : 0), g = local / tiles;
-    tile = local - g * tiles;
-    head = blocks == 1 ? g : g / blocks;
-    block = g - head * blocks;
+    const int start = seg ? plan.cost_end[seg - 1] : 0, n = (c - start + weight - 1) / weight;
+    at = start + n * weight;
+    const int g = n / tiles;
+    tile = n - g * tiles;
+    head = groups == 1 ? g : g / groups;
+    group = g - head * groups;
+    if (head == p.kv_heads) next_segment(p, plan, tok);
   }
-  __device__ __forceinline__ void next(const AttnArgs& p, const Plan& plan, int tok) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++block < blocks) return;
-    block = 0;
-    if (++head < p.kv_heads) return;
-    head = 0;
-    const int done = plan.units_end[seg];
-    while (seg < p.requests && plan.units_end[seg + 1] == done) ++seg;
+  __device__ __forceinline__ void next_segment(const AttnArgs& p, const Plan& plan, int tok) {
+    head = group = tile = 0;
+    const int done = plan.cost_end[seg];
+    while (seg < p.requests && plan.cost_end[seg + 1] == done) ++seg;
     if (seg < p.requests) {
       ++seg;
       load(p, plan, tok);
     }
+  }
+  // n tiles on, not beyond the group's end
+  __device__ __forceinline__ void skip(const AttnArgs& p, const Plan& plan, int n, int tok) {
+    at += n * weight;
+    tile += n;
+    if (tile < tiles) return;
+    tile = 0;
+    if (++group < groups) return;
+    group = 0;
+    if (++head < p.kv_heads) return;
+    next_segment(p, plan, tok);
   }
 };
 
@@ -358,44 +389,53 @@ struct Cursor {
 // P and O in tensor memory (P takes the place of its S), K and V in a ring of shared-memory stages.
 // K is the product's B operand with the dimension contiguous, V its B operand with N contiguous:
 // both lie as loaded, [token][64 dimensions] rows of 128 bytes, swizzled.
-//   warps 0-3  softmax: a thread owns a row (its lane of tensor memory), so the running maximum and
-//              sum need no exchange between threads; they also bring Q in and take O out
-//   warp 4     issues the products: the first of tile i + 1 before the second of tile i, so that
-//              the tensor cores work while the softmax of tile i runs
-//   warps 5, 6 (kTma) K and V: one TMA box per group of tokens of one page and 64 dimensions; two
-//              warps, so that one's look-ups pass behind the other's copies
-//   warps 5-8  (otherwise) 16 bytes per cp.async, for any page size and strides
+//
+// Chains: tensor memory holds two sets of O, S and Q up to kDim = 128, one at 256. With two, groups
+// of more than 128 rows give each chain a block of rows and both take every tile, so K and V are
+// brought in once for 256 rows; smaller groups give both chains the same rows, and the tiles in
+// turn, so two tiles are under way at a time. With one, S alone is held twice.
+//   warps 0-3 (4-7)  softmax of a chain: a thread owns a row (its lane of tensor memory), so the
+//                    running maximum and sum need no exchange between threads; they also bring Q
+//                    in and take O out
+//   next warp        issues the products, in the order in which their operands become ready
+//   next 2 warps     (kTma) K and V: one TMA box per group of tokens of one page and 64 dimensions
+//   next 4 warps     (otherwise) 16 bytes per cp.async, for any page size and strides
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the one its weights refer
 // to (the weights stay below 2^8, in range of fp16, with the same relative rounding); the sum l and
 // the partial refer to the same maximum, so nothing is approximated.
 // ------------------------------------------------------------------------------------------------
-template <int kDim>
+template <int kDim, bool kTma>
 struct Shape {
+  static constexpr int kChains = kTma && kDim <= 128 ? 2 : 1;
+  static constexpr int kSoftWarps = 4 * kChains;
+  static constexpr int kLoadWarps = kTma ? 2 : kLoadThreads / 32;
+  static constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
   static constexpr int kTok = kDim == 64 ? 128 : 64;  // tokens per tile
   static constexpr int kStages = kDim == 256 ? 3 : 6;
-  static constexpr int kSub = kTok * 128;              // [token][64 dimensions] of K or V
-  static constexpr int kHalf = kSub * (kDim / 64);     // K or V of a stage
+  static constexpr int kSub = kTok * 128;           // [token][64 dimensions] of K or V
+  static constexpr int kHalf = kSub * (kDim / 64);  // K or V of a stage
   static constexpr int kRing = kStages * 2 * kHalf;
-  static constexpr int kS = kDim, kQ = kDim + 2 * kTok;  // columns of tensor memory; O at 0
+  // columns of tensor memory: O of each chain, two S, Q of each chain
+  static constexpr int kS = kChains * kDim, kQ = kS + 2 * kTok;
   static constexpr int kColumns = 512;
-  static_assert(kQ + kDim / 2 <= kColumns, "tensor memory of an SM");
+  static_assert(kQ + kChains * kDim / 2 <= kColumns, "tensor memory of an SM");
 };
 
 struct Control {
   uint64_t full[6], empty[6];
-  uint64_t s_full[2], p_full[2], o_done[2], q_full, o_free, sync, drain;
+  uint64_t s_full[2], p_full[2], o_done[2];  // per S: of a chain, or of every other tile
+  uint64_t q_full[2], o_free[2], sync[3];    // per chain; sync[2]: both
+  uint64_t drain;
   uint32_t tmem;
   int abort;
-  int bad_unit[6];  // per stage: 1 + the unit, if any, for which a page id outside the cache was met
-  int bad_value;    // 1 + the unit for which a value that is no number was met in a masked tile
-  unsigned char bad_token[128];
+  int bad_page[6];   // per stage: 1 + the tile, if any, for which a page outside the cache was met
+  int bad_value[2];  // per chain: 1 + the tile for which a value that is no number was met
+  unsigned char bad_token[2][128];
 };
 
-constexpr int attn_threads(bool tma) { return kSoftWarps * 32 + 32 + (tma ? 64 : kLoadThreads); }
-
-template <int kDim>
+template <int kDim, bool kTma>
 constexpr size_t attn_smem() {
-  return 1024 + Shape<kDim>::kRing + sizeof(Plan) + sizeof(Control) + 16;
+  return 1024 + Shape<kDim, kTma>::kRing + sizeof(Plan) + sizeof(Control) + 16;
 }
 
 __device__ int g_attn_status;
@@ -428,11 +468,12 @@ __device__ __forceinline__ bool mbar_test_now(uint64_t* bar, uint32_t parity) {
 }
 
 template <typename T, int kDim, bool kTma>
-__global__ void __launch_bounds__(attn_threads(kTma), 1)
+__global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
     attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const AttnArgs p) {
-  using S = Shape<kDim>;
-  constexpr int kTok = S::kTok, kStages = S::kStages;
+  using S = Shape<kDim, kTma>;
+  constexpr int kTok = S::kTok, kStages = S::kStages, kChains = S::kChains;
+  constexpr int kSoftWarps = S::kSoftWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -441,56 +482,60 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
   volatile int* s_abort = &c.abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (kTma && threadIdx.x >= (kSoftWarps + 1) * 32 && lane == 0)
+  if (kTma && warp > kSoftWarps && lane == 0)
     tma_prefetch_desc(warp == kSoftWarps + 2 ? &map_v : &map_k);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&c.full[s], kTma ? 2 : kLoadThreads + kLoadThreads / 32);
       mbar_init(&c.empty[s], 1);
-      c.bad_unit[s] = 0;
+      c.bad_page[s] = 0;
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&c.s_full[b], 1);
-      mbar_init(&c.p_full[b], kSoftWarps);
+      mbar_init(&c.p_full[b], 4);
       mbar_init(&c.o_done[b], 1);
+      mbar_init(&c.q_full[b], 4);
+      mbar_init(&c.o_free[b], 4);
+      mbar_init(&c.sync[b], 4);
+      c.bad_value[b] = 0;
     }
-    mbar_init(&c.q_full, kSoftWarps);
-    mbar_init(&c.o_free, kSoftWarps);
-    mbar_init(&c.sync, kSoftWarps);
+    mbar_init(&c.sync[2], 8);
     mbar_init(&c.drain, 1);
     c.abort = 0;
-    c.bad_value = 0;
     mbar_fence_init();
   }
   if (warp == kSoftWarps) tmem_alloc(&c.tmem, S::kColumns);
   {  // page tables into L2 behind the plan
-    const int line = 32, step = gridDim.x * blockDim.x * line, at = (blockIdx.x * blockDim.x + threadIdx.x) * line;
+    const int line = 32, step = gridDim.x * blockDim.x * line;
+    const int at = (blockIdx.x * blockDim.x + threadIdx.x) * line;
     for (int i = at; i < p.n_prefix_pages; i += step) prefetch_l2(p.prefix_pages + i);
     const int64_t all = p.requests > 0 ? (p.requests - 1) * p.pages_stride + p.max_pages : 0;
     for (int64_t i = at; i < all; i += step) prefetch_l2(p.pages + i);
   }
   grid_dep_wait();
   grid_dep_launch();
-  make_plan(p, kTok, plan);
+  make_plan<kChains>(p, kTok, plan);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, c.tmem, 0);
-  const int units = plan.units_end[p.requests];
-  const int ctas = plan_ctas(units, gridDim.x);
-  const bool idle = (int)blockIdx.x >= ctas;
-  const int u_lo = idle ? 0 : plan_begin(units, ctas, blockIdx.x);
-  const int u_hi = idle ? 0 : plan_begin(units, ctas, blockIdx.x + 1);
+  const int cost = plan.cost_end[p.requests];
+  const int ctas = plan_ctas(cost, gridDim.x);
+  const bool idle = cost == 0 || (int)blockIdx.x >= ctas;
+  const int c_lo = idle ? 0 : plan_begin(cost, ctas, blockIdx.x);
+  const int c_hi = idle ? 0 : plan_begin(cost, ctas, blockIdx.x + 1);
   const uint32_t ring = smem_u32(smem);
   const int stage_bytes = 2 * S::kHalf;
 
-  Cursor cur;
-  if (!idle) cur.seek(p, plan, u_lo, kTok);
+  Cursor<kChains> cur;
+  cur.at = c_hi;
+  if (!idle) cur.seek(p, plan, c_lo, kTok);
 
   if (kTma && warp > kSoftWarps) {
     // ------------------------------------------------------------------------------ loaders (TMA)
-    // Boxes of box_rows tokens x 64 dimensions, their pages looked up by a lane each. A box behind the length, or of a page that does not
-    // exist, is loaded from behind the last page: zeros, without a read.
+    // Boxes of box_rows tokens x 64 dimensions, their pages looked up by a lane each. A box behind
+    // the length, or of a page that does not exist, is loaded from behind the last page: zeros,
+    // without a read.
     const int groups = kTok / p.box_rows;  // a power of two, at most 16
     const int box_bytes = p.box_rows * 128;
     const bool leader = elect_one();
@@ -511,17 +556,17 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     const uint64_t once = l2_evict_first_policy(), again = l2_evict_normal_policy();
     if (!idle) look_up();
     int issued = 0;
-    for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
-      const int stage = i % kStages;
+    for (int i = 0; cur.at < c_hi; ++i) {
+      const int stage = i % kStages, at_cost = cur.at;
       const int head = cur.head, tok = cur.tile * kTok + row0, len = cur.len;
-      const uint64_t pol = cur.blocks > 1 ? again : once;
+      const uint64_t pol = cur.groups > 1 ? again : once;
       const int raw = id, tile_at = at;
-      cur.next(p, plan, kTok);
-      if (u + 1 < u_hi) look_up();  // its latency passes behind this tile's wait
+      cur.skip(p, plan, 1, kTok);
+      if (cur.at < c_hi) look_up();  // its latency passes behind this tile's wait
       if (!__all_sync(~0u, bar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort))) break;
       const bool exists = raw >= 0 && raw < p.total_pages;
       const int page = tok < len && exists ? raw : p.total_pages;
-      if (tok < len && !exists) *const_cast<volatile int*>(&c.bad_unit[stage]) = u + 1;
+      if (tok < len && !exists) *const_cast<volatile int*>(&c.bad_page[stage]) = at_cost + 1;
       __syncwarp();
       // One lane issues every box, with operands that are the same in the whole warp.
       const uint32_t dst = ring + stage * stage_bytes + (is_v ? S::kHalf : 0);
@@ -551,7 +596,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     // ------------------------------------------------------------------------------ loaders
     constexpr int kChunks = kDim / 8;               // 16-byte chunks per token
     constexpr int kWarpRows = 32 / kChunks;         // tokens per warp and copy
-    constexpr int kLoadWarps = kLoadThreads / 32;
+    constexpr int kLoadWarps = S::kLoadWarps;
     constexpr int kIters = kTok / (kWarpRows * kLoadWarps);
     const int lw = warp - kSoftWarps - 1;
     const int chunk = lane % kChunks;
@@ -572,19 +617,19 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     };
     int id = -1, at = 0;
     if (!idle) look_up(id, at);
-    for (int u = u_lo, i = 0; u < u_hi; ++u, ++i) {
-      const int stage = i % kStages;
+    for (int i = 0; cur.at < c_hi; ++i) {
+      const int stage = i % kStages, at_cost = cur.at;
       const int head = cur.head;
       const int tile_id = id, tile_at = at;
       const T* kc = static_cast<const T*>(p.k) + head * p.ks[2] + chunk * 8;
       const T* vc = static_cast<const T*>(p.v) + head * p.vs[2] + chunk * 8;
-      cur.next(p, plan, kTok);
-      if (u + 1 < u_hi) look_up(id, at);  // its latency passes behind this tile's wait and copies
+      cur.skip(p, plan, 1, kTok);
+      if (cur.at < c_hi) look_up(id, at);  // its latency passes behind this tile's wait and copies
       bool ok = true;
       if (lane == 0) ok = bar_wait(&c.empty[stage], ((i / kStages) & 1) ^ 1, s_abort);
       ok = __shfl_sync(~0u, ok, 0);
       if (!ok) break;
-      if (tile_id == -2) c.bad_unit[stage] = u + 1;
+      if (tile_id == -2) c.bad_page[stage] = at_cost + 1;
       const uint32_t kb = ring + stage * stage_bytes + (chunk >> 3) * S::kSub;
 #pragma unroll
       for (int j = 0; j < kIters; ++j) {
@@ -600,7 +645,7 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
       }
       cp_async_arrive(&c.full[stage]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&c.full[stage]);  // orders bad_unit before the stage is full
+      if (lane == 0) mbar_arrive(&c.full[stage]);  // orders bad_page before the stage is full
     }
     cp_async_wait_all();
   } else if (warp == kSoftWarps) {
@@ -612,67 +657,126 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     __syncwarp();
     if (!idle) {
       constexpr uint32_t kIdescS = instr_desc<T>(kTok, false), kIdescO = instr_desc<T>(kDim, true);
-      int pieces = 0;  // pieces whose second product has begun
-      bool ok = true;
       const bool leader = elect_one();
-      auto second = [&](int i, bool first) {  // O (+)= P V of tile i; `first`: it opens its piece
-        ok = ok && __all_sync(~0u, bar_wait(&c.p_full[i & 1], (i >> 1) & 1, s_abort));
-        if (first) {
-          if (pieces > 0) ok = ok && __all_sync(~0u, bar_wait(&c.o_free, (pieces - 1) & 1, s_abort));
-          ++pieces;
-        }
-        if (!ok) return;
-        tc_fence_after();
-        const int stage = i % kStages;
-        const uint64_t vd = smem_desc(ring + stage * stage_bytes + S::kHalf, S::kSub, 1024);
-        const uint32_t pa = tmem + S::kS + (i & 1) * kTok;
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < kTok / 16; ++ks)
-            tc_mma(tmem, pa + ks * 8, vd + ks * (2048 >> 4), kIdescO, ks > 0 || !first);
-          tc_commit(&c.empty[stage]);
-          tc_commit(&c.o_done[i & 1]);
-        }
-        __syncwarp();
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) {
+        ok = ok && __all_sync(~0u, bar_wait(bar, phase & 1, s_abort));
       };
-      int starts = 0, n = 0;
-      bool before = false;  // the tile before opened its piece
-      for (int u = u_lo; u < u_hi && ok; ++u, ++n) {
-        const bool start = n == 0 || cur.tile == 0;
-        // A new piece's queries arrive after the last weights of the old one: take those first.
-        if (start && n > 0) second(n - 1, before);
-        if (start) {
-          ok = ok && __all_sync(~0u, bar_wait(&c.q_full, starts & 1, s_abort));
-          ++starts;
-        }
-        const int stage = n % kStages;
-        // While this tile's keys are on their way, the weights of the one before may be ready.
-        bool pending = !start;
-        for (unsigned int it = 0; pending && it < kMaxPolls; ++it) {
-          if (__any_sync(~0u, mbar_test_now(&c.full[stage], (n / kStages) & 1))) break;
-          if (!__any_sync(~0u, mbar_test_now(&c.p_full[(n - 1) & 1], ((n - 1) >> 1) & 1))) continue;
-          second(n - 1, before);
-          pending = false;
-        }
-        ok = ok && __all_sync(~0u, bar_wait(&c.full[stage], (n / kStages) & 1, s_abort));
-        if (!ok) break;
+      auto ready = [&](uint64_t* bar, int phase) {
+        return __any_sync(~0u, mbar_test_now(bar, phase & 1));
+      };
+      // S = Q K^T of a stage, for chain w into S number b
+      auto scores = [&](int w, int b, int stage) {
         if constexpr (!kTma) fence_proxy_async_smem();  // cp.async writes through the generic proxy
         tc_fence_after();
         const uint64_t kd = smem_desc(ring + stage * stage_bytes, 16, 1024);
-        const uint32_t sd = tmem + S::kS + (n & 1) * kTok;
+        const uint32_t sd = tmem + S::kS + b * kTok, qd = tmem + S::kQ + w * (kDim / 2);
         if (leader) {
 #pragma unroll
           for (int ks = 0; ks < kDim / 16; ++ks)
-            tc_mma(sd, tmem + S::kQ + ks * 8, kd + (((ks / 4) * S::kSub + (ks % 4) * 32) >> 4), kIdescS,
-                   ks > 0);
-          tc_commit(&c.s_full[n & 1]);
+            tc_mma(sd, qd + ks * 8, kd + (((ks / 4) * S::kSub + (ks % 4) * 32) >> 4), kIdescS, ks > 0);
+          tc_commit(&c.s_full[b]);
         }
         __syncwarp();
-        if (pending) second(n - 1, before);
-        before = start;
-        cur.next(p, plan, kTok);
+      };
+      // O (+)= P V of a stage, for chain w from S number b; `last`: nothing else reads the stage
+      auto weigh = [&](int w, int b, int stage, bool first, bool last) {
+        tc_fence_after();
+        const uint64_t vd = smem_desc(ring + stage * stage_bytes + S::kHalf, S::kSub, 1024);
+        const uint32_t pa = tmem + S::kS + b * kTok, od = tmem + w * kDim;
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < kTok / 16; ++ks)
+            tc_mma(od, pa + ks * 8, vd + ks * (2048 >> 4), kIdescO, ks > 0 || !first);
+          if (last) tc_commit(&c.empty[stage]);
+          tc_commit(&c.o_done[b]);
+        }
+        __syncwarp();
+      };
+      if constexpr (kChains == 1) {
+        int opened = 0, starts = 0, n = 0;
+        bool before = false;  // the tile before opened its piece
+        auto second = [&](int i, bool first) {
+          wait(&c.p_full[i & 1], i >> 1);
+          if (first && opened++ > 0) wait(&c.o_free[0], opened - 2);
+          if (ok) weigh(0, i & 1, i % kStages, first, true);
+        };
+        for (; cur.at < c_hi && ok; ++n) {
+          const bool start = n == 0 || cur.tile == 0;
+          // A new piece's queries arrive after the last weights of the old one: take those first.
+          if (start && n > 0) second(n - 1, before);
+          if (start) wait(&c.q_full[0], starts++);
+          const int stage = n % kStages;
+          // While this tile's keys are on their way, the weights of the one before may be ready.
+          bool pending = !start;
+          for (unsigned int it = 0; pending && it < kMaxPolls; ++it) {
+            if (ready(&c.full[stage], n / kStages)) break;
+            if (!ready(&c.p_full[(n - 1) & 1], (n - 1) >> 1)) continue;
+            second(n - 1, before);
+            pending = false;
+          }
+          wait(&c.full[stage], n / kStages);
+          if (!ok) break;
+          scores(0, n & 1, stage);
+          if (pending) second(n - 1, before);
+          before = start;
+          cur.skip(p, plan, 1, kTok);
+        }
+        if (n > 0) second(n - 1, before);
+      } else {
+        // Per chain: first products issued, pieces opened by a first and by a second product; whether
+        // a second product is due, and its stage and flags.
+        int issued[2] = {0, 0}, opened[2] = {0, 0}, starts[2] = {0, 0}, stages[2] = {0, 0};
+        bool due[2] = {false, false}, firsts[2] = {false, false}, lasts[2] = {false, false};
+        auto second = [&](auto chain) {
+          constexpr int w = decltype(chain)::value;
+          if (!due[w]) return;
+          wait(&c.p_full[w], issued[w] - 1);
+          if (firsts[w] && opened[w]++ > 0) wait(&c.o_free[w], opened[w] - 2);
+          if (ok) weigh(w, w, stages[w], firsts[w], lasts[w]);
+          due[w] = false;
+        };
+        auto first = [&](auto chain, auto other, int i, bool opens, bool last) {
+          constexpr int w = decltype(chain)::value, v = decltype(other)::value;
+          second(chain);
+          if (opens) wait(&c.q_full[w], starts[w]++);
+          const int stage = i % kStages;
+          for (unsigned int it = 0; due[v] && it < kMaxPolls; ++it) {
+            if (ready(&c.full[stage], i / kStages)) break;
+            if (ready(&c.p_full[v], issued[v] - 1)) second(other);
+          }
+          wait(&c.full[stage], i / kStages);
+          if (!ok) return;
+          scores(w, w, stage);
+          ++issued[w];
+          due[w] = true;
+          stages[w] = stage, firsts[w] = opens, lasts[w] = last;
+        };
+        const std::integral_constant<int, 0> A;
+        const std::integral_constant<int, 1> B;
+        int piece = -1, t = 0;
+        bool both = false;
+        for (int n = 0; cur.at < c_hi && ok; ++n, ++t) {
+          if (n == 0 || cur.tile == 0) {
+            // The chains of a shared tile release its stage together, in this order.
+            if (both) second(A), second(B);
+            ++piece;
+            t = 0;
+            both = cur.rows(p) > kBlockRows;
+          }
+          if (both) {
+            first(A, B, n, t == 0, false);
+            first(B, A, n, t == 0, true);
+          } else if (((t + piece) & 1) == 0) {
+            first(A, B, n, t < 2, true);
+          } else {
+            first(B, A, n, t < 2, true);
+          }
+          cur.skip(p, plan, 1, kTok);
+        }
+        second(A);
+        second(B);
       }
-      if (ok && n > 0) second(n - 1, before);
       if (!ok) {  // let what is in flight land before the tensor memory is freed
         if (leader) tc_commit(&c.drain);
         const unsigned long long t0 = globaltimer_ns();
@@ -683,280 +787,319 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------------------------ softmax
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const uint32_t t_o = tmem + lanes, t_q = tmem + lanes + S::kQ;
-    bool ok = !idle;
-    // The rows of a piece and what they see.
-    int rows_here = 0, base = 0, seen = 0;
+    const int w = kChains > 1 ? warp >> 2 : 0;            // the chain
+    const int row = threadIdx.x & (kBlockRows - 1);       // of its block
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_o = tmem + lanes + w * kDim, t_q = tmem + lanes + S::kQ + w * (kDim / 2);
+    bool ok = true;
+    // A barrier of the warps that work on a tile; bounded like the other waits.
+    int syncs[2] = {0, 0};
+    auto sync_rows = [&](bool both) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.sync[both ? 2 : w]);
+      ok = bar_wait(&c.sync[both ? 2 : w], syncs[both]++ & 1, s_abort) && ok;
+      __syncwarp();
+    };
+    // The piece at a cursor: its tiles, and those among them that this chain takes (from its first
+    // on, every `step`-th).
+    struct Piece {
+      int tiles, mine, from, step;
+      bool both;
+    };
+    auto piece_at = [&](const Cursor<kChains>& at, int number) {
+      Piece x;
+      x.tiles = min(at.tiles - at.tile, (c_hi - at.at + at.weight - 1) / at.weight);
+      x.both = kChains > 1 && at.rows(p) > kBlockRows;
+      const bool split = kChains > 1 && !x.both;
+      x.step = split ? 2 : 1;
+      x.from = split ? (w + number) & 1 : 0;
+      x.mine = split ? (x.tiles - x.from + 1) / 2 : x.tiles;
+      return x;
+    };
+    // What this thread's row of the open piece sees, and its queries into tensor memory.
+    int my_rows = 0, base = 0, seen = 0;
     unsigned long long branch = 0;
-    // Queries of the piece at the cursor into tensor memory.
-    auto open_piece = [&] {
-      const int head = cur.head, block = cur.block;
-      rows_here = min(kBlockRows, cur.count * p.group - block * kBlockRows);
-      base = cur.len - cur.count;
-      const int f = block * kBlockRows + threadIdx.x;
-      const bool act = (int)threadIdx.x < rows_here;
-      const int local = act ? p.by_group.div(f) : 0;
-      const int t = cur.first + local;
-      seen = !act ? 0x7fffffff : cur.seg == 0 ? cur.len : min(cur.len, base + local + 1);
+    auto open_piece = [&](const Cursor<kChains>& at, bool both) {
+      const int off = at.group * kChains * kBlockRows + (both ? w * kBlockRows : 0);
+      my_rows = min(kBlockRows, at.count * p.group - off);
+      base = at.len - at.count;
+      const bool act = row < my_rows;
+      const int f = off + row, local = act ? p.by_group.div(f) : 0;
+      const int t = at.first + local;
+      seen = !act ? 0x7fffffff : at.seg == 0 ? at.len : min(at.len, base + local + 1);
       branch = 0;
-      if (p.tree && cur.seg && act) {
+      if (p.tree && at.seg && act) {
         branch = (unsigned long long)p.tree[t];
-        seen = min(cur.len, base);
+        seen = min(at.len, base);
       }
-      if (warp * 32 < rows_here) {
+      if ((warp & 3) * 32 < my_rows) {
         const T* src = static_cast<const T*>(p.q) + (int64_t)t * p.q_row +
-                       (int64_t)(head * p.group + (act ? f - local * p.group : 0)) * p.q_head;
-        uint32_t w[kDim / 2];  // all loads before the first store
+                       (int64_t)(at.head * p.group + (act ? f - local * p.group : 0)) * p.q_head;
+        uint32_t x[kDim / 2];  // all loads before the first store
         if (p.q_vec) {
 #pragma unroll
           for (int j = 0; j < kDim / 8; ++j) {
             uint4 v = make_uint4(0, 0, 0, 0);
             if (act && 8 * j < p.dim) v = *reinterpret_cast<const uint4*>(src + 8 * j);
-            w[4 * j] = v.x, w[4 * j + 1] = v.y, w[4 * j + 2] = v.z, w[4 * j + 3] = v.w;
+            x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
           }
         } else {
 #pragma unroll
           for (int j = 0; j < kDim / 2; ++j)
-            w[j] = act && 2 * j < p.dim ? *reinterpret_cast<const uint32_t*>(src + 2 * j) : 0u;
+            x[j] = act && 2 * j < p.dim ? *reinterpret_cast<const uint32_t*>(src + 2 * j) : 0u;
         }
         __syncwarp();
 #pragma unroll
         for (int c0 = 0; c0 < kDim / 2; c0 += 32)
-          tmem_st32(t_q + c0, *reinterpret_cast<const uint32_t(*)[32]>(&w[c0]));
+          tmem_st32(t_q + c0, *reinterpret_cast<const uint32_t(*)[32]>(&x[c0]));
         tc_wait_st();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&c.q_full);
-    };
-    if (ok) open_piece();
-    // A barrier of the softmax warps whose wait is bounded like the others.
-    int syncs = 0;
-    auto sync_rows = [&] {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c.sync);
-      ok = bar_wait(&c.sync, syncs++ & 1, s_abort) && ok;
-      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.q_full[w]);
     };
 
-    float m_ref = neg_inf(), l = 0.f;  // the maximum the weights refer to, and their sum
-    bool piece_start = true;
-    for (int u = u_lo, i = 0; u < u_hi && ok; ++u, ++i) {
-      const int b = i & 1, stage = i % kStages;
-      const bool act_warp = warp * 32 < rows_here;
-      const uint32_t t_s = tmem + lanes + S::kS + b * kTok;
-      const int tile0 = cur.tile * kTok;
-      if (piece_start) {
-        m_ref = neg_inf();
-        l = 0.f;
-      }
-      ok = bar_wait(&c.s_full[b], (i >> 1) & 1, s_abort);
-      // already complete: S was computed from this stage. Makes its flags and values visible here.
-      ok = ok && bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
-      if (!__all_sync(~0u, ok)) break;
-      tc_fence_after();
-      const bool bad_page = *const_cast<volatile int*>(&c.bad_unit[stage]) == u + 1;
-      const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
-      // Which of the 64 tokens from t0 on this row sees, one bit each.
-      auto visible = [&](int t0) {
-        auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
-        unsigned long long bits = below(seen - t0);
-        if (branch) {
-          const int off = t0 - base;
-          const unsigned long long m = off >= 64 || off <= -64 ? 0ull : off >= 0 ? branch >> off : branch << -off;
-          bits |= m & below(cur.len - t0);
-        }
-        if (bad_page) {
-#pragma unroll 1
-          for (int j = 0; j < 64 && t0 + j < cur.len; ++j) {
-            const int id = table[p.by_page.div(t0 + j)];
-            if (id < 0 || id >= p.total_pages) bits &= ~(1ull << j);
-          }
-        }
-        return bits;
-      };
-      // Some row of the block may not see a token of this tile (uniform over the block).
-      const int sure = cur.seg == 0 ? cur.len : min(cur.len, p.tree ? base : base + 1);
-      const bool masked = tile0 + kTok > sure || bad_page;
-      if (act_warp) {
-        // 64 scores at a time. Of a tile of 128 the second half is read twice: holding both would
-        // cost the registers that the rest needs.
-        uint32_t s[64];
-        const bool plain = !masked && p.scale_log2 > 0.f;
-        const float mul = plain ? p.scale_log2 : 1.f;
-        auto scores = [&](int h) {
-#pragma unroll
-          for (int j = 0; j < 64; j += 32)
-            tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[j]), t_s + h * 64 + j);
-          tc_wait_ld();
-          if (!plain) {
-            const unsigned long long bits = masked ? visible(tile0 + h * 64) : ~0ull;
-            const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              const float x = __uint_as_float(s[j]) * p.scale_log2;
-              s[j] = __float_as_uint((j < 32 ? lo >> j : hi >> (j - 32)) & 1u ? x : neg_inf());
-            }
-            __syncwarp();
-          }
-        };
-        float mx4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
-#pragma unroll
-        for (int h = kTok / 64 - 1; h >= 0; --h) {
-          scores(h);
-#pragma unroll
-          for (int j = 0; j < 64; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
-        }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
-        const bool grow = mx > m_ref + 8.f || (m_ref == neg_inf() && mx > neg_inf());
-        if (__any_sync(~0u, grow)) {
-          const float f = grow ? ex2(m_ref - mx) : 1.f;
-          if (grow) m_ref = mx;
-          l *= f;
-          if (!piece_start) {
-            ok = bar_wait(&c.o_done[b ^ 1], ((i - 1) >> 1) & 1, s_abort);
-            tc_fence_after();
-            __syncwarp();
-#pragma unroll 1
-            for (int c0 = 0; c0 < kDim; c0 += 32) {
-              uint32_t w[32];
-              tmem_ld32(w, t_o + c0);
-              tc_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * f);
-              tmem_st32(t_o + c0, w);
-            }
-          }
-        }
-        const float ref = m_ref == neg_inf() ? 0.f : m_ref;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < kTok / 64; ++h) {
-          if (h > 0) scores(h);
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            const float x = ex2(fmaf(__uint_as_float(s[j]), mul, -ref));
-            const float y = ex2(fmaf(__uint_as_float(s[j + 1]), mul, -ref));
-            sum[j & 2] += x;
-            sum[(j & 2) + 1] += y;
-            s[j / 2] = Pair<T>::pack(x, y);
-          }
-          // over scores that have been read: weights take half the columns
-          tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tc_wait_st();
-      }
-      // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
-      // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
-      // that only some rows see are searched for infinities and NaN: those are replaced by zeros
-      // before the second product, and added afterwards to the rows that see them.
-      bool poisoned = false;
-      if (masked) {
-        uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
-        const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
-        // a thread's chunk column, and every kPass-th token from its first
-        constexpr int kCols = kDim / 8, kPass = kSoftWarps * 32 / kCols;
-        const int col = threadIdx.x % kCols, tok0 = threadIdx.x / kCols;
-        uint8_t* column = vt + (col / 8) * S::kSub + (col & 7) * 16;
-        if (kTma && stored < kTok) {
-          const int end = (stored + p.box_rows - 1) & -p.box_rows;
-          for (int r = stored + tok0; r < end; r += kPass)
-            *reinterpret_cast<uint4*>(column + r * 128) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-        }
-        const int from = max(sure - tile0, 0);
-        if (from < stored) {
-          auto no_number = [](const uint4& w) {
-            return non_finite<T>(w.x) | non_finite<T>(w.y) | non_finite<T>(w.z) | non_finite<T>(w.w);
-          };
-          bool found = false;
-          for (int r = from + tok0; r < stored; r += kPass)
-            found |= no_number(*reinterpret_cast<const uint4*>(column + r * 128));
-          if (found) *const_cast<volatile int*>(&c.bad_value) = u + 1;
-          sync_rows();
-          poisoned = *const_cast<volatile int*>(&c.bad_value) == u + 1;
-          if (poisoned) {
-            for (int x = threadIdx.x; x < kTok; x += kSoftWarps * 32) c.bad_token[x] = 0;
-            sync_rows();
-            for (int r = from + tok0; r < stored; r += kPass) {
-              uint4& w = *reinterpret_cast<uint4*>(column + r * 128);
-              if (!no_number(w)) continue;
-              *const_cast<volatile unsigned char*>(&c.bad_token[r]) = 1;
-              w = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z),
-                             finite_or_zero<T>(w.w));
-            }
-            fence_proxy_async_smem();
-            sync_rows();
-          }
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c.p_full[b]);
-      if (poisoned) {
-        ok = ok && bar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
-        tc_fence_after();
-        __syncwarp();
-        const int head = cur.head;
-        for (int x = 0; x < kTok && act_warp; ++x) {
-          if (!*const_cast<volatile unsigned char*>(&c.bad_token[x])) continue;
-          const int tok = tile0 + x, pg = p.by_page.div(tok);
-          const bool see = (int)threadIdx.x < rows_here && (visible(tok) & 1ull);
-          const T* v = static_cast<const T*>(p.v) + table[pg] * p.vs[0] +
-                       (tok - pg * p.page_size) * p.vs[1] + head * p.vs[2];
-#pragma unroll 1
-          for (int c0 = 0; c0 < kDim; c0 += 32) {
-            uint32_t w[32];
-            tmem_ld32(w, t_o + c0);
-            tc_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (c0 + j >= p.dim || !see) continue;
-              const float y = (float)v[c0 + j];
-              if (!isfinite(y)) w[j] = __float_as_uint(__uint_as_float(w[j]) + y);
-            }
-            tmem_st32(t_o + c0, w);
-          }
-          tc_wait_st();
-        }
-        tc_fence_before();
-        sync_rows();  // bad_token is free again
-      }
-
-      const bool piece_end = cur.tile + 1 == cur.tiles || u + 1 == u_hi;
-      piece_start = piece_end;
-      if (!piece_end) {
-        ++cur.tile;
+    int task = 0;        // tiles this chain has taken
+    int tile_index = 0;  // tiles of the CTA before the piece
+    bool open = false;   // the piece at the cursor has been opened
+    for (int number = 0; cur.at < c_hi && ok; ++number) {
+      const Piece piece = piece_at(cur, number);
+      const bool both = piece.both;
+      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.index();
+      const int64_t part = ((int64_t)slot * kChains + w) * kBlockRows + row;
+      const bool room = slot >= 0 && slot < p.slots;
+      if (kChains > 1 && piece.mine == 0) {  // a single tile, the other chain's: an empty partial
+        if (room && row < cur.rows(p)) p.part_ml[part] = make_float2(neg_inf(), 0.f);
+        tile_index += piece.tiles;
+        cur.skip(p, plan, piece.tiles, kTok);
         continue;
       }
+      if (!open) open_piece(cur, both);
+      open = false;
+      const bool act_warp = (warp & 3) * 32 < my_rows;
+      const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
+      // The first token that some row of the group may not see.
+      const int sure = cur.seg == 0 ? cur.len : max(0, min(cur.len, p.tree ? base : base + 1));
+      float m_ref = neg_inf(), l = 0.f;  // the maximum the weights refer to, and their sum
+
+      for (int k = 0; k < piece.mine; ++k, ++task) {
+        const int step = piece.from + k * piece.step, i = tile_index + step, stage = i % kStages;
+        const int b = kChains > 1 ? w : task & 1, phase = kChains > 1 ? task : task >> 1;
+        const uint32_t t_s = tmem + lanes + S::kS + b * kTok;
+        const int tile0 = (cur.tile + step) * kTok, mark = cur.at + step * cur.weight + 1;
+        ok = bar_wait(&c.s_full[b], phase & 1, s_abort);
+        // already complete: S was computed from this stage. Makes its flags and values visible here.
+        ok = ok && bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
+        if (!__all_sync(~0u, ok)) break;
+        tc_fence_after();
+        const bool bad_page = *const_cast<volatile int*>(&c.bad_page[stage]) == mark;
+        // Which of the 64 tokens from t0 on this row sees, one bit each.
+        auto visible = [&](int t0) {
+          auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+          unsigned long long bits = below(seen - t0);
+          if (branch) {
+            const int off = t0 - base;
+            const unsigned long long m =
+                off >= 64 || off <= -64 ? 0ull : off >= 0 ? branch >> off : branch << -off;
+            bits |= m & below(cur.len - t0);
+          }
+          if (bad_page) {
+#pragma unroll 1
+            for (int j = 0; j < 64 && t0 + j < cur.len; ++j) {
+              const int id = table[p.by_page.div(t0 + j)];
+              if (id < 0 || id >= p.total_pages) bits &= ~(1ull << j);
+            }
+          }
+          return bits;
+        };
+        const bool masked = tile0 + kTok > sure || bad_page;  // the same in the whole group
+        if (act_warp) {
+          // 64 scores at a time. Of a tile of 128 the second half is read twice: holding both would
+          // cost the registers that the rest needs.
+          uint32_t s[64];
+          const bool plain = !masked && p.scale_log2 > 0.f;
+          const float mul = plain ? p.scale_log2 : 1.f;
+          auto scores = [&](int h) {
+#pragma unroll
+            for (int j = 0; j < 64; j += 32)
+              tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[j]), t_s + h * 64 + j);
+            tc_wait_ld();
+            if (!plain) {
+              const unsigned long long bits = masked ? visible(tile0 + h * 64) : ~0ull;
+              const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+#pragma unroll
+              for (int j = 0; j < 64; ++j) {
+                const float x = __uint_as_float(s[j]) * p.scale_log2;
+                s[j] = __float_as_uint((j < 32 ? lo >> j : hi >> (j - 32)) & 1u ? x : neg_inf());
+              }
+              __syncwarp();
+            }
+          };
+          float mx4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+          for (int h = kTok / 64 - 1; h >= 0; --h) {
+            scores(h);
+#pragma unroll
+            for (int j = 0; j < 64; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+          const bool grow = mx > m_ref + 8.f || (m_ref == neg_inf() && mx > neg_inf());
+          if (__any_sync(~0u, grow)) {
+            const float f = grow ? ex2(m_ref - mx) : 1.f;
+            if (grow) m_ref = mx;
+            l *= f;
+            if (k > 0) {  // O holds the chain's tiles so far
+              const int last = task - 1;
+              ok = kChains > 1 ? bar_wait(&c.o_done[w], last & 1, s_abort)
+                               : bar_wait(&c.o_done[last & 1], (last >> 1) & 1, s_abort);
+              tc_fence_after();
+              __syncwarp();
+#pragma unroll 1
+              for (int c0 = 0; c0 < kDim; c0 += 32) {
+                uint32_t x[32];
+                tmem_ld32(x, t_o + c0);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+                tmem_st32(t_o + c0, x);
+              }
+            }
+          }
+          const float ref = m_ref == neg_inf() ? 0.f : m_ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < kTok / 64; ++h) {
+            if (h > 0) scores(h);
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+              const float x = ex2(fmaf(__uint_as_float(s[j]), mul, -ref));
+              const float y = ex2(fmaf(__uint_as_float(s[j + 1]), mul, -ref));
+              sum[j & 2] += x;
+              sum[(j & 2) + 1] += y;
+              s[j / 2] = Pair<T>::pack(x, y);
+            }
+            // over scores that have been read: weights take half the columns
+            tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tc_wait_st();
+        }
+        // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
+        // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
+        // that only some rows see are searched for infinities and NaN: those are replaced by zeros
+        // before the second product, and added afterwards to the rows that see them.
+        bool poisoned = false;
+        const int set = both ? 0 : w;  // whose flags
+        if (masked) {
+          uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
+          const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
+          // a thread's chunk column, and every kPass-th token from its first
+          constexpr int kCols = kDim / 8, kPass = kBlockRows / kCols;
+          const int col = row % kCols, tok0 = row / kCols;
+          uint8_t* column = vt + (col / 8) * S::kSub + (col & 7) * 16;
+          if (kTma && stored < kTok) {
+            const int end = (stored + p.box_rows - 1) & -p.box_rows;
+            for (int r = stored + tok0; r < end; r += kPass)
+              *reinterpret_cast<uint4*>(column + r * 128) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          const int from = max(sure - tile0, 0);
+          if (from < stored) {
+            auto no_number = [](const uint4& x) {
+              return non_finite<T>(x.x) | non_finite<T>(x.y) | non_finite<T>(x.z) | non_finite<T>(x.w);
+            };
+            bool found = false;
+            for (int r = from + tok0; r < stored; r += kPass)
+              found |= no_number(*reinterpret_cast<const uint4*>(column + r * 128));
+            if (found) *const_cast<volatile int*>(&c.bad_value[set]) = mark;
+            sync_rows(both);
+            poisoned = *const_cast<volatile int*>(&c.bad_value[set]) == mark;
+            if (poisoned) {
+              for (int x = row; x < kTok; x += kBlockRows) c.bad_token[set][x] = 0;
+              sync_rows(both);
+              for (int r = from + tok0; r < stored; r += kPass) {
+                uint4& x = *reinterpret_cast<uint4*>(column + r * 128);
+                if (!no_number(x)) continue;
+                *const_cast<volatile unsigned char*>(&c.bad_token[set][r]) = 1;
+                x = make_uint4(finite_or_zero<T>(x.x), finite_or_zero<T>(x.y), finite_or_zero<T>(x.z),
+                               finite_or_zero<T>(x.w));
+              }
+              fence_proxy_async_smem();
+              sync_rows(both);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.p_full[b]);
+        if (poisoned) {
+          ok = ok && bar_wait(&c.o_done[b], phase & 1, s_abort);
+          tc_fence_after();
+          __syncwarp();
+          for (int x = 0; x < kTok && act_warp; ++x) {
+            if (!*const_cast<volatile unsigned char*>(&c.bad_token[set][x])) continue;
+            const int tok = tile0 + x, pg = p.by_page.div(tok);
+            const bool see = row < my_rows && (visible(tok) & 1ull);
+            const T* v = static_cast<const T*>(p.v) + table[pg] * p.vs[0] +
+                         (tok - pg * p.page_size) * p.vs[1] + cur.head * p.vs[2];
+#pragma unroll 1
+            for (int c0 = 0; c0 < kDim; c0 += 32) {
+              uint32_t y[32];
+              tmem_ld32(y, t_o + c0);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (c0 + j >= p.dim || !see) continue;
+                const float z = (float)v[c0 + j];
+                if (!isfinite(z)) y[j] = __float_as_uint(__uint_as_float(y[j]) + z);
+              }
+              __syncwarp();
+              tmem_st32(t_o + c0, y);
+            }
+            tc_wait_st();
+          }
+          tc_fence_before();
+          sync_rows(both);  // the flags are free again
+        }
+      }
+      if (!__all_sync(~0u, ok)) {
+        ok = false;
+        break;
+      }
+
       // ---- end of a piece: the next one's queries first, then O out
-      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.group();
-      const int done_rows = rows_here;
-      cur.next(p, plan, kTok);
-      if (u + 1 < u_hi) open_piece();
-      ok = ok && bar_wait(&c.o_done[b], (i >> 1) & 1, s_abort);
+      const int done_rows = my_rows, last = task - 1;
+      tile_index += piece.tiles;
+      cur.skip(p, plan, piece.tiles, kTok);
+      if (cur.at < c_hi) {
+        const Piece next = piece_at(cur, number + 1);
+        if (kChains == 1 || next.mine > 0) {
+          open_piece(cur, next.both);
+          open = true;
+        }
+      }
+      ok = kChains > 1 ? bar_wait(&c.o_done[w], last & 1, s_abort)
+                       : bar_wait(&c.o_done[last & 1], (last >> 1) & 1, s_abort);
       tc_fence_after();
       __syncwarp();
-      if (warp * 32 < done_rows) {
-        const bool act = (int)threadIdx.x < done_rows && slot >= 0 && slot < p.slots;
-        const int64_t at = (int64_t)slot * kBlockRows + threadIdx.x;
-        float* dst = p.part_o + at * p.dim;
+      if ((warp & 3) * 32 < done_rows) {
+        const bool act = row < done_rows && room;
+        float* dst = p.part_o + part * p.dim;
 #pragma unroll 1
         for (int c0 = 0; c0 < p.dim; c0 += 32) {
-          uint32_t w[32];
-          tmem_ld32(w, t_o + c0);
+          uint32_t x[32];
+          tmem_ld32(x, t_o + c0);
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
-            if (act && c0 + j < p.dim) st_256(dst + c0 + j, &w[j]);
+            if (act && c0 + j < p.dim) st_256(dst + c0 + j, &x[j]);
+          __syncwarp();
         }
-        if (act) p.part_ml[at] = make_float2(m_ref, l);
+        if (act) p.part_ml[part] = make_float2(m_ref, l);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&c.o_free);
+      if (lane == 0) mbar_arrive(&c.o_free[w]);
     }
   }
   tc_fence_before();
@@ -972,13 +1115,13 @@ __global__ void __launch_bounds__(attn_threads(kTma), 1)
 // ------------------------------------------------------------------------------------------------
 // Join: one block per (row, query head). The row's partials are those of its prefix group and of
 // its request's own group, each from a run of CTAs: partial j lies at slot from[0] + j for the first
-// n[0], at from[1] + j - n[0] for the others. kThreads / kCols threads take the partials in turn, a
+// n[0], at from[1] + j - n[0] for the others (two at each where the chains took turns). kThreads / kCols threads take the partials in turn, a
 // thread four dimensions of each; the first loads of O are on their way before the weights are
 // known. Sums run over fixed sets in a fixed order.
 // ------------------------------------------------------------------------------------------------
-constexpr int kMaxPartials = 2 * kMaxCtas;
+constexpr int kMaxPartials = 4 * kMaxCtas;
 
-template <typename T, int kCols, int kThreads>
+template <typename T, int kCols, int kThreads, int kChains>
 __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int grid) {
   constexpr int kWarps = kThreads / 32, kTeams = kThreads / kCols, kAhead = 4;
   __shared__ float s_w[kMaxPartials];
@@ -992,26 +1135,34 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
   grid_dep_launch();
   const RowPlan r = p.row_plan[t];
   const int head = p.by_group.div(h), g = h - head * p.group;
-  int from[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0};
+  int from[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0}, both[2] = {1, 1};
   if (r.owned) {
-    const int ctas = plan_ctas(r.units, grid);
+    const int ctas = plan_ctas(r.cost, grid);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int tiles = i ? r.tiles : r.prefix_tiles, blocks = i ? r.blocks : r.prefix_blocks;
+      const int tiles = i ? r.tiles : r.prefix_tiles, count = i ? r.count : r.prefix_count;
       if (tiles == 0) continue;
       const int f = (t - (i ? r.first : r.prefix_first)) * p.group + g;
-      const int group = head * blocks + f / kBlockRows;
-      row[i] = f % kBlockRows;
-      const int u0 = (i ? r.unit0 : 0) + group * tiles;
-      const int c0 = plan_owner(r.units, ctas, u0), c1 = plan_owner(r.units, ctas, u0 + tiles - 1);
+      const int index = f / (kChains * kBlockRows);
+      const int group = head * groups_of<kChains>(count, p.group) + index;
+      both[i] = kChains == 1 || group_rows<kChains>(count, p.group, index) > kBlockRows;
+      row[i] = f % (kChains * kBlockRows);
+      const int weight = weight_of<kChains>(count, p.group);
+      const int at = (i ? r.cost0 : 0) + group * tiles * weight;
+      const int c0 = plan_owner(r.cost, ctas, at), c1 = plan_owner(r.cost, ctas, at + (tiles - 1) * weight);
       from[i] = c0 + (i ? r.group0 : 0) + group;
-      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i]));
+      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i])) * (both[i] ? 1 : 2);
     }
   }
   const int total = n[0] + n[1];
   auto place = [&](int j) {
-    const bool own = j >= n[0];
-    return (int64_t)(own ? from[1] + j - n[0] : from[0] + j) * kBlockRows + (own ? row[1] : row[0]);
+    const int i = j >= n[0];
+    const int k = i ? j - n[0] : j;
+    const int f = i ? from[1] : from[0], r0 = i ? row[1] : row[0];
+    const bool whole = i ? both[1] : both[0];
+    // a whole group's rows run over its chains; a shared block is in each
+    return (int64_t)(f + (whole ? k : k >> 1)) * (kChains * kBlockRows) + r0 +
+           (whole ? 0 : (k & 1) * kBlockRows);
   };
   float4 x[kAhead];
   auto fetch = [&](int j0) {
@@ -1064,6 +1215,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
       const int j = j0 + k * kTeams;
       if (j >= total) continue;
       const float w = s_w[j];
+      if (w == 0.f) continue;  // an empty partial has no O
       acc.x += x[k].x * w, acc.y += x[k].y * w, acc.z += x[k].z * w, acc.w += x[k].w * w;
     }
   }
@@ -1083,16 +1235,24 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
 }
 
 int round_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-int64_t slots_for(int requests, int rows, int group, int kv_heads) {
-  const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
-  return kMaxCtas + kv_heads * (2 * blocks + requests);
+// Slots, and partials in all, of the variant with `chains` chains.
+int64_t slots_for(int requests, int rows, int group, int kv_heads, int chains) {
+  const int64_t groups = ((int64_t)rows * group + chains * kBlockRows - 1) / (chains * kBlockRows);
+  return kMaxCtas + kv_heads * (2 * groups + requests);
+}
+int64_t partials_for(int requests, int rows, int group, int kv_heads) {
+  return kBlockRows * std::max(slots_for(requests, rows, group, kv_heads, 1),
+                               2 * slots_for(requests, rows, group, kv_heads, 2));
 }
 
 template <typename T, int kDim, bool kTma>
-int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& p, int ctas,
+int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int ctas,
                  cudaStream_t stream) {
-  constexpr size_t smem = attn_smem<kDim>();
+  using S = Shape<kDim, kTma>;
+  constexpr int kChains = S::kChains;
+  constexpr size_t smem = attn_smem<kDim, kTma>();
   static_assert(smem <= 227 * 1024, "shared memory of a block");
+  p.slots = (int)slots_for(p.requests, p.rows, p.group, p.kv_heads, kChains);
   auto kernel = attn_kernel<T, kDim, kTma>;
   static bool configured[64] = {};
   int dev = 0;
@@ -1101,14 +1261,17 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& p
     B2_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured[dev] = true;
   }
-  int rc = launch_kernel(kernel, ctas, attn_threads(kTma), smem, stream, /*early=*/true, mk, mv, p);
+  int rc = launch_kernel(kernel, ctas, S::kThreads, smem, stream, /*early=*/true, mk, mv, p);
   if (rc) return rc;
   // Partials of a row: about as many as CTAs per group. Few of them: few threads.
-  const int64_t groups = (int64_t)p.kv_heads * (((int64_t)p.rows * p.group + kBlockRows - 1) / kBlockRows);
+  const int64_t rows = (int64_t)p.rows * p.group;
+  const int64_t groups = p.kv_heads * ((rows + kChains * kBlockRows - 1) / (kChains * kBlockRows));
   const int grid = p.rows * p.q_heads;
   if (ctas / groups <= 8)
-    return launch_kernel(join_kernel<T, kDim / 4, 128>, grid, 128, 0, stream, /*early=*/true, p, ctas);
-  return launch_kernel(join_kernel<T, kDim / 4, 512>, grid, 512, 0, stream, /*early=*/true, p, ctas);
+    return launch_kernel(join_kernel<T, kDim / 4, 128, kChains>, grid, 128, 0, stream, /*early=*/true, p,
+                         ctas);
+  return launch_kernel(join_kernel<T, kDim / 4, 512, kChains>, grid, 512, 0, stream, /*early=*/true, p,
+                       ctas);
 }
 
 // A cache as a tensor map (dimension, place in the page, head, page), boxes of box_rows tokens and
@@ -1134,7 +1297,7 @@ bool cache_map(CUtensorMap* map, const void* base, const int64_t* s, const AttnA
 template <typename T, int kDim>
 int launch_dim(AttnArgs& p, int ctas, cudaStream_t stream) {
   CUtensorMap mk = {}, mv = {};
-  p.box_rows = std::min(Shape<kDim>::kTok, p.page_size & -p.page_size);
+  p.box_rows = std::min(Shape<kDim, true>::kTok, p.page_size & -p.page_size);
   if (p.box_rows >= 8 && p.dim >= 64 && cache_map<T>(&mk, p.k, p.ks, p) &&
       cache_map<T>(&mv, p.v, p.vs, p))
     return launch_typed<T, kDim, true>(mk, mv, p, ctas, stream);
@@ -1184,8 +1347,8 @@ extern "C" size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, 
                                            int head_dim) {
   using namespace b2;
   if (check_shape(requests, rows, q_heads, kv_heads, head_dim)) return 0;
-  const int64_t slots = slots_for(requests, rows, q_heads / kv_heads, kv_heads);
-  return (size_t)slots * kBlockRows * (head_dim * sizeof(float) + sizeof(float2)) +
+  return (size_t)partials_for(requests, rows, q_heads / kv_heads, kv_heads) *
+             (head_dim * sizeof(float) + sizeof(float2)) +
          (size_t)rows * sizeof(RowPlan) + 256;
 }
 
@@ -1229,10 +1392,10 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
                 need);
   const int group = q_heads / kv_heads;
   const int tok = round_dim(head_dim) == 64 ? 128 : 64;
-  // units are counted in 32 bits
+  // costs are counted in 32 bits
   const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
   const int64_t tiles = ((int64_t)std::max(n_prefix_pages, max_pages) * page_size + tok - 1) / tok;
-  if ((2 * blocks + requests) * kv_heads * tiles > 0x7fffffff)
+  if ((2 * blocks + requests) * kv_heads * tiles * kMaxWeight > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "%s: tables too long for %d rows", op, rows);
   DeviceInfo di;
   rc = device_info(&di);
@@ -1252,11 +1415,10 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.n_prefix_pages = n_prefix_pages, p.max_pages = max_pages;
   p.requests = requests, p.rows = rows, p.q_heads = q_heads, p.kv_heads = kv_heads, p.group = group;
   p.dim = head_dim;
-  p.slots = (int)slots_for(requests, rows, group, kv_heads);
   p.scale_log2 = scale * kLog2e;
   p.row_plan = static_cast<RowPlan*>(ws);
   p.part_ml = reinterpret_cast<float2*>(p.row_plan + rows);
-  const size_t ml_bytes = ((size_t)rows * sizeof(RowPlan) + (size_t)p.slots * kBlockRows * sizeof(float2) + 255) & ~(size_t)255;
+  const size_t ml_bytes = ((size_t)rows * sizeof(RowPlan) + (size_t)partials_for(requests, rows, group, kv_heads) * sizeof(float2) + 255) & ~(size_t)255;
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + ml_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == B2_DTYPE_F16 ? launch_type<__half>(p, ctas, s)
