@@ -43,7 +43,8 @@ struct RowPlan {
   int tiles, first, count;                        // of the row's request; tiles = 0: none
   int cost0, group0;                              // cost and groups before the request's
   int owned;                                      // the row belongs to a request
-  int pad[2];
+  int even;                                       // every tile costs the same (Cost)
+  int pad;
 };
 
 // Division of 0 <= n < 2^31 by a number fixed for the launch, as a product and a shift (Granlund and
@@ -89,6 +90,21 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 numbers in 64 bits, and operations on both at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 template <typename T>
@@ -226,25 +242,37 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 
 // ------------------------------------------------------------------------------------------------
 // The plan: every block derives it from the lengths on the device. A group is kChains blocks of rows
-// of one head and segment. A tile of a segment with more than one block of rows costs 3, any other
-// 2: with two chains the tensor cores and the softmax then take longer than the copies.
+// of one head and segment. Costs, in halves of the time a tile takes from memory: 2 for a tile, 4
+// where it is used for two blocks of rows (3000 clocks against 1490 at 64 tokens of 128 dimensions),
+// and 2 more to open a group. With few tiles for each CTA, every tile costs 1: one each is best then.
 // ------------------------------------------------------------------------------------------------
+struct Cost {
+  int tile, both, open;
+  __device__ __forceinline__ explicit Cost(bool even)
+      : tile(even ? 1 : 2), both(even ? 1 : 4), open(even ? 0 : 2) {}
+  // CTAs that share a cost: each range is as long as the longest way from one tile's start to the
+  // next one's, so that a tile starts in it. A tile belongs to the CTA in whose range it starts.
+  __device__ __forceinline__ int ctas(int cost, int most) const {
+    return max(1, min(cost / (both + open), most));
+  }
+};
 struct Plan {
   int cost_end[kMaxRequests + 1];    // running sum of costs up to and with segment s
   int groups_end[kMaxRequests + 1];  // running sum of groups
   int first[kMaxRequests + 1];       // first row of the segment
   int count[kMaxRequests + 1];       // and how many
   int len[kMaxRequests + 1];         // tokens
+  int even;
 };
-constexpr int kMaxWeight = 3;
+constexpr int kMaxCost = 6;  // of a tile, with the opening of its group
 
 template <int kChains>
 __device__ __forceinline__ int groups_of(int count, int group) {
   return (count * group + kChains * kBlockRows - 1) / (kChains * kBlockRows);
 }
 template <int kChains>
-__device__ __forceinline__ int weight_of(int count, int group) {
-  return kChains > 1 && count * group > kBlockRows ? kMaxWeight : 2;
+__device__ __forceinline__ int tile_cost(const Cost& cost, int count, int group) {
+  return kChains > 1 && count * group > kBlockRows ? cost.both : cost.tile;
 }
 // Rows of group g of a segment.
 template <int kChains>
@@ -270,13 +298,20 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
   }
   bad = __syncthreads_or(bad);
   if (threadIdx.x < 32) {
+    auto groups = [&](int s) { return bad ? 0 : p.kv_heads * groups_of<kChains>(plan.count[s], p.group); };
+    auto tiles = [&](int s) { return (plan.len[s] + tok - 1) / tok; };
+    int all = 0;
+    for (int s = threadIdx.x; s <= p.requests; s += 32) all += groups(s) * tiles(s);
+    all = __reduce_add_sync(~0u, all);
+    const bool even = all <= 2 * (int)gridDim.x;
+    const Cost cost(even);
     int c_base = 0, g_base = 0;
     for (int s0 = 0; s0 <= p.requests; s0 += 32) {
       const int s = s0 + threadIdx.x;
       int c = 0, g = 0;
-      if (s <= p.requests && !bad && plan.len[s] > 0) {
-        g = p.kv_heads * groups_of<kChains>(plan.count[s], p.group);
-        c = g * ((plan.len[s] + tok - 1) / tok) * weight_of<kChains>(plan.count[s], p.group);
+      if (s <= p.requests && plan.len[s] > 0) {
+        g = groups(s);
+        c = g * (cost.open + tiles(s) * tile_cost<kChains>(cost, plan.count[s], p.group));
       }
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -288,6 +323,7 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
       c_base = __shfl_sync(~0u, c, 31);
       g_base = __shfl_sync(~0u, g, 31);
     }
+    if (threadIdx.x == 0) plan.even = even;
   }
   __syncthreads();
 }
@@ -296,6 +332,7 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
 __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const Plan& plan, int t) {
   RowPlan r = {};
   r.cost = plan.cost_end[p.requests];
+  r.even = plan.even;
   r.prefix_tiles = (plan.len[0] + tok - 1) / tok;
   r.prefix_first = plan.first[0];
   r.prefix_count = plan.count[0];
@@ -316,11 +353,6 @@ __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const
   p.row_plan[t] = r;
 }
 
-// CTAs that share a cost: each range is at least one tile wide, so that the tiles that start in it
-// are at least one. A tile belongs to the CTA in whose range it starts.
-__device__ __forceinline__ int plan_ctas(int cost, int ctas) {
-  return max(1, min(cost / kMaxWeight, ctas));
-}
 __device__ __forceinline__ int plan_begin(int cost, int ctas, int c) {
   return (int)((int64_t)cost * c / ctas);
 }
@@ -333,11 +365,14 @@ template <int kChains>
 struct Cursor {
   int seg, head, group, tile, at;  // at: the cost before it
   int first, count, len, tiles, groups, weight;
+  int open;
   __device__ __forceinline__ void load(const AttnArgs& p, const Plan& plan, int tok) {
+    const Cost cost(plan.even);
     first = plan.first[seg], count = plan.count[seg], len = plan.len[seg];
     tiles = (len + tok - 1) / tok;
     groups = groups_of<kChains>(count, p.group);
-    weight = weight_of<kChains>(count, p.group);
+    weight = tile_cost<kChains>(cost, count, p.group);
+    open = cost.open;
   }
   __device__ __forceinline__ int index() const { return head * groups + group; }  // in the segment
   __device__ __forceinline__ int rows(const AttnArgs& p) const {
@@ -352,13 +387,24 @@ struct Cursor {
     }
     seg = lo;
     load(p, plan, tok);
-    const int start = seg ? plan.cost_end[seg - 1] : 0, n = (c - start + weight - 1) / weight;
-    at = start + n * weight;
-    const int g = n / tiles;
-    tile = n - g * tiles;
+    const int start = seg ? plan.cost_end[seg - 1] : 0, whole = open + tiles * weight;
+    int g = (c - start) / whole;
+    const int rest = c - start - g * whole;
+    tile = rest == 0 ? 0 : max(1, (rest - open + weight - 1) / weight);
+    if (tile >= tiles) tile = 0, ++g;
+    at = start + g * whole + cost_to(tile);
     head = groups == 1 ? g : g / groups;
     group = g - head * groups;
     if (head == p.kv_heads) next_segment(p, plan, tok);
+  }
+  // From the group's start to tile t of it.
+  __device__ __forceinline__ int cost_to(int t) const { return t == 0 ? 0 : open + t * weight; }
+  // The start of the tile n on, in the same group.
+  __device__ __forceinline__ int ahead(int n) const { return at + cost_to(tile + n) - cost_to(tile); }
+  // Tiles from here on that start before `end`, in the same group.
+  __device__ __forceinline__ int tiles_before(int end) const {
+    const int left = end - at - (tile == 0 ? open : 0);
+    return min(tiles - tile, max(1, (left + weight - 1) / weight));
   }
   __device__ __forceinline__ void next_segment(const AttnArgs& p, const Plan& plan, int tok) {
     head = group = tile = 0;
@@ -369,9 +415,9 @@ struct Cursor {
       load(p, plan, tok);
     }
   }
-  // n tiles on, not beyond the group's end
+  // n >= 1 tiles on, not beyond the group's end
   __device__ __forceinline__ void skip(const AttnArgs& p, const Plan& plan, int n, int tok) {
-    at += n * weight;
+    at = ahead(n);
     tile += n;
     if (tile < tiles) return;
     tile = 0;
@@ -411,7 +457,7 @@ struct Shape {
   static constexpr int kLoadWarps = kTma ? 2 : kLoadThreads / 32;
   static constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
   static constexpr int kTok = kDim == 64 ? 128 : 64;  // tokens per tile
-  static constexpr int kStages = kDim == 256 ? 3 : 6;
+  static constexpr int kStages = kDim == 256 ? 3 : 4;
   static constexpr int kSub = kTok * 128;           // [token][64 dimensions] of K or V
   static constexpr int kHalf = kSub * (kDim / 64);  // K or V of a stage
   static constexpr int kRing = kStages * 2 * kHalf;
@@ -520,7 +566,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, c.tmem, 0);
   const int cost = plan.cost_end[p.requests];
-  const int ctas = plan_ctas(cost, gridDim.x);
+  const int ctas = Cost(plan.even).ctas(cost, gridDim.x);
   const bool idle = cost == 0 || (int)blockIdx.x >= ctas;
   const int c_lo = idle ? 0 : plan_begin(cost, ctas, blockIdx.x);
   const int c_hi = idle ? 0 : plan_begin(cost, ctas, blockIdx.x + 1);
@@ -739,13 +785,17 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
         auto first = [&](auto chain, auto other, int i, bool opens, bool last) {
           constexpr int w = decltype(chain)::value, v = decltype(other)::value;
           second(chain);
-          if (opens) wait(&c.q_full[w], starts[w]++);
           const int stage = i % kStages;
-          for (unsigned int it = 0; due[v] && it < kMaxPolls; ++it) {
-            if (ready(&c.full[stage], i / kStages)) break;
-            if (ready(&c.p_full[v], issued[v] - 1)) second(other);
+          bool queries = !opens, keys = false;
+          for (unsigned int it = 0; it < kMaxPolls; ++it) {
+            if (!keys) keys = ready(&c.full[stage], i / kStages);
+            if (!queries) queries = ready(&c.q_full[w], starts[w]);
+            if (queries && keys) break;
+            if (due[v] && ready(&c.p_full[v], issued[v] - 1)) second(other);
           }
-          wait(&c.full[stage], i / kStages);
+          if (!queries) wait(&c.q_full[w], starts[w]);
+          if (opens) ++starts[w];
+          if (!keys) wait(&c.full[stage], i / kStages);
           if (!ok) return;
           scores(w, w, stage);
           ++issued[w];
@@ -808,7 +858,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
     };
     auto piece_at = [&](const Cursor<kChains>& at, int number) {
       Piece x;
-      x.tiles = min(at.tiles - at.tile, (c_hi - at.at + at.weight - 1) / at.weight);
+      x.tiles = at.tiles_before(c_hi);
       x.both = kChains > 1 && at.rows(p) > kBlockRows;
       const bool split = kChains > 1 && !x.both;
       x.step = split ? 2 : 1;
@@ -861,21 +911,30 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 
     int task = 0;        // tiles this chain has taken
     int tile_index = 0;  // tiles of the CTA before the piece
-    bool open = false;   // the piece at the cursor has been opened
-    for (int number = 0; cur.at < c_hi && ok; ++number) {
-      const Piece piece = piece_at(cur, number);
-      const bool both = piece.both;
-      const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.index();
-      const int64_t part = ((int64_t)slot * kChains + w) * kBlockRows + row;
-      const bool room = slot >= 0 && slot < p.slots;
-      if (kChains > 1 && piece.mine == 0) {  // a single tile, the other chain's: an empty partial
+    int number = 0;
+    Piece piece;
+    int64_t part = 0;  // where this row's partial goes
+    bool room = false;
+    // To the next piece that this chain takes tiles of, and open it. A single tile that is the other
+    // chain's leaves an empty partial.
+    auto advance = [&] {
+      for (; cur.at < c_hi; ++number) {
+        piece = piece_at(cur, number);
+        const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.index();
+        part = ((int64_t)slot * kChains + w) * kBlockRows + row;
+        room = slot >= 0 && slot < p.slots;
+        if (kChains == 1 || piece.mine > 0) {
+          open_piece(cur, piece.both);
+          return true;
+        }
         if (room && row < cur.rows(p)) p.part_ml[part] = make_float2(neg_inf(), 0.f);
         tile_index += piece.tiles;
         cur.skip(p, plan, piece.tiles, kTok);
-        continue;
       }
-      if (!open) open_piece(cur, both);
-      open = false;
+      return false;
+    };
+    for (bool more = advance(); more && ok;) {
+      const bool both = piece.both;
       const bool act_warp = (warp & 3) * 32 < my_rows;
       const int32_t* table = cur.seg ? p.pages + (int64_t)(cur.seg - 1) * p.pages_stride : p.prefix_pages;
       // The first token that some row of the group may not see.
@@ -886,12 +945,10 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
         const int step = piece.from + k * piece.step, i = tile_index + step, stage = i % kStages;
         const int b = kChains > 1 ? w : task & 1, phase = kChains > 1 ? task : task >> 1;
         const uint32_t t_s = tmem + lanes + S::kS + b * kTok;
-        const int tile0 = (cur.tile + step) * kTok, mark = cur.at + step * cur.weight + 1;
-        ok = bar_wait(&c.s_full[b], phase & 1, s_abort);
-        // already complete: S was computed from this stage. Makes its flags and values visible here.
-        ok = ok && bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
+        const int tile0 = (cur.tile + step) * kTok, mark = cur.ahead(step) + 1;
+        // the stage's flags and, in a masked tile, its values are read here
+        ok = bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
         if (!__all_sync(~0u, ok)) break;
-        tc_fence_after();
         const bool bad_page = *const_cast<volatile int*>(&c.bad_page[stage]) == mark;
         // Which of the 64 tokens from t0 on this row sees, one bit each.
         auto visible = [&](int t0) {
@@ -913,6 +970,55 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           return bits;
         };
         const bool masked = tile0 + kTok > sure || bad_page;  // the same in the whole group
+        // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
+        // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
+        // that only some rows see are searched for infinities and NaN: those are replaced by zeros
+        // before the second product, and added afterwards to the rows that see them. All this while
+        // the first product runs.
+        bool poisoned = false;
+        const int set = both ? 0 : w;  // whose flags
+        if (masked) {
+          uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
+          const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
+          // a thread's chunk column, and every kPass-th token from its first
+          constexpr int kCols = kDim / 8, kPass = kBlockRows / kCols;
+          const int col = row % kCols, tok0 = row / kCols;
+          uint8_t* column = vt + (col / 8) * S::kSub + (col & 7) * 16;
+          if (kTma && stored < kTok) {
+            const int end = (stored + p.box_rows - 1) & -p.box_rows;
+            for (int r = stored + tok0; r < end; r += kPass)
+              *reinterpret_cast<uint4*>(column + r * 128) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          const int from = max(sure - tile0, 0);
+          if (from < stored) {
+            auto no_number = [](const uint4& x) {
+              return non_finite<T>(x.x) | non_finite<T>(x.y) | non_finite<T>(x.z) | non_finite<T>(x.w);
+            };
+            bool found = false;
+            for (int r = from + tok0; r < stored; r += kPass)
+              found |= no_number(*reinterpret_cast<const uint4*>(column + r * 128));
+            if (found) *const_cast<volatile int*>(&c.bad_value[set]) = mark;
+            sync_rows(both);
+            poisoned = *const_cast<volatile int*>(&c.bad_value[set]) == mark;
+            if (poisoned) {
+              for (int x = row; x < kTok; x += kBlockRows) c.bad_token[set][x] = 0;
+              sync_rows(both);
+              for (int r = from + tok0; r < stored; r += kPass) {
+                uint4& x = *reinterpret_cast<uint4*>(column + r * 128);
+                if (!no_number(x)) continue;
+                *const_cast<volatile unsigned char*>(&c.bad_token[set][r]) = 1;
+                x = make_uint4(finite_or_zero<T>(x.x), finite_or_zero<T>(x.y), finite_or_zero<T>(x.z),
+                               finite_or_zero<T>(x.w));
+              }
+              fence_proxy_async_smem();
+              sync_rows(both);
+            }
+          }
+        }
+        ok = bar_wait(&c.s_full[b], phase & 1, s_abort) && ok;
+        if (!__all_sync(~0u, ok)) break;
+        tc_fence_after();
         if (act_warp) {
           // 64 scores at a time. Of a tile of 128 the second half is read twice: holding both would
           // cost the registers that the rest needs.
@@ -966,68 +1072,24 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
             }
           }
           const float ref = m_ref == neg_inf() ? 0.f : m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t mul2 = pair_of(mul, mul), ref2 = pair_of(-ref, -ref);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
           for (int h = 0; h < kTok / 64; ++h) {
             if (h > 0) scores(h);
 #pragma unroll
             for (int j = 0; j < 64; j += 2) {
-              const float x = ex2(fmaf(__uint_as_float(s[j]), mul, -ref));
-              const float y = ex2(fmaf(__uint_as_float(s[j + 1]), mul, -ref));
-              sum[j & 2] += x;
-              sum[(j & 2) + 1] += y;
+              const uint64_t e = fma_pair((uint64_t)s[j + 1] << 32 | s[j], mul2, ref2);
+              const float x = ex2(__uint_as_float((uint32_t)e)), y = ex2(__uint_as_float((uint32_t)(e >> 32)));
+              sum2[(j >> 1) & 1] = add_pair(sum2[(j >> 1) & 1], pair_of(x, y));
               s[j / 2] = Pair<T>::pack(x, y);
             }
             // over scores that have been read: weights take half the columns
             tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          const uint64_t sum = add_pair(sum2[0], sum2[1]);
+          l += __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32));
           tc_wait_st();
-        }
-        // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
-        // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
-        // that only some rows see are searched for infinities and NaN: those are replaced by zeros
-        // before the second product, and added afterwards to the rows that see them.
-        bool poisoned = false;
-        const int set = both ? 0 : w;  // whose flags
-        if (masked) {
-          uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
-          const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
-          // a thread's chunk column, and every kPass-th token from its first
-          constexpr int kCols = kDim / 8, kPass = kBlockRows / kCols;
-          const int col = row % kCols, tok0 = row / kCols;
-          uint8_t* column = vt + (col / 8) * S::kSub + (col & 7) * 16;
-          if (kTma && stored < kTok) {
-            const int end = (stored + p.box_rows - 1) & -p.box_rows;
-            for (int r = stored + tok0; r < end; r += kPass)
-              *reinterpret_cast<uint4*>(column + r * 128) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-          }
-          const int from = max(sure - tile0, 0);
-          if (from < stored) {
-            auto no_number = [](const uint4& x) {
-              return non_finite<T>(x.x) | non_finite<T>(x.y) | non_finite<T>(x.z) | non_finite<T>(x.w);
-            };
-            bool found = false;
-            for (int r = from + tok0; r < stored; r += kPass)
-              found |= no_number(*reinterpret_cast<const uint4*>(column + r * 128));
-            if (found) *const_cast<volatile int*>(&c.bad_value[set]) = mark;
-            sync_rows(both);
-            poisoned = *const_cast<volatile int*>(&c.bad_value[set]) == mark;
-            if (poisoned) {
-              for (int x = row; x < kTok; x += kBlockRows) c.bad_token[set][x] = 0;
-              sync_rows(both);
-              for (int r = from + tok0; r < stored; r += kPass) {
-                uint4& x = *reinterpret_cast<uint4*>(column + r * 128);
-                if (!no_number(x)) continue;
-                *const_cast<volatile unsigned char*>(&c.bad_token[set][r]) = 1;
-                x = make_uint4(finite_or_zero<T>(x.x), finite_or_zero<T>(x.y), finite_or_zero<T>(x.z),
-                               finite_or_zero<T>(x.w));
-              }
-              fence_proxy_async_smem();
-              sync_rows(both);
-            }
-          }
         }
         tc_fence_before();
         __syncwarp();
@@ -1069,22 +1131,19 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 
       // ---- end of a piece: the next one's queries first, then O out
       const int done_rows = my_rows, last = task - 1;
+      const int64_t done_part = part;
+      const bool done_room = room;
       tile_index += piece.tiles;
+      ++number;
       cur.skip(p, plan, piece.tiles, kTok);
-      if (cur.at < c_hi) {
-        const Piece next = piece_at(cur, number + 1);
-        if (kChains == 1 || next.mine > 0) {
-          open_piece(cur, next.both);
-          open = true;
-        }
-      }
+      more = advance();
       ok = kChains > 1 ? bar_wait(&c.o_done[w], last & 1, s_abort)
                        : bar_wait(&c.o_done[last & 1], (last >> 1) & 1, s_abort);
       tc_fence_after();
       __syncwarp();
       if ((warp & 3) * 32 < done_rows) {
-        const bool act = row < done_rows && room;
-        float* dst = p.part_o + part * p.dim;
+        const bool act = row < done_rows && done_room;
+        float* dst = p.part_o + done_part * p.dim;
 #pragma unroll 1
         for (int c0 = 0; c0 < p.dim; c0 += 32) {
           uint32_t x[32];
@@ -1095,7 +1154,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
             if (act && c0 + j < p.dim) st_256(dst + c0 + j, &x[j]);
           __syncwarp();
         }
-        if (act) p.part_ml[part] = make_float2(m_ref, l);
+        if (act) p.part_ml[done_part] = make_float2(m_ref, l);
       }
       tc_fence_before();
       __syncwarp();
@@ -1113,14 +1172,62 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 }
 
 // ------------------------------------------------------------------------------------------------
-// Join: one block per (row, query head). The row's partials are those of its prefix group and of
-// its request's own group, each from a run of CTAs: partial j lies at slot from[0] + j for the first
-// n[0], at from[1] + j - n[0] for the others (two at each where the chains took turns). kThreads / kCols threads take the partials in turn, a
-// thread four dimensions of each; the first loads of O are on their way before the weights are
-// known. Sums run over fixed sets in a fixed order.
+// Join of the partials of a row: those of its prefix group and of its request's own group, each
+// from a run of CTAs.
 // ------------------------------------------------------------------------------------------------
 constexpr int kMaxPartials = 4 * kMaxCtas;
 
+// Where the partials of (row t, query head h) are: n[0] of the prefix, then n[1] of the request; two
+// in each slot where the chains took turns.
+template <int kChains>
+struct Partials {
+  int n[2], from[2], row[2], both[2];
+  __device__ __forceinline__ Partials(const AttnArgs& p, const RowPlan& r, int grid, int t, int h) {
+    const int head = p.by_group.div(h), g = h - head * p.group;
+    const Cost cost(r.even);
+    const int ctas = cost.ctas(r.cost, grid);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      n[i] = from[i] = row[i] = 0;
+      both[i] = 1;
+      const int tiles = i ? r.tiles : r.prefix_tiles, count = i ? r.count : r.prefix_count;
+      if (!r.owned || tiles == 0) continue;
+      const int f = (t - (i ? r.first : r.prefix_first)) * p.group + g;
+      const int index = f / (kChains * kBlockRows);
+      const int group = head * groups_of<kChains>(count, p.group) + index;
+      both[i] = kChains == 1 || group_rows<kChains>(count, p.group, index) > kBlockRows;
+      row[i] = f % (kChains * kBlockRows);
+      const int weight = tile_cost<kChains>(cost, count, p.group);
+      const int at = (i ? r.cost0 : 0) + group * (cost.open + tiles * weight);
+      const int last = at + (tiles > 1 ? cost.open + (tiles - 1) * weight : 0);
+      const int c0 = plan_owner(r.cost, ctas, at), c1 = plan_owner(r.cost, ctas, last);
+      from[i] = c0 + (i ? r.group0 : 0) + group;
+      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i])) * (both[i] ? 1 : 2);
+    }
+  }
+  __device__ __forceinline__ int64_t place(int j) const {
+    const bool own = j >= n[0], whole = own ? both[1] : both[0];
+    const int k = own ? j - n[0] : j, f = own ? from[1] : from[0], r = own ? row[1] : row[0];
+    // a whole group's rows run over its chains; a shared block of rows is in each
+    return (int64_t)(f + (whole ? k : k >> 1)) * (kChains * kBlockRows) + r +
+           (whole ? 0 : (k & 1) * kBlockRows);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnArgs& p, int t, int h, int col, const float4& acc,
+                                          float sum) {
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim + col * 4;
+  out[0] = T(acc.x * inv), out[1] = T(acc.y * inv), out[2] = T(acc.z * inv), out[3] = T(acc.w * inv);
+}
+__device__ __forceinline__ void write_lse(const AttnArgs& p, int t, int h, float top, float sum) {
+  p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
+}
+
+// Few rows, many partials: one block per (row, query head). kThreads / kCols threads take the
+// partials in turn, a thread four dimensions of each; the first loads of O are on their way before
+// the weights are known. Sums run over fixed sets in a fixed order.
 template <typename T, int kCols, int kThreads, int kChains>
 __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int grid) {
   constexpr int kWarps = kThreads / 32, kTeams = kThreads / kCols, kAhead = 4;
@@ -1133,44 +1240,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
   const bool col_in = col * 4 < p.dim;
   grid_dep_wait();
   grid_dep_launch();
-  const RowPlan r = p.row_plan[t];
-  const int head = p.by_group.div(h), g = h - head * p.group;
-  int from[2] = {0, 0}, n[2] = {0, 0}, row[2] = {0, 0}, both[2] = {1, 1};
-  if (r.owned) {
-    const int ctas = plan_ctas(r.cost, grid);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int tiles = i ? r.tiles : r.prefix_tiles, count = i ? r.count : r.prefix_count;
-      if (tiles == 0) continue;
-      const int f = (t - (i ? r.first : r.prefix_first)) * p.group + g;
-      const int index = f / (kChains * kBlockRows);
-      const int group = head * groups_of<kChains>(count, p.group) + index;
-      both[i] = kChains == 1 || group_rows<kChains>(count, p.group, index) > kBlockRows;
-      row[i] = f % (kChains * kBlockRows);
-      const int weight = weight_of<kChains>(count, p.group);
-      const int at = (i ? r.cost0 : 0) + group * tiles * weight;
-      const int c0 = plan_owner(r.cost, ctas, at), c1 = plan_owner(r.cost, ctas, at + (tiles - 1) * weight);
-      from[i] = c0 + (i ? r.group0 : 0) + group;
-      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i])) * (both[i] ? 1 : 2);
-    }
-  }
-  const int total = n[0] + n[1];
-  auto place = [&](int j) {
-    const int i = j >= n[0];
-    const int k = i ? j - n[0] : j;
-    const int f = i ? from[1] : from[0], r0 = i ? row[1] : row[0];
-    const bool whole = i ? both[1] : both[0];
-    // a whole group's rows run over its chains; a shared block is in each
-    return (int64_t)(f + (whole ? k : k >> 1)) * (kChains * kBlockRows) + r0 +
-           (whole ? 0 : (k & 1) * kBlockRows);
-  };
+  const Partials<kChains> at(p, p.row_plan[t], grid, t, h);
+  const int total = at.n[0] + at.n[1];
   float4 x[kAhead];
   auto fetch = [&](int j0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int j = j0 + k * kTeams;
       x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j < total && col_in) x[k] = *reinterpret_cast<const float4*>(p.part_o + place(j) * p.dim + col * 4);
+      if (j < total && col_in) x[k] = *reinterpret_cast<const float4*>(p.part_o + at.place(j) * p.dim + col * 4);
     }
   };
   constexpr int kMine = (kMaxPartials + kThreads - 1) / kThreads;
@@ -1180,7 +1258,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
   for (int k = 0; k < kMine; ++k) {
     const int j = threadIdx.x + k * kThreads;
     ml[k] = make_float2(neg_inf(), 0.f);
-    if (j < total) ml[k] = p.part_ml[place(j)];
+    if (j < total) ml[k] = p.part_ml[at.place(j)];
   }
   fetch(team);
 #pragma unroll
@@ -1226,12 +1304,71 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
       const float4 y = s_acc[k * kCols + threadIdx.x];
       acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
     }
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-    T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim + col * 4;
-    out[0] = T(acc.x * inv), out[1] = T(acc.y * inv), out[2] = T(acc.z * inv), out[3] = T(acc.w * inv);
+    write_row<T>(p, t, h, col, acc, sum);
   }
-  if (threadIdx.x == 0)
-    p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
+  if (threadIdx.x == 0) write_lse(p, t, h, top, sum);
+}
+
+// Many rows, few partials each: one warp per (row, query head), 32 partials at a time.
+constexpr int kJoinWarps = 4;
+
+template <typename T, int kCols, int kChains>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const AttnArgs p, int grid) {
+  constexpr int kMine = (kCols + 31) / 32, kAhead = 4;
+  const int lane = threadIdx.x & 31, i = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  grid_dep_wait();
+  grid_dep_launch();
+  if (i >= p.rows * p.q_heads) return;
+  const int t = i / p.q_heads, h = i - t * p.q_heads;
+  const Partials<kChains> at(p, p.row_plan[t], grid, t, h);
+  const int total = at.n[0] + at.n[1];
+  float top = neg_inf(), sum = 0.f;
+  float4 acc[kMine];
+#pragma unroll
+  for (int c = 0; c < kMine; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = 0; j0 < total; j0 += 32) {
+    const int n = min(32, total - j0);
+    float2 ml = make_float2(neg_inf(), 0.f);
+    if (lane < n) ml = p.part_ml[at.place(j0 + lane)];
+    float m = ml.x;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    m = fmaxf(m, top);
+    const float safe = m == neg_inf() ? 0.f : m, f = ex2(top - safe), w = ex2(ml.x - safe);
+    top = m;
+    float part = ml.y * w;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(~0u, part, d);
+    sum = sum * f + part;
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) acc[c].x *= f, acc[c].y *= f, acc[c].z *= f, acc[c].w *= f;
+    for (int j = 0; j < n; j += kAhead) {
+      float4 x[kAhead][kMine];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+          const int col = lane + 32 * c;
+          x[k][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (j + k < n && col * 4 < p.dim)
+            x[k][c] = *reinterpret_cast<const float4*>(p.part_o + at.place(j0 + j + k) * p.dim + col * 4);
+        }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const float v = __shfl_sync(~0u, w, (j + k) & 31);
+        if (j + k >= n || v == 0.f) continue;  // an empty partial has no O
+#pragma unroll
+        for (int c = 0; c < kMine; ++c) {
+          acc[c].x += x[k][c].x * v, acc[c].y += x[k][c].y * v;
+          acc[c].z += x[k][c].z * v, acc[c].w += x[k][c].w * v;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kMine; ++c)
+    if ((lane + 32 * c) * 4 < p.dim) write_row<T>(p, t, h, lane + 32 * c, acc[c], sum);
+  if (lane == 0) write_lse(p, t, h, top, sum);
 }
 
 int round_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -1263,13 +1400,14 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int 
   }
   int rc = launch_kernel(kernel, ctas, S::kThreads, smem, stream, /*early=*/true, mk, mv, p);
   if (rc) return rc;
-  // Partials of a row: about as many as CTAs per group. Few of them: few threads.
-  const int64_t rows = (int64_t)p.rows * p.group;
-  const int64_t groups = p.kv_heads * ((rows + kChains * kBlockRows - 1) / (kChains * kBlockRows));
+  // A warp each where there are many rows with few partials, else a block each. Of a prefix a row has
+  // about as many partials as CTAs work on its group.
+  const int64_t groups = p.kv_heads * (((int64_t)p.rows * p.group + kChains * kBlockRows - 1) /
+                                       (kChains * kBlockRows));
   const int grid = p.rows * p.q_heads;
-  if (ctas / groups <= 8)
-    return launch_kernel(join_kernel<T, kDim / 4, 128, kChains>, grid, 128, 0, stream, /*early=*/true, p,
-                         ctas);
+  if (grid > 3 * ctas && ctas <= 24 * groups)
+    return launch_kernel(join_rows_kernel<T, kDim / 4, kChains>, (grid + kJoinWarps - 1) / kJoinWarps,
+                         kJoinWarps * 32, 0, stream, /*early=*/true, p, ctas);
   return launch_kernel(join_kernel<T, kDim / 4, 512, kChains>, grid, 512, 0, stream, /*early=*/true, p,
                        ctas);
 }
@@ -1395,7 +1533,7 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   // costs are counted in 32 bits
   const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
   const int64_t tiles = ((int64_t)std::max(n_prefix_pages, max_pages) * page_size + tok - 1) / tok;
-  if ((2 * blocks + requests) * kv_heads * tiles * kMaxWeight > 0x7fffffff)
+  if ((2 * blocks + requests) * kv_heads * tiles * kMaxCost > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "%s: tables too long for %d rows", op, rows);
   DeviceInfo di;
   rc = device_info(&di);
