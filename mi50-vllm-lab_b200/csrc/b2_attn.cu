@@ -203,6 +203,16 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b_desc, 
       "r"(a), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
+// The same with A in shared memory.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
 // Shared-memory descriptor, 128-byte swizzle; byte offsets between repeats of the 8-row pattern.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(leading >> 4) << 16 |
@@ -431,15 +441,17 @@ struct Cursor {
 // ------------------------------------------------------------------------------------------------
 // Main kernel. kDim: head dimension rounded up (64, 128, 256), the rest of it zero.
 //
-// Per tile: S[128 rows, kTok] = Q K^T and O[128 rows, kDim] += P V on the tensor cores, with Q, S,
-// P and O in tensor memory (P takes the place of its S), K and V in a ring of shared-memory stages.
-// K is the product's B operand with the dimension contiguous, V its B operand with N contiguous:
-// both lie as loaded, [token][64 dimensions] rows of 128 bytes, swizzled.
+// Per tile: S[128 rows, kTok] = Q K^T and O[128 rows, kDim] += P V on the tensor cores, with Q, S and
+// O in tensor memory, K and V in a ring of shared-memory stages. K is the product's B operand with
+// the dimension contiguous, V its B operand with N contiguous: both lie as loaded, [token][64
+// dimensions] rows of 128 bytes, swizzled.
 //
 // Chains: tensor memory holds two sets of O, S and Q up to kDim = 128, one at 256. With two, groups
 // of more than 128 rows give each chain a block of rows and both take every tile, so K and V are
 // brought in once for 256 rows; smaller groups give both chains the same rows, and the tiles in
-// turn, so two tiles are under way at a time. With one, S alone is held twice.
+// turn, so two tiles are under way at a time. P goes through shared memory, which frees S as soon as
+// it has been read: the next tile's first product runs while the softmax works. With one chain, S
+// is held twice, and P takes the place of its S.
 //   warps 0-3 (4-7)  softmax of a chain: a thread owns a row (its lane of tensor memory), so the
 //                    running maximum and sum need no exchange between threads; they also bring Q
 //                    in and take O out
@@ -457,7 +469,8 @@ struct Shape {
   static constexpr int kLoadWarps = kTma ? 2 : kLoadThreads / 32;
   static constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
   static constexpr int kTok = kDim == 64 ? 128 : 64;  // tokens per tile
-  static constexpr int kStages = kDim == 256 ? 3 : 4;
+  static constexpr int kStages = kDim == 256 ? 3 : kDim == 128 ? 5 : 4;
+  static constexpr int kP = kChains > 1 ? kTok * kBlockRows * 2 : 0;  // P of a chain, in shared memory
   static constexpr int kSub = kTok * 128;           // [token][64 dimensions] of K or V
   static constexpr int kHalf = kSub * (kDim / 64);  // K or V of a stage
   static constexpr int kRing = kStages * 2 * kHalf;
@@ -470,6 +483,7 @@ struct Shape {
 struct Control {
   uint64_t full[6], empty[6];
   uint64_t s_full[2], p_full[2], o_done[2];  // per S: of a chain, or of every other tile
+  uint64_t s_free[2];                        // per chain: S has been read
   uint64_t q_full[2], o_free[2], sync[3];    // per chain; sync[2]: both
   uint64_t drain;
   uint32_t tmem;
@@ -481,14 +495,15 @@ struct Control {
 
 template <int kDim, bool kTma>
 constexpr size_t attn_smem() {
-  return 1024 + Shape<kDim, kTma>::kRing + sizeof(Plan) + sizeof(Control) + 16;
+  return 1024 + Shape<kDim, kTma>::kRing + Shape<kDim, kTma>::kChains * Shape<kDim, kTma>::kP + sizeof(Plan) + sizeof(Control) + 16;
 }
 
 __device__ int g_attn_status;
 
-// mbar_wait without its suspend-time hint: the waits of this kernel are short.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_test(bar, parity)) return true;
+// mbar_wait without its suspend-time hint: the waits of this kernel are short. One test in line,
+// which suspends the thread for a while, and the rest out of line: the code of the roles shares the
+// instruction caches of an SM.
+__device__ __noinline__ bool bar_wait_on(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const unsigned long long t0 = globaltimer_ns();
   for (unsigned int it = 1; it < kMaxSpin; ++it) {
     if (mbar_test(bar, parity)) return true;
@@ -499,6 +514,9 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
   }
   *abort = 1;
   return false;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_test(bar, parity) || bar_wait_on(bar, parity, abort);
 }
 // Has the phase completed? Never suspends the thread.
 __device__ __forceinline__ bool mbar_test_now(uint64_t* bar, uint32_t parity) {
@@ -523,7 +541,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Control& c = *reinterpret_cast<Control*>(smem + S::kRing);
+  Control& c = *reinterpret_cast<Control*>(smem + S::kRing + kChains * S::kP);
   Plan& plan = *reinterpret_cast<Plan*>((reinterpret_cast<uintptr_t>(&c + 1) + 15) & ~(uintptr_t)15);
   volatile int* s_abort = &c.abort;
 
@@ -540,6 +558,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       mbar_init(&c.s_full[b], 1);
       mbar_init(&c.p_full[b], 4);
       mbar_init(&c.o_done[b], 1);
+      mbar_init(&c.s_free[b], 4);
       mbar_init(&c.q_full[b], 4);
       mbar_init(&c.o_free[b], 4);
       mbar_init(&c.sync[b], 4);
@@ -551,12 +570,18 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
     mbar_fence_init();
   }
   if (warp == kSoftWarps) tmem_alloc(&c.tmem, S::kColumns);
-  {  // page tables into L2 behind the plan
+  {  // page tables and queries into L2 behind the plan
     const int line = 32, step = gridDim.x * blockDim.x * line;
     const int at = (blockIdx.x * blockDim.x + threadIdx.x) * line;
     for (int i = at; i < p.n_prefix_pages; i += step) prefetch_l2(p.prefix_pages + i);
     const int64_t all = p.requests > 0 ? (p.requests - 1) * p.pages_stride + p.max_pages : 0;
     for (int64_t i = at; i < all; i += step) prefetch_l2(p.pages + i);
+    const int n = p.rows * p.q_heads, first = blockIdx.x * blockDim.x + threadIdx.x;
+    for (int i = first; i < n; i += gridDim.x * blockDim.x) {
+      const int row = i / p.q_heads;
+      const T* q = static_cast<const T*>(p.q) + row * p.q_row + (i - row * p.q_heads) * p.q_head;
+      for (int d = 0; d < p.dim; d += 64) prefetch_l2(q + d);
+    }
   }
   grid_dep_wait();
   grid_dep_launch();
@@ -705,7 +730,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       constexpr uint32_t kIdescS = instr_desc<T>(kTok, false), kIdescO = instr_desc<T>(kDim, true);
       const bool leader = elect_one();
       bool ok = true;
-      auto wait = [&](uint64_t* bar, int phase) {
+      [[maybe_unused]] auto wait = [&](uint64_t* bar, int phase) {
         ok = ok && __all_sync(~0u, bar_wait(bar, phase & 1, s_abort));
       };
       auto ready = [&](uint64_t* bar, int phase) {
@@ -723,21 +748,28 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
             tc_mma(sd, qd + ks * 8, kd + (((ks / 4) * S::kSub + (ks % 4) * 32) >> 4), kIdescS, ks > 0);
           tc_commit(&c.s_full[b]);
         }
-        __syncwarp();
+        if constexpr (kChains == 1) __syncwarp();
       };
       // O (+)= P V of a stage, for chain w from S number b; `last`: nothing else reads the stage
       auto weigh = [&](int w, int b, int stage, bool first, bool last) {
         tc_fence_after();
         const uint64_t vd = smem_desc(ring + stage * stage_bytes + S::kHalf, S::kSub, 1024);
         const uint32_t pa = tmem + S::kS + b * kTok, od = tmem + w * kDim;
+        const uint64_t pd = smem_desc(ring + S::kRing + w * S::kP, 16, 1024);
         if (leader) {
 #pragma unroll
-          for (int ks = 0; ks < kTok / 16; ++ks)
-            tc_mma(od, pa + ks * 8, vd + ks * (2048 >> 4), kIdescO, ks > 0 || !first);
+          for (int ks = 0; ks < kTok / 16; ++ks) {
+            const uint64_t v = vd + ks * (2048 >> 4);
+            if constexpr (kChains > 1)
+              tc_mma_ss(od, pd + (((ks / 4) * kBlockRows * 128 + (ks % 4) * 32) >> 4), v, kIdescO,
+                        ks > 0 || !first);
+            else
+              tc_mma(od, pa + ks * 8, v, kIdescO, ks > 0 || !first);
+          }
           if (last) tc_commit(&c.empty[stage]);
           tc_commit(&c.o_done[b]);
         }
-        __syncwarp();
+        if constexpr (kChains == 1) __syncwarp();
       };
       if constexpr (kChains == 1) {
         int opened = 0, starts = 0, n = 0;
@@ -770,62 +802,82 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
         }
         if (n > 0) second(n - 1, before);
       } else {
-        // Per chain: first products issued, pieces opened by a first and by a second product; whether
-        // a second product is due, and its stage and flags.
-        int issued[2] = {0, 0}, opened[2] = {0, 0}, starts[2] = {0, 0}, stages[2] = {0, 0};
-        bool due[2] = {false, false}, firsts[2] = {false, false}, lasts[2] = {false, false};
-        auto second = [&](auto chain) {
-          constexpr int w = decltype(chain)::value;
-          if (!due[w]) return;
-          wait(&c.p_full[w], issued[w] - 1);
-          if (firsts[w] && opened[w]++ > 0) wait(&c.o_free[w], opened[w] - 2);
-          if (ok) weigh(w, w, stages[w], firsts[w], lasts[w]);
-          due[w] = false;
+        // One thread: straight code that waits for what it needs, in the order in which it is needed.
+        // Per chain, a bit each: parity of the first and second products issued, of the pieces opened
+        // by a first and by a second product, and whether there was one at all.
+        int issued = 0, weighed = 0, starts = 0, opened = 0, any_issued = 0, any_opened = 0;
+        auto wait1 = [&](uint64_t* bar, int phase) { ok = ok && bar_wait(bar, phase & 1, s_abort); };
+        auto first = [&](int w, int stage) {
+          if ((any_issued >> w) & 1) wait1(&c.s_free[w], (issued >> w) ^ 1);
+          if (ok) scores(w, w, stage);
+          issued ^= 1 << w, any_issued |= 1 << w;
         };
-        auto first = [&](auto chain, auto other, int i, bool opens, bool last) {
-          constexpr int w = decltype(chain)::value, v = decltype(other)::value;
-          second(chain);
-          const int stage = i % kStages;
-          bool queries = !opens, keys = false;
-          for (unsigned int it = 0; it < kMaxPolls; ++it) {
-            if (!keys) keys = ready(&c.full[stage], i / kStages);
-            if (!queries) queries = ready(&c.q_full[w], starts[w]);
-            if (queries && keys) break;
-            if (due[v] && ready(&c.p_full[v], issued[v] - 1)) second(other);
-          }
-          if (!queries) wait(&c.q_full[w], starts[w]);
-          if (opens) ++starts[w];
-          if (!keys) wait(&c.full[stage], i / kStages);
-          if (!ok) return;
-          scores(w, w, stage);
-          ++issued[w];
-          due[w] = true;
-          stages[w] = stage, firsts[w] = opens, lasts[w] = last;
+        auto second = [&](int w, int stage, bool opens, bool last) {
+          wait1(&c.p_full[w], weighed >> w);
+          if (opens && ((any_opened >> w) & 1)) wait1(&c.o_free[w], (opened >> w) ^ 1);
+          if (ok) weigh(w, w, stage, opens, last);
+          weighed ^= 1 << w;
+          if (opens) opened ^= 1 << w, any_opened |= 1 << w;
         };
-        const std::integral_constant<int, 0> A;
-        const std::integral_constant<int, 1> B;
-        int piece = -1, t = 0;
-        bool both = false;
-        for (int n = 0; cur.at < c_hi && ok; ++n, ++t) {
-          if (n == 0 || cur.tile == 0) {
-            // The chains of a shared tile release its stage together, in this order.
-            if (both) second(A), second(B);
-            ++piece;
-            t = 0;
-            both = cur.rows(p) > kBlockRows;
-          }
-          if (both) {
-            first(A, B, n, t == 0, false);
-            first(B, A, n, t == 0, true);
-          } else if (((t + piece) & 1) == 0) {
-            first(A, B, n, t < 2, true);
+        auto queries = [&](int w) {
+          wait1(&c.q_full[w], starts >> w);
+          starts ^= 1 << w;
+        };
+        int due = 0, due_opens = 0, due_stage0 = 0, due_stage1 = 0;  // second products, per chain
+        auto settle = [&](int w) {
+          if (!((due >> w) & 1)) return;
+          second(w, w ? due_stage1 : due_stage0, (due_opens >> w) & 1, true);
+          due &= ~(1 << w);
+        };
+        for (int n = 0, stage = 0, turn = 0; leader && cur.at < c_hi && ok;) {
+          const int tiles = cur.tiles_before(c_hi);
+          auto step = [&] {
+            if (++stage == kStages) stage = 0, turn ^= 1;
+            ++n;
+          };
+          if (cur.rows(p) > kBlockRows) {
+            // Both chains take every tile: its first products before the second ones of the tile
+            // before, for which the softmax has yet to finish.
+            settle(n & 1);
+            settle((n & 1) ^ 1);
+            queries(0);
+            queries(1);
+            int before = 0;
+            for (int t = 0; t <= tiles && ok; ++t) {
+              if (t < tiles) {
+                wait1(&c.full[stage], turn);
+                first(0, stage);
+                first(1, stage);
+              }
+              if (t > 0) {
+                second(0, before, t == 1, false);
+                second(1, before, t == 1, true);
+              }
+              before = stage;
+              if (t < tiles) step();
+            }
           } else {
-            first(B, A, n, t < 2, true);
+            // The chains take turns. The second product of a chain's tile comes before the first one
+            // of its next, which may wait for its keys; the other chain works meanwhile.
+            for (int t = 0; t < tiles && ok; ++t) {
+              const int w = n & 1;
+              settle(w);
+              if (t < 2) queries(w);
+              wait1(&c.full[stage], turn);
+              first(w, stage);
+              due |= 1 << w;
+              due_opens = t < 2 ? due_opens | 1 << w : due_opens & ~(1 << w);
+              if (w) due_stage1 = stage; else due_stage0 = stage;
+              step();
+            }
           }
-          cur.skip(p, plan, 1, kTok);
+          cur.skip(p, plan, tiles, kTok);
+          if (cur.at >= c_hi) {
+            settle(n & 1);
+            settle((n & 1) ^ 1);
+          }
         }
-        second(A);
-        second(B);
+        ok = __all_sync(~0u, ok);
       }
       if (!ok) {  // let what is in flight land before the tensor memory is freed
         if (leader) tc_commit(&c.drain);
@@ -856,13 +908,13 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       int tiles, mine, from, step;
       bool both;
     };
-    auto piece_at = [&](const Cursor<kChains>& at, int number) {
+    auto piece_at = [&](const Cursor<kChains>& at, int index) {
       Piece x;
       x.tiles = at.tiles_before(c_hi);
       x.both = kChains > 1 && at.rows(p) > kBlockRows;
       const bool split = kChains > 1 && !x.both;
       x.step = split ? 2 : 1;
-      x.from = split ? (w + number) & 1 : 0;
+      x.from = split ? (w + index) & 1 : 0;
       x.mine = split ? (x.tiles - x.from + 1) / 2 : x.tiles;
       return x;
     };
@@ -911,15 +963,14 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 
     int task = 0;        // tiles this chain has taken
     int tile_index = 0;  // tiles of the CTA before the piece
-    int number = 0;
     Piece piece;
     int64_t part = 0;  // where this row's partial goes
     bool room = false;
     // To the next piece that this chain takes tiles of, and open it. A single tile that is the other
     // chain's leaves an empty partial.
     auto advance = [&] {
-      for (; cur.at < c_hi; ++number) {
-        piece = piece_at(cur, number);
+      while (cur.at < c_hi) {
+        piece = piece_at(cur, tile_index);
         const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.index();
         part = ((int64_t)slot * kChains + w) * kBlockRows + row;
         room = slot >= 0 && slot < p.slots;
@@ -1041,6 +1092,12 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
               __syncwarp();
             }
           };
+          // S has been read: the next tile's may take its place
+          auto give_back = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.s_free[w]);
+          };
           float mx4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
           for (int h = kTok / 64 - 1; h >= 0; --h) {
@@ -1049,6 +1106,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
             for (int j = 0; j < 64; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
           }
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
+          if constexpr (kChains > 1 && kTok == 64) give_back();
           const bool grow = mx > m_ref + 8.f || (m_ref == neg_inf() && mx > neg_inf());
           if (__any_sync(~0u, grow)) {
             const float f = grow ? ex2(m_ref - mx) : 1.f;
@@ -1069,14 +1127,20 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
                 for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
                 tmem_st32(t_o + c0, x);
               }
+              tc_wait_st();
             }
           }
+          // P of the chain's last tile has been used
+          if (kChains > 1 && task > 0) ok = bar_wait(&c.o_done[w], (task - 1) & 1, s_abort) && ok;
           const float ref = m_ref == neg_inf() ? 0.f : m_ref;
           const uint64_t mul2 = pair_of(mul, mul), ref2 = pair_of(-ref, -ref);
           uint64_t sum2[2] = {0, 0};
 #pragma unroll
           for (int h = 0; h < kTok / 64; ++h) {
-            if (h > 0) scores(h);
+            if (h > 0) {
+              scores(h);
+              if constexpr (kChains > 1) give_back();
+            }
 #pragma unroll
             for (int j = 0; j < 64; j += 2) {
               const uint64_t e = fma_pair((uint64_t)s[j + 1] << 32 | s[j], mul2, ref2);
@@ -1084,12 +1148,28 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
               sum2[(j >> 1) & 1] = add_pair(sum2[(j >> 1) & 1], pair_of(x, y));
               s[j / 2] = Pair<T>::pack(x, y);
             }
-            // over scores that have been read: weights take half the columns
-            tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
+            if constexpr (kChains > 1) {
+              uint8_t* to = smem + S::kRing + w * S::kP + h * kBlockRows * 128 + row * 128;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4*>(to + ((j ^ (row & 7)) << 4)) =
+                    make_uint4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
+            } else {
+              // over scores that have been read: weights take half the columns
+              tmem_st32(t_s + h * 32, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
+            }
           }
           const uint64_t sum = add_pair(sum2[0], sum2[1]);
           l += __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32));
-          tc_wait_st();
+          if constexpr (kChains > 1)
+            fence_proxy_async_smem();
+          else
+            tc_wait_st();
+        } else if constexpr (kChains > 1) {
+          if (lane == 0) mbar_arrive(&c.s_free[w]);
+          // A warp without rows waits as the others do: its arrival for this tile must not be counted
+          // for the one before.
+          if (task > 0) ok = bar_wait(&c.o_done[w], (task - 1) & 1, s_abort) && ok;
         }
         tc_fence_before();
         __syncwarp();
@@ -1134,7 +1214,6 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       const int64_t done_part = part;
       const bool done_room = room;
       tile_index += piece.tiles;
-      ++number;
       cur.skip(p, plan, piece.tiles, kTok);
       more = advance();
       ok = kChains > 1 ? bar_wait(&c.o_done[w], last & 1, s_abort)
