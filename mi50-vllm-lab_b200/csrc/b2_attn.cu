@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       c.bad_page[s] = 0;
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&c.s_full[b], 1);
+      mbar_init(&c.s_full[b], 2);  // the products' completion, and the thread that issued them
       mbar_init(&c.p_full[b], 4);
       mbar_init(&c.o_done[b], 1);
       mbar_init(&c.s_free[b], 4);
@@ -747,6 +747,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           for (int ks = 0; ks < kDim / 16; ++ks)
             tc_mma(sd, qd + ks * 8, kd + (((ks / 4) * S::kSub + (ks % 4) * 32) >> 4), kIdescS, ks > 0);
           tc_commit(&c.s_full[b]);
+          mbar_arrive(&c.s_full[b]);
         }
         if constexpr (kChains == 1) __syncwarp();
       };
@@ -997,10 +998,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
         const int b = kChains > 1 ? w : task & 1, phase = kChains > 1 ? task : task >> 1;
         const uint32_t t_s = tmem + lanes + S::kS + b * kTok;
         const int tile0 = (cur.tile + step) * kTok, mark = cur.ahead(step) + 1;
-        // the stage's flags and, in a masked tile, its values are read here
-        ok = bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
-        if (!__all_sync(~0u, ok)) break;
-        const bool bad_page = *const_cast<volatile int*>(&c.bad_page[stage]) == mark;
+        bool bad_page = false;
         // Which of the 64 tokens from t0 on this row sees, one bit each.
         auto visible = [&](int t0) {
           auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
@@ -1020,7 +1018,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           }
           return bits;
         };
-        const bool masked = tile0 + kTok > sure || bad_page;  // the same in the whole group
+        const bool tail = tile0 + kTok > sure;  // the same in the whole group
         // 0 * NaN would carry values that are no numbers into rows that do not see them. Behind the
         // length, a box may have brought what the rest of its page holds: zeros in its place. Tokens
         // that only some rows see are searched for infinities and NaN: those are replaced by zeros
@@ -1028,7 +1026,9 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
         // the first product runs.
         bool poisoned = false;
         const int set = both ? 0 : w;  // whose flags
-        if (masked) {
+        if (tail) {
+          ok = bar_wait(&c.full[stage], (i / kStages) & 1, s_abort);
+          if (!__all_sync(~0u, ok)) break;
           uint8_t* vt = smem + stage * stage_bytes + S::kHalf;
           const int stored = min(cur.len - tile0, kTok);  // tokens of the tile
           // a thread's chunk column, and every kPass-th token from its first
@@ -1074,12 +1074,20 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           // 64 scores at a time. Of a tile of 128 the second half is read twice: holding both would
           // cost the registers that the rest needs.
           uint32_t s[64];
-          const bool plain = !masked && p.scale_log2 > 0.f;
-          const float mul = plain ? p.scale_log2 : 1.f;
-          auto scores = [&](int h) {
+          bool masked = tail, plain = false;
+          float mul = 1.f;
+          auto scores = [&](int h, bool again) {
 #pragma unroll
             for (int j = 0; j < 64; j += 32)
               tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[j]), t_s + h * 64 + j);
+            if (!again && h == kTok / 64 - 1) {
+              // The stage's flag, while the scores arrive: visible through the issuing thread, which
+              // waited for the stage and then arrived on s_full.
+              bad_page = *const_cast<volatile int*>(&c.bad_page[stage]) == mark;
+              masked = tail || bad_page;
+              plain = !masked && p.scale_log2 > 0.f;
+              mul = plain ? p.scale_log2 : 1.f;
+            }
             tc_wait_ld();
             if (!plain) {
               const unsigned long long bits = masked ? visible(tile0 + h * 64) : ~0ull;
@@ -1101,7 +1109,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           float mx4[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
           for (int h = kTok / 64 - 1; h >= 0; --h) {
-            scores(h);
+            scores(h, false);
 #pragma unroll
             for (int j = 0; j < 64; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
           }
@@ -1130,15 +1138,13 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
               tc_wait_st();
             }
           }
-          // P of the chain's last tile has been used
-          if (kChains > 1 && task > 0) ok = bar_wait(&c.o_done[w], (task - 1) & 1, s_abort) && ok;
           const float ref = m_ref == neg_inf() ? 0.f : m_ref;
           const uint64_t mul2 = pair_of(mul, mul), ref2 = pair_of(-ref, -ref);
           uint64_t sum2[2] = {0, 0};
 #pragma unroll
           for (int h = 0; h < kTok / 64; ++h) {
             if (h > 0) {
-              scores(h);
+              scores(h, true);
               if constexpr (kChains > 1) give_back();
             }
 #pragma unroll
@@ -1149,6 +1155,8 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
               s[j / 2] = Pair<T>::pack(x, y);
             }
             if constexpr (kChains > 1) {
+              // once P of the chain's last tile has been used
+              if (h == 0 && task > 0) ok = bar_wait(&c.o_done[w], (task - 1) & 1, s_abort) && ok;
               uint8_t* to = smem + S::kRing + w * S::kP + h * kBlockRows * 128 + row * 128;
 #pragma unroll
               for (int j = 0; j < 8; ++j)
