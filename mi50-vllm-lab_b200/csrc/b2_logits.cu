@@ -14,10 +14,17 @@
 // keeps one 32-bit word per token of its slice in shared memory. The CTAs read an eighth of the
 // history each and post every token to the word of its owner through distributed shared memory
 // (integer atomics: the order does not matter), so that the history crosses L2 once per cluster
-// however long it is. Then each CTA streams its slice of logits through the words.
-//   word = [31] in the prompt | [30:20] 1 + index of the token's first bias entry | [19:0] n
-// Several bias entries for one token are added in list order in fp64 by the thread that holds the
-// first of them; the result does not depend on timing.
+// however long it is. Then each CTA takes its slice of logits through the words. The logits, the
+// mask and the first tokens of the history are loaded into registers before all this, so that one
+// latency covers them.
+//   word = [31] in the prompt | [30:20] key of the token's first bias entry | [19:0] n
+// The first of the bias entries for a token wins its word by an atomic maximum of keys that fall
+// with the index; its thread adds the others, if there are any, in list order in fp64. The result
+// does not depend on timing.
+//
+// Vectors: with columns counted from the last multiple of 8 elements at or before the row's start
+// (`shift` columns before it), vectors of 8 are aligned in the logits and in the output alike, for
+// any vocabulary size, as long as the rows of both start at the same place modulo 8.
 //
 // Bound: memory (logits once, fp32 out once); for few rows the latency of history -> words ->
 // stream.
@@ -34,10 +41,12 @@ namespace {
 
 constexpr int kCluster = 8;
 constexpr int kThreads = 512;
-constexpr int kVec = 8;                     // tokens per thread and step
-constexpr int kMaxSlice = 40960;            // words of shared memory per CTA
-constexpr int kMaxBias = 2047;              // 11 bits of the word
-constexpr int kMaxHistory = (1 << 20) - 1;  // 20 bits
+constexpr int kVec = 8;                                // tokens per thread and step
+constexpr int kSteps = 5;                              // steps of a slice
+constexpr int kMaxSlice = kThreads * kVec * kSteps;    // words of shared memory per CTA
+constexpr int kAhead = 4;                              // tokens of the history loaded at a time
+constexpr int kMaxBias = 2047;                         // 11 bits of the word
+constexpr int kMaxHistory = (1 << 20) - 1;             // 20 bits
 constexpr uint32_t kPromptBit = 0x80000000u;
 
 struct LogitArgs {
@@ -55,8 +64,9 @@ struct LogitArgs {
   int mask_words;
   int vocab, vocab_start, seqs, max_tokens, n_bias;
   int tokens64;
-  int slice;     // tokens per CTA, a multiple of kVec
+  int slice;     // columns per CTA, a multiple of kVec
   int clusters;  // clusters per row
+  FastDiv by_slice;
 };
 
 __device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t v) {
@@ -70,11 +80,11 @@ __device__ __forceinline__ float lo_f(float v) { return v; }
 __device__ __forceinline__ float lo_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float lo_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// 32 mask bits from bit position `bit` on (the words behind the row's end read as zero).
+// kVec mask bits from bit position `bit` on (those before and behind the row read as zero).
 __device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, int bit) {
-  const int w = bit >> 5, sh = bit & 31;
-  const uint32_t lo = w < words ? row[w] : 0u;
-  const uint32_t hi = (sh && w + 1 < words) ? row[w + 1] : 0u;
+  const int w = bit >> 5, sh = bit & 31;  // bit may be negative: floor, remainder
+  const uint32_t lo = w >= 0 && w < words ? row[w] : 0u;
+  const uint32_t hi = (sh > 32 - kVec && w + 1 >= 0 && w + 1 < words) ? row[w + 1] : 0u;
   return __funnelshift_r(lo, hi, sh);
 }
 
@@ -96,15 +106,24 @@ __device__ __forceinline__ float process(float x, uint32_t word, const RowParams
   return x;
 }
 
-// kVector: rows of logits and of the output are 16-byte aligned.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// kVector: vectors of 8 columns (see above); otherwise element by element, for any strides.
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
   extern __shared__ __align__(16) uint32_t words[];
   const int rank = (int)cluster_ctarank();
   const int cluster = blockIdx.x / kCluster;
   const int row = cluster / p.clusters, part = cluster - row * p.clusters;
-  const int lo = (part * kCluster + rank) * p.slice;  // first column of this CTA
-  const int n = max(0, min(p.slice, p.vocab - lo));
+  // columns with the shift: the row's are shift .. shift + vocab - 1
+  const int shift = kVector ? (int)((int64_t)row * p.vocab & 7) : 0;
+  const int first = part * kCluster * p.slice, lo = first + rank * p.slice;  // of the cluster, the CTA
+  const int from = max(0, shift - lo), to = min(p.slice, p.vocab + shift - lo);  // of the slice
   float* bias_sums = reinterpret_cast<float*>(words + p.slice);
   int32_t* bias_ids = reinterpret_cast<int32_t*>(bias_sums + p.n_bias);
   const bool history = p.tokens != nullptr;
@@ -117,114 +136,167 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
   grid_dep_wait();
   grid_dep_launch();
 
+  // ---- loads ahead: the slice's logits and mask, the first tokens
+  const T* in = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + lo - shift;
+  float* out = p.out + (int64_t)row * p.vocab + lo - shift;
+  const uint32_t* mask = p.mask ? p.mask + (int64_t)row * p.mask_stride : nullptr;
+  const int bit0 = p.vocab_start + lo - shift;
+  constexpr int kLoads = kVec * sizeof(T) / 16;
+  uint4 raw[kVector ? kSteps : 1][kLoads];
+  uint32_t bits[kVector ? kSteps : 1];
+  if constexpr (kVector) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int i = (s * kThreads + threadIdx.x) * kVec;
+      if (i >= from && i + kVec <= to) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) raw[s][j] = reinterpret_cast<const uint4*>(in + i)[j];
+      } else {
+        T e[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) e[j] = i + j >= from && i + j < to ? in[i + j] : T(0.f);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) raw[s][j] = reinterpret_cast<const uint4*>(e)[j];
+      }
+      bits[s] = mask && i < to ? mask_bits(mask, p.mask_words, bit0 + i) : ~0u;
+    }
+  }
+  int total = 0, prompt = 0;
+  int64_t at = 0;
+  if (history) {
+    const int seq = p.row_seq ? p.row_seq[row] : row;
+    if (seq >= 0 && seq < p.seqs) {
+      total = min(max(p.total_lens[row], 0), p.max_tokens);
+      prompt = p.prompt_lens[row];
+      at = (int64_t)seq * p.tokens_stride;
+    }
+  }
+  int32_t ids[kAhead];  // columns of the cluster, or -1
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kCluster * kThreads;
+      int64_t id = -1;
+      if (i < total)
+        id = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at + i]
+                        : (int64_t)static_cast<const int32_t*>(p.tokens)[at + i];
+      const int64_t col = id - p.vocab_start;
+      ids[k] = col >= 0 && col < p.vocab ? (int32_t)col + shift - first : -1;
+    }
+  };
+  const int mine = rank * kThreads + threadIdx.x;
+  if (history) fetch(mine);
   RowParams rp = {1.f, 0.f, 0.f};
   if (p.repetition) rp.rep = p.repetition[row];
   if (p.frequency) rp.freq = p.frequency[row];
   if (p.presence) rp.pres = p.presence[row];
 
+  // ---- biases: keys into the words, sums by key
+  if (p.n_bias > 0) {
+    const int64_t list = (int64_t)row * p.n_bias;
+    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
+      const int id = p.bias_ids[list + e];
+      const int64_t col = id < 0 ? -1 : (int64_t)id - p.vocab_start + shift - lo;
+      bias_ids[e] = col >= from && col < to ? (int)col : -1;
+      bias_sums[p.n_bias - 1 - e] = p.bias_values[list + e];  // by key - 1
+    }
+    __syncthreads();  // the words are zero, the list is here
+    for (int e = threadIdx.x; e < p.n_bias; e += kThreads)
+      if (bias_ids[e] >= 0) atomicMax(&words[bias_ids[e]], (uint32_t)(p.n_bias - e) << 20);
+    __syncthreads();
+    // an entry that is not its token's first leaves a mark at the one that is
+    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
+      const uint32_t entry = (uint32_t)bias_ids[e];  // perhaps marked already
+      if (entry == 0xffffffffu) continue;
+      const int one = p.n_bias - (int)(words[entry & 0x3fffffffu] >> 20);
+      if (one != e) atomicOr(reinterpret_cast<uint32_t*>(&bias_ids[one]), 0x40000000u);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
+      const uint32_t entry = (uint32_t)bias_ids[e];
+      if (entry == 0xffffffffu || !(entry & 0x40000000u)) continue;
+      const int col = (int)(entry & 0x3fffffffu);
+      double sum = 0.0;
+      for (int j = e; j < p.n_bias; ++j)
+        if (((uint32_t)bias_ids[j] & 0xbfffffffu) == (uint32_t)col) sum += (double)p.bias_values[list + j];
+      bias_sums[p.n_bias - 1 - e] = (float)sum;
+    }
+  }
+
+  // ---- history
   if (history) {
-    const int seq = p.row_seq ? p.row_seq[row] : row;
-    int total = 0, prompt = 0;
-    if (seq >= 0 && seq < p.seqs) {
-      total = min(max(p.total_lens[row], 0), p.max_tokens);
-      prompt = p.prompt_lens[row];
-    }
     __syncwarp();
-    cluster_sync_all();  // every CTA's words are zero
+    cluster_arrive();  // this CTA's words are ready
+    cluster_wait();
     const uint32_t base = smem_u32(words);
-    const int first = part * kCluster * p.slice;  // first column of the cluster
-    const int64_t at = (int64_t)seq * p.tokens_stride;
-    for (int i = rank * kThreads + threadIdx.x; i < total; i += kCluster * kThreads) {
-      const int64_t id = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at + i]
-                                    : (int64_t)static_cast<const int32_t*>(p.tokens)[at + i];
-      const int64_t col = id - p.vocab_start;
-      if (col < first || col >= p.vocab) continue;
-      const int off = (int)(col - first), owner = off / p.slice;
-      if (owner >= kCluster) continue;
-      const uint32_t addr = mapa_shared(base + 4u * (uint32_t)(off - owner * p.slice), (uint32_t)owner);
-      if (i < prompt)
-        red_or_cluster(addr, kPromptBit);
-      else
-        red_add_cluster(addr, 1u);
+    for (int i = mine; i < total; i += kAhead * kCluster * kThreads) {
+      if (i != mine) fetch(i);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (ids[k] < 0) continue;
+        const int owner = p.by_slice.div(ids[k]);
+        if (owner >= kCluster) continue;
+        const uint32_t addr = mapa_shared(base + 4u * (uint32_t)(ids[k] - owner * p.slice), (uint32_t)owner);
+        if (i + k * kCluster * kThreads < prompt)
+          red_or_cluster(addr, kPromptBit);
+        else
+          red_add_cluster(addr, 1u);
+      }
     }
     __syncwarp();
-    cluster_sync_all();  // every post has landed
+    cluster_arrive();
+    cluster_wait();  // every post has landed
   } else if (use_words) {
     __syncthreads();
   }
 
-  if (p.n_bias > 0) {
-    const int64_t at = (int64_t)row * p.n_bias;
-    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) bias_ids[e] = p.bias_ids[at + e];
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
-      const int id = bias_ids[e];
-      const int64_t col = (int64_t)id - p.vocab_start - lo;
-      if (id < 0 || col < 0 || col >= n) continue;
-      bool is_first = true;
-      for (int j = 0; j < e && is_first; ++j) is_first = bias_ids[j] != id;
-      if (!is_first) continue;
-      double sum = 0.0;
-      for (int j = e; j < p.n_bias; ++j)
-        if (bias_ids[j] == id) sum += (double)p.bias_values[at + j];
-      bias_sums[e] = (float)sum;
-      words[col] |= (uint32_t)(e + 1) << 20;  // one thread per token
-    }
-    __syncthreads();
-  }
-
-  const T* in = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + lo;
-  float* out = p.out + (int64_t)row * p.vocab + lo;
-  const uint32_t* mask = p.mask ? p.mask + (int64_t)row * p.mask_stride : nullptr;
+  // ---- the slice
   const float ninf = __int_as_float(0xff800000);
   if constexpr (kVector) {
-    for (int i = threadIdx.x * kVec; i < n; i += kThreads * kVec) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int i = (s * kThreads + threadIdx.x) * kVec;
+      if (i >= to) break;
+      const T* e = reinterpret_cast<const T*>(raw[s]);
       float x[kVec];
-      if (i + kVec <= n) {
-        constexpr int kLoads = kVec * sizeof(T) / 16;
-        uint4 raw[kLoads];
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) raw[j] = reinterpret_cast<const uint4*>(in + i)[j];
-        const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = lo_f(e[j]);
-      } else {
-        for (int j = 0; j < kVec; ++j) x[j] = i + j < n ? lo_f(in[i + j]) : 0.f;
-      }
+      for (int j = 0; j < kVec; ++j) x[j] = lo_f(e[j]);
       if (use_words) {
         const uint4 w0 = *reinterpret_cast<const uint4*>(words + i);
         const uint4 w1 = *reinterpret_cast<const uint4*>(words + i + 4);
         const uint32_t w[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        if (((w0.x | w0.y) | (w0.z | w0.w)) | ((w1.x | w1.y) | (w1.z | w1.w))) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = process(x[j], w[j], rp, bias_sums);
+          for (int j = 0; j < kVec; ++j) x[j] = process(x[j], w[j], rp, bias_sums);
+        }
       }
-      if (mask) {
-        const uint32_t bits = mask_bits(mask, p.mask_words, p.vocab_start + lo + i);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = (bits >> j) & 1u ? x[j] : ninf;
-      }
-      if (i + kVec <= n) {
-        reinterpret_cast<float4*>(out + i)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(out + i)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      for (int j = 0; j < kVec; ++j) x[j] = (bits[s] >> j) & 1u ? x[j] : ninf;
+      if (i >= from && i + kVec <= to) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i), "f"(x[0]),
+                     "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                     : "memory");
       } else {
-        for (int j = 0; j < kVec && i + j < n; ++j) out[i + j] = x[j];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (i + j >= from && i + j < to) out[i + j] = x[j];
       }
     }
   } else {
-    // any stride: a step covers kVec * kThreads consecutive tokens, kThreads apart in a thread
-    for (int i0 = threadIdx.x; i0 < n; i0 += kThreads * kVec) {
+    // a step covers kVec * kThreads consecutive tokens, kThreads apart in a thread
+    for (int i0 = threadIdx.x; i0 < to; i0 += kThreads * kVec) {
       float x[kVec];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const int i = i0 + j * kThreads;
-        x[j] = i < n ? lo_f(in[i]) : 0.f;
+        x[j] = i < to ? lo_f(in[i]) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const int i = i0 + j * kThreads;
-        if (i >= n) continue;
+        if (i >= to) continue;
         if (use_words) x[j] = process(x[j], words[i], rp, bias_sums);
-        if (mask && !(mask_bits(mask, p.mask_words, p.vocab_start + lo + i) & 1u)) x[j] = ninf;
+        if (mask && !(mask_bits(mask, p.mask_words, bit0 + i) & 1u)) x[j] = ninf;
         out[i] = x[j];
       }
     }
@@ -237,12 +309,15 @@ int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
   int rc = device_info(&di);
   if (rc) return rc;
   // Enough clusters per row to give every SM work, as long as a CTA keeps a whole step.
-  const int steps = (p.vocab + kCluster * kThreads * kVec - 1) / (kCluster * kThreads * kVec);
-  int need = (p.vocab + kCluster * kMaxSlice - 1) / (kCluster * kMaxSlice);
-  const int fill = (di.sm_count + rows * kCluster - 1) / (rows * kCluster);
+  const int columns = p.vocab + kVec - 1;  // with the shift
+  const int steps = (columns + kCluster * kThreads * kVec - 1) / (kCluster * kThreads * kVec);
+  const int need = (columns + kCluster * kMaxSlice - 1) / (kCluster * kMaxSlice);
+  const int64_t ctas = (int64_t)rows * kCluster;
+  const int fill = (int)((di.sm_count + ctas - 1) / ctas);
   p.clusters = std::max(need, std::min(fill, steps));
-  int slice = (p.vocab + p.clusters * kCluster - 1) / (p.clusters * kCluster);
+  const int slice = (columns + p.clusters * kCluster - 1) / (p.clusters * kCluster);
   p.slice = (slice + kVec - 1) / kVec * kVec;
+  p.by_slice = make_div(p.slice);
   const int64_t grid = (int64_t)rows * p.clusters * kCluster;
   if (grid > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "logits_process: %d rows of %d logits are too many", rows, p.vocab);
@@ -309,8 +384,8 @@ extern "C" int b2_logits_process(const void* logits, int64_t row_stride, int dty
   p.bias_ids = bias_ids, p.bias_values = bias_values, p.n_bias = n_bias;
   p.mask = mask, p.mask_stride = mask_stride, p.mask_words = mask_words;
   p.vocab = vocab, p.vocab_start = vocab_start;
-  const size_t es = dtype == B2_DTYPE_F32 ? 4 : 2;
-  const bool vector = aligned16(logits) && aligned16(out) && row_stride * es % 16 == 0 && vocab % 4 == 0;
+  const bool vector = (reinterpret_cast<uintptr_t>(logits) & 15u) == 0 &&
+                      (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (row_stride - vocab) % kVec == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == B2_DTYPE_F16)
     return vector ? launch_typed<__half, true>(p, rows, s) : launch_typed<__half, false>(p, rows, s);

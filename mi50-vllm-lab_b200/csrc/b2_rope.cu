@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "b2_device.cuh"
 #include "b2_internal.h"
 
@@ -27,6 +29,8 @@ namespace {
 
 constexpr int kMaxDim = 1024;
 constexpr int kRopeThreads = 128;
+constexpr int kFewRows = 148;
+constexpr int kAhead = 3;  // items of a thread whose loads are under way together
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -41,6 +45,7 @@ struct RopeArgs {
   int units;        // work units per head
   int items;        // units of a whole row
   int chunk;        // items per block
+  FastDiv by_units;
   int pos64;
   float scale;
 };
@@ -97,7 +102,7 @@ __device__ __forceinline__ Item<T> locate(const RopeArgs& p, int64_t row, int he
 // two copied elements behind the turned part (any type, stride and even rot).
 template <typename T, bool kInterleaved, bool kCache, bool kVec>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs p) {
-  __shared__ float s_cos[kMaxDim / 2], s_sin[kMaxDim / 2];
+  __shared__ __align__(16) float s_cos[kMaxDim / 2], s_sin[kMaxDim / 2];
   const int64_t row = blockIdx.x;
   const int first = blockIdx.y * p.chunk;
   const int last = min(first + p.chunk, p.items);
@@ -131,43 +136,59 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs p) {
   if constexpr (kVec) {
     const int turned = p.rot / 16, vectors = p.dim / 8;
     bool built = false;
-    for (int base = first; base < last || !built; base += kRopeThreads) {
-      const int i = base + threadIdx.x;
-      const bool act = i < last;
-      const int head = act ? i / p.units : 0, u = act ? i - head * p.units : 0;
-      Item<T> it = locate<T, kCache>(p, row, head, k_at, v_at);
-      const bool turn = it.turn && u < turned;
-      // vector indices of the unit's two vectors
-      const int a = (!kInterleaved && turn) ? u : 2 * u;
-      const int b = (!kInterleaved && turn) ? u + turned : 2 * u + 1;
-      uint4 va = make_uint4(0, 0, 0, 0), vb = va;
-      if (act) {
-        va = *reinterpret_cast<const uint4*>(it.in + 8 * a);
-        if (b < vectors) vb = *reinterpret_cast<const uint4*>(it.in + 8 * b);
+    for (int base = first; base < last || !built; base += kAhead * kRopeThreads) {
+      // all loads of kAhead items before the table and the arithmetic
+      uint4 va[kAhead], vb[kAhead];
+      Item<T> it[kAhead];
+      int unit[kAhead], a[kAhead], b[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = base + k * kRopeThreads + threadIdx.x;
+        const int head = i < last ? p.by_units.div(i) : 0;
+        const int u = i < last ? i - head * p.units : 0;
+        it[k] = locate<T, kCache>(p, row, head, k_at, v_at);
+        if (i >= last) it[k].out = nullptr;
+        it[k].turn = it[k].turn && u < turned;
+        unit[k] = u;
+        a[k] = (!kInterleaved && it[k].turn) ? u : 2 * u;
+        b[k] = (!kInterleaved && it[k].turn) ? u + turned : 2 * u + 1;
+        va[k] = vb[k] = make_uint4(0, 0, 0, 0);
+        if (it[k].out) {
+          va[k] = *reinterpret_cast<const uint4*>(it[k].in + 8 * a[k]);
+          if (b[k] < vectors) vb[k] = *reinterpret_cast<const uint4*>(it[k].in + 8 * b[k]);
+        }
       }
       if (!built) table();
       built = true;
-      if (!act || !it.out) continue;
-      if (turn) {
-        T* ea = reinterpret_cast<T*>(&va);
-        T* eb = reinterpret_cast<T*>(&vb);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float c = s_cos[8 * u + j], s = s_sin[8 * u + j];
-          T& ra = kInterleaved ? (j < 4 ? ea[2 * (j & 3)] : eb[2 * (j & 3)]) : ea[j];
-          T& rb = kInterleaved ? (j < 4 ? ea[2 * (j & 3) + 1] : eb[2 * (j & 3) + 1]) : eb[j];
-          const float x = to_f(ra), y = to_f(rb);
-          ra = from_f<T>(x * c - y * s);
-          rb = from_f<T>(y * c + x * s);
+      for (int k = 0; k < kAhead; ++k) {
+        if (!it[k].out) continue;
+        if (it[k].turn) {
+          T* ea = reinterpret_cast<T*>(&va[k]);
+          T* eb = reinterpret_cast<T*>(&vb[k]);
+          float c[8], s[8];
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            *reinterpret_cast<float4*>(&c[j]) = *reinterpret_cast<const float4*>(&s_cos[8 * unit[k] + j]);
+            *reinterpret_cast<float4*>(&s[j]) = *reinterpret_cast<const float4*>(&s_sin[8 * unit[k] + j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            T& ra = kInterleaved ? (j < 4 ? ea[2 * (j & 3)] : eb[2 * (j & 3)]) : ea[j];
+            T& rb = kInterleaved ? (j < 4 ? ea[2 * (j & 3) + 1] : eb[2 * (j & 3) + 1]) : eb[j];
+            const float x = to_f(ra), y = to_f(rb);
+            ra = from_f<T>(x * c[j] - y * s[j]);
+            rb = from_f<T>(y * c[j] + x * s[j]);
+          }
         }
+        *reinterpret_cast<uint4*>(it[k].out + 8 * a[k]) = va[k];
+        if (b[k] < vectors) *reinterpret_cast<uint4*>(it[k].out + 8 * b[k]) = vb[k];
       }
-      *reinterpret_cast<uint4*>(it.out + 8 * a) = va;
-      if (b < vectors) *reinterpret_cast<uint4*>(it.out + 8 * b) = vb;
     }
   } else {
     table();
     for (int i = first + threadIdx.x; i < last; i += kRopeThreads) {
-      const int head = i / p.units, u = i - head * p.units;
+      const int head = p.by_units.div(i), u = i - head * p.units;
       const Item<T> it = locate<T, kCache>(p, row, head, k_at, v_at);
       if (!it.out) continue;
       const bool turn = it.turn && u < half;
@@ -192,7 +213,9 @@ int launch_typed(RopeArgs& p, int rows, bool vec, cudaStream_t stream) {
   const int heads = p.q_heads + p.kv_heads * (kCache ? 2 : 1);
   p.units = vec ? (p.dim + 15) / 16 : (p.dim + 1) / 2;
   p.items = heads * p.units;
-  p.chunk = p.items;
+  p.by_units = make_div(p.units);
+  // A block per row, or with few rows an item per thread, so that more SMs take part.
+  p.chunk = rows >= kFewRows ? p.items : std::min(p.items, kRopeThreads);
   const dim3 grid((unsigned)rows, (unsigned)((p.items + p.chunk - 1) / p.chunk));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
