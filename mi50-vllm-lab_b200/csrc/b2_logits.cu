@@ -10,24 +10,29 @@
 //   x += sum of the row's biases for v
 //   mask bit of v clear: x = -inf
 //
-// A thread-block cluster of 8 CTAs owns a row (or an equal part of its vocabulary): every CTA
-// keeps one 32-bit word per token of its slice in shared memory. The CTAs read an eighth of the
-// history each and post every token to the word of its owner through distributed shared memory
-// (integer atomics: the order does not matter), so that the history crosses L2 once per cluster
-// however long it is. Then each CTA takes its slice of logits through the words. The logits, the
-// mask and the first tokens of the history are loaded into registers before all this, so that one
-// latency covers them.
+// A CTA owns a slice of a row's vocabulary and keeps one 32-bit word per token of it in shared
+// memory. It reads the row's whole history (from L2, which the CTAs of the row share) and counts the
+// tokens of its slice in its own memory; then the slice of logits, loaded into registers ahead of
+// everything else, goes through the words and the mask to the output. The other splits measured, on
+// 128 rows of 151936 logits with histories of up to 16384 tokens (this one: 56 us): a cluster whose
+// CTAs read a part of the history each and post the counts to one another's memory, 84 us (the posts
+// of a token that a text repeats queue at one CTA); the words applied behind the stream, by a second
+// look at the history 85 us, by a list of the touched columns 64 us; a launch of its own for the
+// touched columns, 65 us and twice the latency for few rows.
 //   word = [31] in the prompt | [30:20] key of the token's first bias entry | [19:0] n
 // The first of the bias entries for a token wins its word by an atomic maximum of keys that fall
-// with the index; its thread adds the others, if there are any, in list order in fp64. The result
-// does not depend on timing.
+// with the index; a warp adds the other entries to it, if there are any, in a fixed order in fp64. The
+// result does not depend on timing.
 //
 // Vectors: with columns counted from the last multiple of 8 elements at or before the row's start
 // (`shift` columns before it), vectors of 8 are aligned in the logits and in the output alike, for
 // any vocabulary size, as long as the rows of both start at the same place modulo 8.
 //
-// Bound: memory (logits once, fp32 out once); for few rows the latency of history -> words ->
-// stream.
+// Bound: memory where histories are short (logits once, fp32 out once): 128 rows of 151936 bf16
+// logits alone take 19.1 us, 6.1 TB/s; with biases and masks 25 us; with histories of 300 tokens as
+// well 32 us. Long histories add the read of 8 bytes per token by each of a row's CTAs out of L2 and
+// the shared-memory atomics: up to 16384 tokens per row 56 us. Few rows are bound by the latency of
+// lengths -> history -> words -> stream: one row 3.3 us, 32 rows of a verify step 13.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,15 +44,18 @@
 namespace b2 {
 namespace {
 
-constexpr int kCluster = 8;
 constexpr int kThreads = 512;
 constexpr int kVec = 8;                                // tokens per thread and step
-constexpr int kSteps = 5;                              // steps of a slice
+// Steps of a slice. Five at two CTAs per SM (64 registers) keep 128 rows' stream at 19.1 us; four at
+// three CTAs spill at 40 registers, 23.7 us. Smaller CTAs read the history more often: 256 threads
+// take 73 us for the long histories, and 2.6 instead of 3.3 us for one row.
+constexpr int kSteps = 5;
 constexpr int kMaxSlice = kThreads * kVec * kSteps;    // words of shared memory per CTA
-constexpr int kAhead = 4;                              // tokens of the history loaded at a time
+constexpr int kAhead = 8;                              // tokens of the history a thread loads at a time
 constexpr int kMaxBias = 2047;                         // 11 bits of the word
 constexpr int kMaxHistory = (1 << 20) - 1;             // 20 bits
 constexpr uint32_t kPromptBit = 0x80000000u;
+constexpr uint32_t kMark = 0x40000000u;
 
 struct LogitArgs {
   const void* logits;
@@ -64,17 +72,9 @@ struct LogitArgs {
   int mask_words;
   int vocab, vocab_start, seqs, max_tokens, n_bias;
   int tokens64;
-  int slice;     // columns per CTA, a multiple of kVec
-  int clusters;  // clusters per row
-  FastDiv by_slice;
+  int slice;   // columns per CTA, a multiple of kVec
+  int slices;  // CTAs per row
 };
-
-__device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void red_add_cluster(uint32_t addr, uint32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
 __device__ __forceinline__ float lo_f(float v) { return v; }
 __device__ __forceinline__ float lo_f(__half v) { return __half2float(v); }
@@ -88,55 +88,73 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, in
   return __funnelshift_r(lo, hi, sh);
 }
 
+// A row's penalties. The division by `rep` is a product with its reciprocal and one correction by
+// the residual (Markstein, IBM J. Res. Dev. 34, 1990), which gives the rounded quotient in a few
+// instructions without a branch: a warp works on 32 tokens of which some are divided and others
+// multiplied. Where the residual is no number (infinite x) the product stands. `plain`: the row's
+// `rep` is too small or too large for that, or 0 or infinite, and the row divides.
 struct RowParams {
-  float rep, freq, pres;
+  float rep, inv, freq, pres;
+  bool plain;
 };
+
+__device__ __forceinline__ RowParams row_params(const LogitArgs& p, int row) {
+  RowParams r = {1.f, 1.f, 0.f, 0.f, false};
+  if (p.repetition) r.rep = p.repetition[row];
+  if (p.frequency) r.freq = p.frequency[row];
+  if (p.presence) r.pres = p.presence[row];
+  return r;  // inv and plain are the caller's, once rep is here
+}
 
 __device__ __forceinline__ float process(float x, uint32_t word, const RowParams& rp,
                                          const float* bias_sums) {
-  if (word != 0) {
-    const uint32_t n = word & (uint32_t)kMaxHistory;
-    const uint32_t bias = (word >> 20) & 2047u;
-    if (n != 0 || (word & kPromptBit)) {
-      x = x > 0.f ? __fdiv_rn(x, rp.rep) : x * rp.rep;
-      if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(rp.freq, (float)n)), rp.pres);
-    }
-    if (bias != 0) x += bias_sums[bias - 1];
-  }
+  const uint32_t n = word & (uint32_t)kMaxHistory, bias = (word >> 20) & 2047u;
+  const float q = __fmul_rn(x, rp.inv), residual = __fmaf_rn(-q, rp.rep, x);
+  float quotient = isfinite(residual) ? __fmaf_rn(residual, rp.inv, q) : q;
+  if (rp.plain) quotient = __fdiv_rn(x, rp.rep);
+  const float y = x > 0.f ? quotient : __fmul_rn(x, rp.rep);
+  x = n != 0 || (word & kPromptBit) ? y : x;
+  const float less = __fsub_rn(__fsub_rn(x, __fmul_rn(rp.freq, (float)n)), rp.pres);
+  x = n != 0 ? less : x;
+  if (bias != 0) x += bias_sums[bias - 1];
   return x;
-}
-
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // kVector: vectors of 8 columns (see above); otherwise element by element, for any strides.
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs p) {
   extern __shared__ __align__(16) uint32_t words[];
-  const int rank = (int)cluster_ctarank();
-  const int cluster = blockIdx.x / kCluster;
-  const int row = cluster / p.clusters, part = cluster - row * p.clusters;
+  const int row = blockIdx.x / p.slices;
   // columns with the shift: the row's are shift .. shift + vocab - 1
   const int shift = kVector ? (int)((int64_t)row * p.vocab & 7) : 0;
-  const int first = part * kCluster * p.slice, lo = first + rank * p.slice;  // of the cluster, the CTA
+  const int lo = (blockIdx.x - row * p.slices) * p.slice;  // the slice's first
   const int from = max(0, shift - lo), to = min(p.slice, p.vocab + shift - lo);  // of the slice
   float* bias_sums = reinterpret_cast<float*>(words + p.slice);
-  int32_t* bias_ids = reinterpret_cast<int32_t*>(bias_sums + p.n_bias);
-  const bool history = p.tokens != nullptr;
-  const bool use_words = history || p.n_bias > 0;
-
-  if (use_words) {
+  uint32_t* bias_cols = reinterpret_cast<uint32_t*>(bias_sums + p.n_bias);  // or ~0
+  const bool history = p.tokens != nullptr, touches = history || p.n_bias > 0;
+  if (touches) {
     for (int i = threadIdx.x * 4; i < p.slice; i += kThreads * 4)
       *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
   }
   grid_dep_wait();
   grid_dep_launch();
 
-  // ---- loads ahead: the slice's logits and mask, the first tokens
+  // ---- loads ahead: lengths, parameters, biases, the slice's logits and mask; then, with the
+  // lengths, the first tokens
+  int seq = row, total = 0, prompt = 0;
+  if (history) {
+    if (p.row_seq) seq = p.row_seq[row];
+    total = p.total_lens[row];
+    prompt = p.prompt_lens[row];
+  }
+  RowParams rp = row_params(p, row);
+  const int64_t list = (int64_t)row * p.n_bias;
+  int bias_id = -1;
+  float bias_value = 0.f;
+  if ((int)threadIdx.x < p.n_bias) {
+    bias_id = p.bias_ids[list + threadIdx.x];
+    bias_value = p.bias_values[list + threadIdx.x];
+  }
   const T* in = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride + lo - shift;
   float* out = p.out + (int64_t)row * p.vocab + lo - shift;
   const uint32_t* mask = p.mask ? p.mask + (int64_t)row * p.mask_stride : nullptr;
@@ -158,97 +176,85 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) raw[s][j] = reinterpret_cast<const uint4*>(e)[j];
       }
-      bits[s] = mask && i < to ? mask_bits(mask, p.mask_words, bit0 + i) : ~0u;
+      bits[s] = !mask || i >= to ? ~0u
+                : (bit0 & 7) == 0 ? reinterpret_cast<const uint8_t*>(mask)[(bit0 + i) >> 3]
+                                  : mask_bits(mask, p.mask_words, bit0 + i);
     }
   }
-  int total = 0, prompt = 0;
-  int64_t at = 0;
-  if (history) {
-    const int seq = p.row_seq ? p.row_seq[row] : row;
-    if (seq >= 0 && seq < p.seqs) {
-      total = min(max(p.total_lens[row], 0), p.max_tokens);
-      prompt = p.prompt_lens[row];
-      at = (int64_t)seq * p.tokens_stride;
-    }
-  }
-  int32_t ids[kAhead];  // columns of the cluster, or -1
+  // Columns of the slice, counted from `from`, of up to kAhead tokens from i0 on; others: ~0.
+  const uint32_t token0 = (uint32_t)(bit0 + from), width = (uint32_t)max(0, to - from);
+  total = seq < 0 || seq >= p.seqs ? 0 : min(max(total, 0), p.max_tokens);
+  const int64_t at = (int64_t)(total ? seq : 0) * p.tokens_stride;
+  uint32_t cols[kAhead];
   auto fetch = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kCluster * kThreads;
+      const int i = i0 + k * kThreads;
       int64_t id = -1;
       if (i < total)
         id = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at + i]
                         : (int64_t)static_cast<const int32_t*>(p.tokens)[at + i];
-      const int64_t col = id - p.vocab_start;
-      ids[k] = col >= 0 && col < p.vocab ? (int32_t)col + shift - first : -1;
+      cols[k] = id >= 0 && id <= 0x7fffffff ? (uint32_t)id - token0 : ~0u;
     }
   };
-  const int mine = rank * kThreads + threadIdx.x;
-  if (history) fetch(mine);
-  RowParams rp = {1.f, 0.f, 0.f};
-  if (p.repetition) rp.rep = p.repetition[row];
-  if (p.frequency) rp.freq = p.frequency[row];
-  if (p.presence) rp.pres = p.presence[row];
+  if (history) fetch(threadIdx.x);
+  rp.inv = __frcp_rn(rp.rep);
+  rp.plain = !(fabsf(rp.rep) > 0x1p-100f && fabsf(rp.rep) < 0x1p100f);
 
   // ---- biases: keys into the words, sums by key
   if (p.n_bias > 0) {
-    const int64_t list = (int64_t)row * p.n_bias;
     for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
-      const int id = p.bias_ids[list + e];
-      const int64_t col = id < 0 ? -1 : (int64_t)id - p.vocab_start + shift - lo;
-      bias_ids[e] = col >= from && col < to ? (int)col : -1;
-      bias_sums[p.n_bias - 1 - e] = p.bias_values[list + e];  // by key - 1
+      if (e >= kThreads) bias_id = p.bias_ids[list + e], bias_value = p.bias_values[list + e];
+      const uint32_t col = (uint32_t)bias_id - token0;
+      bias_cols[e] = bias_id >= 0 && col < width ? (uint32_t)from + col : ~0u;
+      bias_sums[p.n_bias - 1 - e] = bias_value;  // by key - 1
     }
     __syncthreads();  // the words are zero, the list is here
     for (int e = threadIdx.x; e < p.n_bias; e += kThreads)
-      if (bias_ids[e] >= 0) atomicMax(&words[bias_ids[e]], (uint32_t)(p.n_bias - e) << 20);
+      if (bias_cols[e] != ~0u) atomicMax(&words[bias_cols[e]], (uint32_t)(p.n_bias - e) << 20);
     __syncthreads();
     // an entry that is not its token's first leaves a mark at the one that is
     for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
-      const uint32_t entry = (uint32_t)bias_ids[e];  // perhaps marked already
-      if (entry == 0xffffffffu) continue;
-      const int one = p.n_bias - (int)(words[entry & 0x3fffffffu] >> 20);
-      if (one != e) atomicOr(reinterpret_cast<uint32_t*>(&bias_ids[one]), 0x40000000u);
+      const uint32_t col = bias_cols[e];  // perhaps marked already
+      if (col == ~0u) continue;
+      const int one = p.n_bias - (int)(words[col & ~kMark] >> 20);
+      if (one != e) atomicOr(&bias_cols[one], kMark);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < p.n_bias; e += kThreads) {
-      const uint32_t entry = (uint32_t)bias_ids[e];
-      if (entry == 0xffffffffu || !(entry & 0x40000000u)) continue;
-      const int col = (int)(entry & 0x3fffffffu);
-      double sum = 0.0;
-      for (int j = e; j < p.n_bias; ++j)
-        if (((uint32_t)bias_ids[j] & 0xbfffffffu) == (uint32_t)col) sum += (double)p.bias_values[list + j];
-      bias_sums[p.n_bias - 1 - e] = (float)sum;
+    // a warp per marked entry: the lanes' sums are joined in a fixed order
+    const int lane = threadIdx.x & 31;
+    for (int e0 = (int)threadIdx.x - lane; e0 < p.n_bias; e0 += kThreads) {
+      const uint32_t mine = e0 + lane < p.n_bias ? bias_cols[e0 + lane] : ~0u;
+      for (uint32_t left = __ballot_sync(~0u, mine != ~0u && (mine & kMark)); left; left &= left - 1) {
+        const int e = e0 + __ffs(left) - 1;
+        const uint32_t col = bias_cols[e];
+        double sum = 0.0;
+        for (int j = e + lane; j < p.n_bias; j += 32)
+          if ((bias_cols[j] & ~kMark) == (col & ~kMark)) sum += (double)p.bias_values[list + j];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane == 0) bias_sums[p.n_bias - 1 - e] = (float)sum;
+      }
     }
   }
 
   // ---- history
-  if (history) {
-    __syncwarp();
-    cluster_arrive();  // this CTA's words are ready
-    cluster_wait();
-    const uint32_t base = smem_u32(words);
-    for (int i = mine; i < total; i += kAhead * kCluster * kThreads) {
-      if (i != mine) fetch(i);
+  if (touches) __syncthreads();  // the words are zero, or hold the biases' keys
+  for (int i0 = threadIdx.x; i0 < total; i0 += kAhead * kThreads) {
+    uint32_t now[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (ids[k] < 0) continue;
-        const int owner = p.by_slice.div(ids[k]);
-        if (owner >= kCluster) continue;
-        const uint32_t addr = mapa_shared(base + 4u * (uint32_t)(ids[k] - owner * p.slice), (uint32_t)owner);
-        if (i + k * kCluster * kThreads < prompt)
-          red_or_cluster(addr, kPromptBit);
-        else
-          red_add_cluster(addr, 1u);
-      }
+    for (int k = 0; k < kAhead; ++k) now[k] = cols[k];
+    if (i0 + kAhead * kThreads < total) fetch(i0 + kAhead * kThreads);  // behind these counts
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (now[k] >= width) continue;
+      if (i0 + k * kThreads < prompt)
+        atomicOr(&words[from + now[k]], kPromptBit);
+      else
+        atomicAdd(&words[from + now[k]], 1u);
     }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();  // every post has landed
-  } else if (use_words) {
-    __syncthreads();
   }
+  if (touches) __syncthreads();
 
   // ---- the slice
   const float ninf = __int_as_float(0xff800000);
@@ -261,13 +267,16 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
       float x[kVec];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) x[j] = lo_f(e[j]);
-      if (use_words) {
-        const uint4 w0 = *reinterpret_cast<const uint4*>(words + i);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(words + i + 4);
-        const uint32_t w[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-        if (((w0.x | w0.y) | (w0.z | w0.w)) | ((w1.x | w1.y) | (w1.z | w1.w))) {
+      if (touches) {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) x[j] = process(x[j], w[j], rp, bias_sums);
+        for (int h = 0; h < kVec; h += 4) {
+          const uint4 w = *reinterpret_cast<const uint4*>(words + i + h);
+          if ((w.x | w.y) | (w.z | w.w)) {
+            x[h] = w.x ? process(x[h], w.x, rp, bias_sums) : x[h];
+            x[h + 1] = w.y ? process(x[h + 1], w.y, rp, bias_sums) : x[h + 1];
+            x[h + 2] = w.z ? process(x[h + 2], w.z, rp, bias_sums) : x[h + 2];
+            x[h + 3] = w.w ? process(x[h + 3], w.w, rp, bias_sums) : x[h + 3];
+          }
         }
       }
 #pragma unroll
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const LogitArgs p) {
       for (int j = 0; j < kVec; ++j) {
         const int i = i0 + j * kThreads;
         if (i >= to) continue;
-        if (use_words) x[j] = process(x[j], words[i], rp, bias_sums);
+        if (touches && words[i]) x[j] = process(x[j], words[i], rp, bias_sums);
         if (mask && !(mask_bits(mask, p.mask_words, bit0 + i) & 1u)) x[j] = ninf;
         out[i] = x[j];
       }
@@ -308,20 +317,18 @@ int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
   DeviceInfo di;
   int rc = device_info(&di);
   if (rc) return rc;
-  // Enough clusters per row to give every SM work, as long as a CTA keeps a whole step.
+  // Enough slices per row to give every SM work, as long as a CTA keeps a whole step.
   const int columns = p.vocab + kVec - 1;  // with the shift
-  const int steps = (columns + kCluster * kThreads * kVec - 1) / (kCluster * kThreads * kVec);
-  const int need = (columns + kCluster * kMaxSlice - 1) / (kCluster * kMaxSlice);
-  const int64_t ctas = (int64_t)rows * kCluster;
-  const int fill = (int)((di.sm_count + ctas - 1) / ctas);
-  p.clusters = std::max(need, std::min(fill, steps));
-  const int slice = (columns + p.clusters * kCluster - 1) / (p.clusters * kCluster);
+  const int steps = (columns + kThreads * kVec - 1) / (kThreads * kVec);
+  const int need = (columns + kMaxSlice - 1) / kMaxSlice;
+  p.slices = std::max(need, std::min((di.sm_count + rows - 1) / rows, steps));
+  const int slice = (columns + p.slices - 1) / p.slices;
   p.slice = (slice + kVec - 1) / kVec * kVec;
-  p.by_slice = make_div(p.slice);
-  const int64_t grid = (int64_t)rows * p.clusters * kCluster;
+  const int64_t grid = (int64_t)rows * p.slices;
   if (grid > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "logits_process: %d rows of %d logits are too many", rows, p.vocab);
-  const size_t smem = sizeof(uint32_t) * ((size_t)p.slice + 2 * (size_t)p.n_bias);
+  const bool touches = p.tokens || p.n_bias > 0;
+  const size_t smem = touches ? sizeof(uint32_t) * ((size_t)p.slice + 2 * (size_t)p.n_bias) : 0;
   static bool configured[64] = {};
   int dev = 0;
   B2_CUDA_TRY(cudaGetDevice(&dev));
@@ -331,8 +338,7 @@ int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
                                      (int)(sizeof(uint32_t) * (kMaxSlice + 2 * kMaxBias))));
     configured[dev] = true;
   }
-  return launch_kernel_clusters(logits_kernel<T, kVector>, (int)grid, kCluster, kThreads, smem,
-                                stream, /*early=*/true, p);
+  return launch_kernel(logits_kernel<T, kVector>, (int)grid, kThreads, smem, stream, /*early=*/true, p);
 }
 
 }  // namespace

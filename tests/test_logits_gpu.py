@@ -117,6 +117,26 @@ def test_special_values(ops):
     assert bool((out[1] == -float("inf")).all())
 
 
+def test_division_is_rounded_once(ops):
+    """The quotient by the repetition penalty has the bits of an IEEE division, for ordinary
+    penalties (by Markstein's theorem: a rounded reciprocal, one correction) and for those at the
+    ends of fp32, where the kernel divides."""
+    reps = [1.3, 0.77, 1.1, 3.0, 1e-40, 1e-45, 2e-31, 7e-31, 1.2e30, 2e38, 3.4e38, float("inf"), 0.0]
+    vocab = 4096
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn(len(reps), vocab, generator=g) * 10.0 ** torch.randint(-8, 9, (vocab,), generator=g)
+    x[:, :4] = torch.tensor([float("inf"), -float("inf"), 0.0, -0.0])
+    rep = torch.tensor(reps)
+    tokens = torch.arange(vocab, dtype=torch.int32).expand(len(reps), vocab).contiguous()
+    n = torch.full((len(reps),), vocab, dtype=torch.int32)
+    for view in (x, x[:, 1:]):  # vectors, and element by element
+        out = ops.logits_process(view.cuda(), tokens=tokens.cuda(), prompt_lens=n.cuda(),
+                                 total_lens=n.cuda(), repetition=rep.cuda())
+        exact = torch.where(view > 0, view / rep[:, None], view * rep[:, None])
+        assert torch.equal(out.cpu().nan_to_num(7.0), exact.nan_to_num(7.0))
+        assert torch.equal(out.cpu().isnan(), exact.isnan())
+
+
 def test_lengths_outside_the_contract(ops):
     """Lengths are cut at the table; a row_seq outside it means no history; ids that are no token
     of the shard are skipped."""
