@@ -14,7 +14,7 @@
 // memory. It reads the row's whole history (from L2, which the CTAs of the row share) and counts the
 // tokens of its slice in its own memory; then the slice of logits, loaded into registers ahead of
 // everything else, goes through the words and the mask to the output. The other splits measured, on
-// 128 rows of 151936 logits with histories of up to 16384 tokens (this one: 56 us): a cluster whose
+// 128 rows of 151936 logits with histories of up to 16384 tokens (this one: 50 us): a cluster whose
 // CTAs read a part of the history each and post the counts to one another's memory, 84 us (the posts
 // of a token that a text repeats queue at one CTA); the words applied behind the stream, by a second
 // look at the history 85 us, by a list of the touched columns 64 us; a launch of its own for the
@@ -30,9 +30,10 @@
 //
 // Bound: memory where histories are short (logits once, fp32 out once): 128 rows of 151936 bf16
 // logits alone take 19.1 us, 6.1 TB/s; with biases and masks 25 us; with histories of 300 tokens as
-// well 32 us. Long histories add the read of 8 bytes per token by each of a row's CTAs out of L2 and
-// the shared-memory atomics: up to 16384 tokens per row 56 us. Few rows are bound by the latency of
-// lengths -> history -> words -> stream: one row 3.3 us, 32 rows of a verify step 13.3 us.
+// well 31 us. Long histories add their read out of L2 by each of a row's eight CTAs (10300 tokens per
+// row on average: 14 us of instructions and latency; with a load per token 21 us) and the atomics in
+// shared memory (14 us), in all 50 us. Few rows are bound by the latency of lengths -> history ->
+// words -> stream: one row 3.2 us; 8 rows of 151936 logits with 300 biases each 8.4 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -48,7 +49,7 @@ constexpr int kThreads = 512;
 constexpr int kVec = 8;                                // tokens per thread and step
 // Steps of a slice. Five at two CTAs per SM (64 registers) keep 128 rows' stream at 19.1 us; four at
 // three CTAs spill at 40 registers, 23.7 us. Smaller CTAs read the history more often: 256 threads
-// take 73 us for the long histories, and 2.6 instead of 3.3 us for one row.
+// took 73 us for the long histories where 512 took 56, and 2.6 instead of 3.3 us for one row.
 constexpr int kSteps = 5;
 constexpr int kMaxSlice = kThreads * kVec * kSteps;    // words of shared memory per CTA
 constexpr int kAhead = 8;                              // tokens of the history a thread loads at a time
@@ -71,7 +72,7 @@ struct LogitArgs {
   int64_t mask_stride;
   int mask_words;
   int vocab, vocab_start, seqs, max_tokens, n_bias;
-  int tokens64;
+  int tokens64, tokens_by4;
   int slice;   // columns per CTA, a multiple of kVec
   int slices;  // CTAs per row
 };
@@ -181,23 +182,46 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs p) 
                                   : mask_bits(mask, p.mask_words, bit0 + i);
     }
   }
-  // Columns of the slice, counted from `from`, of up to kAhead tokens from i0 on; others: ~0.
+  // The first of the history's tokens in place k of a thread's batch from i0 on, and its column of
+  // the slice, counted from `from` (or a value behind the slice): four neighbours per load where the
+  // rows of int32 tokens are aligned for it.
   const uint32_t token0 = (uint32_t)(bit0 + from), width = (uint32_t)max(0, to - from);
   total = seq < 0 || seq >= p.seqs ? 0 : min(max(total, 0), p.max_tokens);
   const int64_t at = (int64_t)(total ? seq : 0) * p.tokens_stride;
   uint32_t cols[kAhead];
+  auto place = [&](int i0, int k) {
+    return p.tokens_by4 ? i0 + ((k >> 2) * kThreads + (int)threadIdx.x) * 4 + (k & 3)
+                        : i0 + k * kThreads + (int)threadIdx.x;
+  };
   auto fetch = [&](int i0) {
+    if (p.tokens_by4) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kThreads;
-      int64_t id = -1;
-      if (i < total)
-        id = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at + i]
-                        : (int64_t)static_cast<const int32_t*>(p.tokens)[at + i];
-      cols[k] = id >= 0 && id <= 0x7fffffff ? (uint32_t)id - token0 : ~0u;
+      for (int k = 0; k < kAhead; k += 4) {
+        const int i = place(i0, k);
+        uint4 four = make_uint4(~0u, ~0u, ~0u, ~0u);
+        const int32_t* src = static_cast<const int32_t*>(p.tokens) + at + i;
+        if (i + 4 <= total) {
+          four = *reinterpret_cast<const uint4*>(src);
+        } else {
+          if (i < total) four.x = (uint32_t)src[0];
+          if (i + 1 < total) four.y = (uint32_t)src[1];
+          if (i + 2 < total) four.z = (uint32_t)src[2];
+        }
+        cols[k] = four.x, cols[k + 1] = four.y, cols[k + 2] = four.z, cols[k + 3] = four.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = place(i0, k);
+        int64_t id = -1;
+        if (i < total)
+          id = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at + i]
+                          : (int64_t)static_cast<const int32_t*>(p.tokens)[at + i];
+        cols[k] = id >= 0 && id <= 0x7fffffff ? (uint32_t)id : ~0u;
+      }
     }
   };
-  if (history) fetch(threadIdx.x);
+  if (history) fetch(0);
   rp.inv = __frcp_rn(rp.rep);
   rp.plain = !(fabsf(rp.rep) > 0x1p-100f && fabsf(rp.rep) < 0x1p100f);
 
@@ -240,15 +264,15 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs p) 
 
   // ---- history
   if (touches) __syncthreads();  // the words are zero, or hold the biases' keys
-  for (int i0 = threadIdx.x; i0 < total; i0 += kAhead * kThreads) {
+  for (int i0 = 0; i0 < total; i0 += kAhead * kThreads) {
     uint32_t now[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) now[k] = cols[k];
+    for (int k = 0; k < kAhead; ++k) now[k] = cols[k] - token0;  // ids below the slice: huge
     if (i0 + kAhead * kThreads < total) fetch(i0 + kAhead * kThreads);  // behind these counts
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (now[k] >= width) continue;
-      if (i0 + k * kThreads < prompt)
+      if (place(i0, k) < prompt)
         atomicOr(&words[from + now[k]], kPromptBit);
       else
         atomicAdd(&words[from + now[k]], 1u);
@@ -385,6 +409,7 @@ extern "C" int b2_logits_process(const void* logits, int64_t row_stride, int dty
   const bool penalties = repetition || frequency || presence;
   p.tokens = penalties && max_tokens > 0 ? tokens : nullptr;
   p.tokens64 = tokens_64, p.tokens_stride = tokens_stride, p.seqs = n_seqs, p.max_tokens = max_tokens;
+  p.tokens_by4 = !tokens_64 && tokens_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(tokens) & 15u) == 0;
   p.row_seq = row_seq, p.prompt_lens = prompt_lens, p.total_lens = total_lens;
   p.repetition = repetition, p.frequency = frequency, p.presence = presence;
   p.bias_ids = bias_ids, p.bias_values = bias_values, p.n_bias = n_bias;
