@@ -28,6 +28,7 @@ CUDA events and taken as the max over ranks. The line also carries:
     python bench.py --sweep               # every single-GEMM BASELINE config, one JSON line each
     python bench.py --config1             # config 1 alone (fp16 lm_head GEMM, TB/s)
     python bench.py --norm-epilogue       # row-parallel layer + residual add + RMSNorm, fused vs separate
+    python bench.py --verify-step         # the decode-verify step with rotary, attention and logit processors
 """
 
 from __future__ import annotations
@@ -963,6 +964,97 @@ def run_norm_epilogue(args):
 
 
 
+def run_verify_step(args):
+    """The decode-verify step with what runs between its products, on one GPU: per layer rotary
+    positions with the cache write and attention on the paged cache between qkv_proj and o_proj, and
+    the logit processors behind the lm_head, through the library's call sites (vllm_shim). Two
+    mixes of M = 8 rows at 32768 tokens of context (48 query and 8 KV heads of 128, pages of 16):
+    one request that verifies 8 rows, and 8 requests of one row on a shared prefix. Per mix one
+    JSON line: the captured step with and without these operators, and each operator alone (a graph
+    of its launches in the step); every layer has its own weights and cache, far above L2."""
+    import torch
+
+    import __graft_entry__ as entry
+
+    ops = entry.load_package().ops()
+    from mi50_vllm_lab_b200 import vllm_shim as shim
+
+    torch.cuda.set_device(0)
+    c, D, HQ, HK, page, context = CFG4, 128, 48, 8, 16, 32768
+    M, layers = c["M"], c["layers"]
+    model = DecodeModel(ops, 1, 0, None)
+    rotary = shim.RotaryPositions(D, D, 1e6)
+    pages = context // page + 8 * 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    caches = [torch.randn(2, pages, page, HK, D, device="cuda", generator=g, dtype=torch.float16)
+              for _ in range(layers)]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, device="cuda", generator=g).int()
+    tokens = torch.randint(0, c["vocab"], (8, context), generator=g, **i32)
+    rep = torch.full((M,), 1.1, device="cuda")
+    mask = torch.randint(-2**31, 2**31 - 1, (M, -(-c["vocab"] // 32)), generator=g, **i32)
+    peak, peak_src = hbm_peak()
+    for name, requests in (("one request, 8 rows", 1), ("8 requests on a prefix", 8)):
+        own = 256 if requests > 1 else M  # tokens of a request's own
+        common = (context - own) // page * page
+        n = M // requests
+        table = torch.empty(requests, common // page + 16, **i32)
+        table[:, :common // page] = order[:common // page]
+        table[:, common // page:] = order[common // page:common // page + 16 * requests].view(requests, 16)
+        lens = torch.full((requests,), common + own, **i32)
+        starts = torch.arange(0, M + 1, n, **i32)
+        seq = torch.arange(M, device="cuda") // n
+        pos = common + own - n + torch.arange(M, device="cuda") % n
+        slots = table[seq, pos // page].long() * page + pos % page
+        hist = dict(tokens=tokens, row_seq=seq.int(), prompt_lens=torch.full((M,), common, **i32),
+                    total_lens=(pos + 1).int().clamp(max=context), repetition=rep, frequency=rep - 1,
+                    presence=rep - 1, mask=mask)
+        tables = shim.PrefixTables(common, page, table, lens, starts)
+        model.step()  # the GEMMs' workspace exists before the captures
+        qkv0 = model.w4(model.x0, model.layers[0], "qkv")
+
+        def split(qkv):
+            return qkv.split([HQ * D, HK * D, HK * D], 1)
+
+        def rotate(layer, qkv):
+            return rotary.forward_and_cache(pos, *split(qkv), caches[layer][0], caches[layer][1], slots)
+
+        def attend(layer, q):
+            return shim.prefix_attention(q.view(M, HQ, D), caches[layer][0], caches[layer][1], tables,
+                                         D ** -0.5)[0].view(M, HQ * D)
+
+        def whole():
+            h = model.x0
+            for i, L in enumerate(model.layers):
+                h = model.w4(attend(i, rotate(i, model.w4(h, L, "qkv"))), L, "o")
+                model.w4(h, L, "gate_up")
+                h = model.w4(model.a_d, L, "down")
+            return shim.process_logits(ops.gemm(h, model.lm, 0), **hist)
+
+        q0, lm0 = rotate(0, qkv0), ops.gemm(model.x0, model.lm, 0)
+        parts = {"step": (whole, 1), "step_products_only": (model.step, 1),
+                 "rope_cache": (lambda: [rotate(i, qkv0) for i in range(layers)], layers),
+                 "prefix_attn": (lambda: [attend(i, q0) for i in range(layers)], layers),
+                 "logits_process": (lambda: [shim.process_logits(lm0, **hist) for _ in range(8)], 8)}
+        row = {"workload": f"verify step, {name}", "M": M, "layers": layers, "context": context,
+               "unit": "us", "l2": "weights and caches of a step exceed L2 (logits_process: its "
+                                   "inputs stay in L2, as behind the lm_head)"}
+        for part, (fn, count) in parts.items():
+            fn()
+            graph, _ = capture(fn)
+            for _ in range(args.warmup):
+                graph.replay()
+            ms = time_steps(graph.replay, args.steps, 1, torch.cuda.current_stream())
+            row[part] = round(ms * 1e3 / args.steps / count, 2)
+            del graph
+        read = 2 * 2 * (common + requests * own) * HK * D
+        row["prefix_attn_cache_bytes"] = read
+        row["prefix_attn_of_peak"] = round(read / row["prefix_attn"] / 1e3 / peak, 3)
+        row["peak"] = f"{peak} GB/s ({peak_src})"
+        row["status"] = int(ops.workspace_status(False))
+        print(json.dumps(row), flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -983,6 +1075,9 @@ def main():
                     help="under torchrun: phase timeline of the fused GEMM + all-reduce (trace build)")
     ap.add_argument("--norm-epilogue", action="store_true",
                     help="row-parallel W4 layer + residual add + RMSNorm: fused vs separate, 1 GPU")
+    ap.add_argument("--verify-step", action="store_true",
+                    help="the decode-verify step with rotary positions, attention and logit "
+                         "processors, 1 GPU")
     ap.add_argument("--no-cpu", action="store_true", help="skip the CPU baseline leg")
     ap.add_argument("--cpu-seconds", type=float, default=10.0)
     ap.add_argument("--tune", action="append", default=[], metavar="KEY=VALUE",
@@ -1024,6 +1119,8 @@ def main():
         run_config1(args)
     elif args.norm_epilogue:
         run_norm_epilogue(args)
+    elif args.verify_step:
+        run_verify_step(args)
     else:
         run_gpu(args)
 

@@ -10,6 +10,12 @@ handled, use the stock path") so the patches can point at the B200 library uncha
 * :func:`skinny8`              - ``_gfx906_skinny8`` (patches/vllm/utils.patch:25-46)
 * :class:`NvlinkAllReduce`     - ``Gfx906HostAllReduce`` (patches/vllm/gfx906_host_allreduce.py)
 
+and, for what a verify step runs between these products (the reference leaves it to stock vLLM):
+
+* :class:`RotaryPositions`     - ``RotaryEmbedding.forward``, and the same with the cache write
+* :class:`PrefixTables`, :func:`prefix_attention` - cascade attention over a common prefix
+* :func:`process_logits`       - penalties, biases and grammar masks before the sampler
+
 Predicates are wider than the reference's because the sm_100a kernels are: M = 1 is handled
 (the reference leaves it to Exllama), N needs only % 32 (W4) or nothing (fp16), K needs % 128
 (W4) or % 8 (fp16), and any group size of 32, 64 or a multiple of 128 (the reference gates on
@@ -71,6 +77,118 @@ def skinny8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor | None:
     x_view = x.reshape(-1, k).contiguous()
     out = _ops().gemm(x_view, weight, 0)
     return out.reshape(*x.shape[:-1], m)
+
+
+_HALF = (torch.float16, torch.bfloat16)
+_FLOATS = (*_HALF, torch.float32)
+
+
+class RotaryPositions:
+    """Rotary positions of one kind of layer, with the call of vLLM's ``RotaryEmbedding``: query and
+    key [rows, heads * head_size], or [rows, heads, head_size]. ``scaling`` holds keyword arguments
+    of :func:`.positions.inverse_frequencies` (kind, factor, ...). Results are new tensors."""
+
+    def __init__(self, head_size: int, rotary_dim: int, base: float = 10000.0,
+                 is_neox_style: bool = True, device="cuda", ops=None, **scaling):
+        from .positions import inverse_frequencies
+
+        self.head_size, self.rotary_dim = head_size, rotary_dim
+        self.interleaved = not is_neox_style
+        self.inv_freq, self.scale = inverse_frequencies(rotary_dim, base, device=device, **scaling)
+        self.ops = ops or _ops()
+
+    def _heads(self, t: torch.Tensor) -> torch.Tensor | None:
+        if t.dtype not in _FLOATS or t.dim() not in (2, 3) or t.shape[-1] % self.head_size:
+            return None
+        t = t.unflatten(1, (-1, self.head_size)) if t.dim() == 2 else t
+        return t if t.shape[-1] == self.head_size and t.stride(-1) == 1 else None
+
+    def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor):
+        """(query, key) turned, in the inputs' shapes, or None."""
+        q, k = self._heads(query), self._heads(key)
+        if q is None or k is None or q.dtype != k.dtype or positions.dim() != 1:
+            return None
+        q, k = self.ops.rope(q, k, positions, self.inv_freq, self.scale, self.interleaved)
+        return q.view(query.shape), k.view(key.shape)
+
+    def forward_and_cache(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
+                          value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          slot_mapping: torch.Tensor) -> torch.Tensor | None:
+        """The turned query; the turned key and the value go to ``slot_mapping`` of the caches
+        [blocks, block_size, kv_heads, head_size] (vLLM's reshape_and_cache, in the same launch;
+        -1 writes nothing). None, with the caches untouched, when the shapes are not handled."""
+        q, k, v = self._heads(query), self._heads(key), self._heads(value)
+        if q is None or k is None or v is None or positions.dim() != 1:
+            return None
+        if any(t.dtype != q.dtype for t in (k, v, key_cache, value_cache)):  # e.g. an fp8 cache
+            return None
+        return self.ops.rope_cache(q, k, v, positions, self.inv_freq, slot_mapping, key_cache,
+                                   value_cache, self.scale, self.interleaved).view(query.shape)
+
+
+class PrefixTables:
+    """What attention reads of a step's metadata, formed once per step and used by every layer:
+    vLLM's ``block_table`` [requests, blocks], ``seq_lens`` (with the step's own rows) and
+    ``query_start_loc`` [requests + 1], int32, of requests whose first ``common_prefix_len`` tokens
+    (whole blocks) are the same. The tables are views of the caller's buffers. Formed inside a
+    capture, a replay follows changed lengths and tables; the common prefix is the captured one."""
+
+    def __init__(self, common_prefix_len: int, block_size: int, block_table: torch.Tensor,
+                 seq_lens: torch.Tensor, query_start_loc: torch.Tensor):
+        if common_prefix_len < 0 or common_prefix_len % block_size:
+            raise ValueError(f"a common prefix of {common_prefix_len} tokens in blocks of {block_size}")
+        shared = common_prefix_len // block_size
+        if shared > block_table.shape[1] or (shared and not block_table.shape[0]):
+            raise ValueError(f"{shared} shared blocks in a table of {tuple(block_table.shape)}")
+        table = block_table[0, :shared] if shared else block_table.new_empty(0)
+        self.prefix_pages = table
+        self.prefix_len = torch.full((1,), common_prefix_len, dtype=torch.int32,
+                                     device=seq_lens.device)
+        self.pages = block_table[:, shared:]
+        self.own_lens = seq_lens - common_prefix_len
+        self.row_start = query_start_loc
+
+
+def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     tables: PrefixTables, scale: float, tree: torch.Tensor | None = None,
+                     ops=None) -> tuple[torch.Tensor, torch.Tensor] | None:
+    """Causal attention of query [rows, heads, head_size] over the common prefix and each request's
+    own blocks: (output, log-sum-exp [rows, heads] in fp32), or None when the kernel does not take
+    the shapes. ``tree`` (int64 [rows]) replaces the causal order among a request's new rows: bit m
+    lets a row see the m-th of them."""
+    rows, heads, dim = query.shape
+    kv_heads = key_cache.shape[2]
+
+    def loadable(cache):  # 16-byte loads
+        return (cache.dtype == query.dtype and cache.stride(3) == 1 and cache.data_ptr() % 16 == 0
+                and all(s % 8 == 0 for s in cache.stride()[:3]))
+
+    if not (query.dtype in _HALF and loadable(key_cache) and loadable(value_cache)
+            and query.stride(2) == 1 and query.stride(0) % 2 == 0 and query.stride(1) % 2 == 0
+            and query.data_ptr() % 4 == 0 and dim % 8 == 0 and dim <= 256 and heads <= 1024
+            and heads % kv_heads == 0 and rows <= 4096 and tables.pages.shape[0] <= 1024):
+        return None
+    return (ops or _ops()).prefix_attn(query, key_cache, value_cache, tables.prefix_pages,
+                                       tables.prefix_len, tables.pages, tables.own_lens,
+                                       tables.row_start, scale, tree)
+
+
+def process_logits(logits: torch.Tensor, tokens=None, row_seq=None, prompt_lens=None,
+                   total_lens=None, repetition=None, frequency=None, presence=None, bias_ids=None,
+                   bias_values=None, mask=None, vocab_start: int = 0, ops=None):
+    """fp32 logits [rows, vocab] behind vLLM's penalties (repetition, then frequency and presence),
+    logit biases and grammar bitmask, in one pass, or None. ``tokens`` holds the requests' prompts
+    and outputs, ``row_seq`` each row's request; ``vocab_start`` is a tensor-parallel shard's
+    first token."""
+    if logits.dtype not in _FLOATS or logits.dim() != 2 or logits.stride(1) != 1:
+        return None
+    if tokens is not None and tokens.shape[1] >= 1 << 20:
+        return None
+    if bias_ids is not None and bias_ids.shape[1] > 2047:
+        return None
+    return (ops or _ops()).logits_process(logits, tokens, row_seq, prompt_lens, total_lens,
+                                          repetition, frequency, presence, bias_ids, bias_values,
+                                          mask, vocab_start)
 
 
 class NvlinkAllReduce:

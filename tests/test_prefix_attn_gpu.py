@@ -319,3 +319,47 @@ def test_refusals(ops):
         wide = torch.zeros(*odd[name].shape[:3], 65, dtype=F16, device="cuda")
         with pytest.raises(RuntimeError):
             ops.prefix_attn(**{**odd, name: wide[..., :64]})
+
+
+@pytest.mark.parametrize("rows_of,prefix,own,hq,hk,dim,page,tree", [
+    ([150], 500, [300], 1, 1, 128, 16, False),        # 150 rows per KV head
+    ([40, 30], 700, [64, 200], 8, 2, 128, 16, True),  # 280: three blocks of rows
+    ([64, 64, 60], 200, [64, 90, 60], 2, 1, 64, 32, False),
+    ([9, 64], 33, [130, 64], 8, 1, 256, 8, True),     # 584 of dimension 256
+    ([200], 0, [200], 2, 1, 128, 64, False),
+    ([33] * 9, 1030, [33 + 20 * i for i in range(9)], 4, 4, 64, 24, False),
+])
+def test_many_rows_per_kv_head(ops, rows_of, prefix, own, hq, hk, dim, page, tree):
+    """Several blocks of rows read the same tiles; unseen places hold NaN (see inputs)."""
+    check(ops, inputs(rows_of, prefix, own, hq, hk, dim, BF16, page, 30, tree=tree, pad_rows=3))
+
+
+@pytest.mark.parametrize("n", [300, 1024])
+def test_many_requests(ops, n):
+    """More requests than blocks, of lengths from zero to a few tiles."""
+    own = [(37 * b) % 260 for b in range(n)]
+    check(ops, inputs([1] * n, 96, own, 2, 1, 64, F16, 16, 31))
+
+
+@pytest.mark.parametrize("page", [8, 24, 64, 128, 256])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_pages_and_tiles(ops, dim, page):
+    """Pages that end inside a tile, and tiles inside a page; lengths around both."""
+    own = [1, page - 1, page, page + 1, 63, 64, 65, 127, 128, 129, 3 * page + 5]
+    check(ops, inputs([1] * len(own), page + 3, own, 4, 2, dim, F16, page, 32))
+
+
+def test_infinite_queries_and_keys(ops):
+    """An infinity in one row's query or in a seen key makes that row and head NaN at most: the
+    other rows and heads keep the bits that they have without it."""
+    a = inputs([2, 2], 200, [40, 90], 8, 2, 128, F16, 16, 33)
+    out, lse = ops.prefix_attn(**a)
+    a["q"][1, 3, 5] = INF
+    got, gl = ops.prefix_attn(**a)
+    keep = torch.ones(4, 8, dtype=torch.bool, device="cuda")
+    keep[1, 3] = False
+    assert torch.equal(got[keep], out[keep]) and torch.equal(gl[keep], lse[keep])
+
+
+def test_status_stays_clear(ops):
+    assert ops.workspace_status(False) == 0
