@@ -235,14 +235,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 
 // ------------------------------------------------------------------------------------------------
 // The plan: every block derives it from the lengths on the device. A group is kChains blocks of rows
-// of one head and segment. Costs, in halves of the time a tile takes from memory: 2 for a tile, 4
-// where it is used for two blocks of rows (3000 clocks against 1490 at 64 tokens of 128 dimensions),
-// and 2 more to open a group. With few tiles for each CTA, every tile costs 1: one each is best then.
+// of one head and segment. Costs, in halves of the time a tile takes from memory (1400 clocks at 64
+// tokens of 128 dimensions, 23 bytes a clock for each SM): 2 for a tile, 4 where it is used for two
+// blocks of rows (2350 clocks), and 4 more to open a group: queries in, a chain's first and last tile
+// alone, the mask of the tail, O out, 3000 clocks of which the other chain's work hides some. With 2
+// for that, one request of 8 rows on a prefix of 32768 tokens (48 query and 8 KV heads of 128) took
+// 43.7 us instead of 38.0, the last CTAs having all its own short pieces, and 64 requests on a prefix
+// 103 instead of 100; with 6, requests of 300 own tokens lose 3 %. With few tiles for each CTA, every
+// tile costs 1: one each is best then.
 // ------------------------------------------------------------------------------------------------
 struct Cost {
   int tile, both, open;
   __device__ __forceinline__ explicit Cost(bool even)
-      : tile(even ? 1 : 2), both(even ? 1 : 4), open(even ? 0 : 2) {}
+      : tile(even ? 1 : 2), both(even ? 1 : 4), open(even ? 0 : 4) {}
   // CTAs that share a cost: each range is as long as the longest way from one tile's start to the
   // next one's, so that a tile starts in it. A tile belongs to the CTA in whose range it starts.
   __device__ __forceinline__ int ctas(int cost, int most) const {
@@ -257,7 +262,7 @@ struct Plan {
   int len[kMaxRequests + 1];         // tokens
   int even;
 };
-constexpr int kMaxCost = 6;  // of a tile, with the opening of its group
+constexpr int kMaxCost = 8;  // of a tile, with the opening of its group
 
 template <int kChains>
 __device__ __forceinline__ int groups_of(int count, int group) {
@@ -1295,8 +1300,8 @@ __device__ __forceinline__ void write_lse(const AttnArgs& p, int t, int h, float
   p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
 }
 
-// Few rows, many partials: one block per (row, query head). kThreads / kCols threads take the
-// partials in turn, a thread four dimensions of each; the first loads of O are on their way before
+// Few rows, many partials: one block per (row, query head). kThreads / kCols threads (8, or 16 at
+// dimension 64) take the partials in turn, a thread four dimensions of each; the first loads of O are on their way before
 // the weights are known. Sums run over fixed sets in a fixed order.
 template <typename T, int kCols, int kThreads, int kChains>
 __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int grid) {
@@ -1380,7 +1385,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
 }
 
 // Many rows, few partials each: one warp per (row, query head), 32 partials at a time.
-constexpr int kJoinWarps = 4;
+constexpr int kJoinWarps = 8;
 
 template <typename T, int kCols, int kChains>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const AttnArgs p, int grid) {
@@ -1470,7 +1475,8 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int 
   }
   int rc = launch_kernel(kernel, ctas, S::kThreads, smem, stream, /*early=*/true, mk, mv, p);
   if (rc) return rc;
-  // A warp each where there are many rows with few partials, else a block each. Of a prefix a row has
+  // A warp each where there are many rows with few partials, else a block each: 8192 rows of dimension
+  // 128 with 5 partials take 10 us against 35; 384 rows with 37 partials 16 us against 6. Of a prefix a row has
   // about as many partials as CTAs work on its group.
   const int64_t groups = p.kv_heads * (((int64_t)p.rows * p.group + kChains * kBlockRows - 1) /
                                        (kChains * kBlockRows));
@@ -1478,7 +1484,10 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int 
   if (grid > 3 * ctas && ctas <= 24 * groups)
     return launch_kernel(join_rows_kernel<T, kDim / 4, kChains>, (grid + kJoinWarps - 1) / kJoinWarps,
                          kJoinWarps * 32, 0, stream, /*early=*/true, p, ctas);
-  return launch_kernel(join_kernel<T, kDim / 4, 512, kChains>, grid, 512, 0, stream, /*early=*/true, p,
+  // 8 partials at a time: 384 rows of dimension 128 with 512 threads 1.1 us more, with 128 threads
+  // 1.7 us; 192 rows of dimension 256 with 256 threads 2 us more.
+  constexpr int kJoin = kDim == 256 ? 512 : 256;
+  return launch_kernel(join_kernel<T, kDim / 4, kJoin, kChains>, grid, kJoin, 0, stream, /*early=*/true, p,
                        ctas);
 }
 
