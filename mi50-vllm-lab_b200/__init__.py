@@ -5,9 +5,12 @@ kernels for them behind the reference's operator library ``gfx906_skinny``:
 
 * ``gfx906_skinny.so`` (``torch.ops.gfx906_skinny``): ``gemm``, ``w4gemm``, ``hostar_*`` with the
   reference's schemas, plus ``nvar_*`` (N-rank NVLink all-reduce) and ``w4gemm_ar`` (row-parallel
-  W4 GEMM with the all-reduce fused into its epilogue);
+  W4 GEMM with the all-reduce fused into its epilogue) and, for what a step runs between its
+  products, ``rope``, ``rope_cache``, ``prefix_attn`` and ``logits_process``;
 * ``libb2skinny.so``: the CUDA kernels and their C ABI (``include/b2_skinny.h``);
-* :mod:`.vllm_shim`: the vLLM call sites of the reference (predicates and set-up), ported;
+* :mod:`.vllm_shim`: the vLLM call sites of the reference (predicates and set-up), ported, and those
+  of the operators between the products;
+* :mod:`.positions`: inverse frequencies of rotary positions, scaled for long contexts;
 * :mod:`.capi`: a ctypes binding of the C ABI.
 
 There is no CPU fallback: on a machine without the built libraries or without an sm_100 GPU the
