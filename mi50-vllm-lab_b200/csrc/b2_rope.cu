@@ -15,10 +15,9 @@
 //
 // Bound: memory. A row's heads are read and written once, 16 bytes per access; a thread owns both
 // members of its pairs, so outputs may alias inputs. The table is built behind the loads of the
-// first item (a block holds one row, or part of one when there are few rows). 4099
-// rows of 32 + 8 heads of 128 in bf16: b2_rope 15.8 us, 5.3 TB/s; 2048 such rows: b2_rope_cache
-// 10.3 us, 4.9 TB/s. 8 rows are bound by launch and the latency positions ->
-// table -> stores: 2.0 and 2.3 us.
+// first item (a block holds one row, or part of one when there are few rows). 4099 rows of
+// 32 + 8 heads of 128 in bf16: b2_rope 15.8 us, 5.3 TB/s; 2048 such rows: b2_rope_cache 10.3 us, 4.9
+// TB/s. 8 rows are bound by launch and the latency positions -> table -> stores: 1.7 and 2.1 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,7 +32,11 @@ namespace {
 constexpr int kMaxDim = 1024;
 constexpr int kRopeThreads = 128;
 constexpr int kFewRows = 148;
-constexpr int kAhead = 3;  // items of a thread whose loads are under way together
+// Items of a thread whose loads are under way together, with many rows; with few, a thread has one.
+// With one, 2048 rows with the cache write take 11.3 us instead of 10.3; with four 11.9, and 4099 rows
+// 16.9 instead of 15.8. Blocks of 64 threads: 9.4 and 16.5; of 256: 13.8 and 19.9. Where a thread has
+// one, room for three costs 8 rows 2.0 us instead of 1.7.
+constexpr int kManyAhead = 3;
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -101,9 +104,9 @@ __device__ __forceinline__ Item<T> locate(const RopeArgs& p, int64_t row, int he
   return it;
 }
 
-// kVec: units of two 8-element vectors (16-bit types, aligned); otherwise units of one pair, or of
+// kAhead > 0: units of two 8-element vectors (16-bit types, aligned); otherwise units of one pair, or of
 // two copied elements behind the turned part (any type, stride and even rot).
-template <typename T, bool kInterleaved, bool kCache, bool kVec>
+template <typename T, bool kInterleaved, bool kCache, int kAhead>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs p) {
   __shared__ __align__(16) float s_cos[kMaxDim / 2], s_sin[kMaxDim / 2];
   const int64_t row = blockIdx.x;
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs p) {
     __syncthreads();
   };
 
-  if constexpr (kVec) {
+  if constexpr (kAhead > 0) {
     const int turned = p.rot / 16, vectors = p.dim / 8;
     bool built = false;
     for (int base = first; base < last || !built; base += kAhead * kRopeThreads) {
@@ -231,11 +234,14 @@ int launch_typed(RopeArgs& p, int rows, bool vec, cudaStream_t stream) {
   cfg.numAttrs = tuning(B2_TUNE_NO_PDL) == 0 ? 1 : 0;
   if constexpr (sizeof(T) == 2) {
     if (vec) {
-      B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kernel<T, kInterleaved, kCache, true>, p));
+      if (p.chunk <= kRopeThreads)
+        B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kernel<T, kInterleaved, kCache, 1>, p));
+      else
+        B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kernel<T, kInterleaved, kCache, kManyAhead>, p));
       return B2_OK;
     }
   }
-  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kernel<T, kInterleaved, kCache, false>, p));
+  B2_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kernel<T, kInterleaved, kCache, 0>, p));
   return B2_OK;
 }
 
