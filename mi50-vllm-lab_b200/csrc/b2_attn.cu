@@ -351,10 +351,15 @@ __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const
   p.row_plan[t] = r;
 }
 
+// Below this, costs times kMaxCtas fit 31 bits: divisions of 64 bits take four times as long, which
+// shows in calls of a few microseconds.
+constexpr int kShortCost = 0x7fffffff / kMaxCtas;
 __device__ __forceinline__ int plan_begin(int cost, int ctas, int c) {
+  if (cost < kShortCost) return (int)((uint32_t)(cost * c) / (uint32_t)ctas);
   return (int)((int64_t)cost * c / ctas);
 }
 __device__ __forceinline__ int plan_owner(int cost, int ctas, int at) {
+  if (cost < kShortCost) return (int)((uint32_t)((at + 1) * ctas - 1) / (uint32_t)cost);
   return (int)((((int64_t)at + 1) * ctas - 1) / cost);
 }
 
