@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "b2_device.cuh"
@@ -566,8 +567,8 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
   {  // page tables and queries into L2 behind the plan
     const int line = 32, step = gridDim.x * blockDim.x * line;
     const int at = (blockIdx.x * blockDim.x + threadIdx.x) * line;
-    for (int i = at; i < p.n_prefix_pages; i += step) prefetch_l2(p.prefix_pages + i);
-    const int64_t all = p.requests > 0 ? (p.requests - 1) * p.pages_stride + p.max_pages : 0;
+    for (int64_t i = at; i < p.n_prefix_pages; i += step) prefetch_l2(p.prefix_pages + i);
+    const int64_t all = p.requests > 0 && p.max_pages > 0 ? (p.requests - 1) * p.pages_stride + p.max_pages : 0;
     for (int64_t i = at; i < all; i += step) prefetch_l2(p.pages + i);
     const int n = p.rows * p.q_heads, first = blockIdx.x * blockDim.x + threadIdx.x;
     for (int i = first; i < n; i += gridDim.x * blockDim.x) {
@@ -1592,8 +1593,8 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   if (total_pages < 0 || page_size < 1 || n_prefix_pages < 0 || max_pages < 0)
     return fail(B2_ERR_INVALID_ARG, "%s: %d pages of %d tokens, tables of %d and %d", op, total_pages,
                 page_size, n_prefix_pages, max_pages);
-  if (!(scale == scale) || scale - scale != 0.f)
-    return fail(B2_ERR_INVALID_ARG, "%s: scale is not finite", op);
+  if (!(std::fabs(scale * kLog2e) <= 3.4e38f))
+    return fail(B2_ERR_INVALID_ARG, "%s: scale=%g is not finite", op, (double)scale);
   if (rows == 0) return B2_OK;
   if (!q_strides || !k_strides || !v_strides || !q || !k_cache || !v_cache || !prefix_len ||
       (requests > 0 && !own_lens) || !row_start || !out || !lse || (n_prefix_pages > 0 && !prefix_pages) ||

@@ -363,3 +363,42 @@ def test_infinite_queries_and_keys(ops):
 
 def test_status_stays_clear(ops):
     assert ops.workspace_status(False) == 0
+
+
+@pytest.mark.parametrize("requests", [1, 3, 200])
+def test_tables_without_pages(ops, requests):
+    """Requests whose tables have no columns see the prefix alone; without a prefix, nothing."""
+    a = inputs([2] * requests, 150, [0] * requests, 8, 2, 128, F16, 16, 34)
+    a["pages"] = torch.empty(requests, 0, dtype=torch.int32, device="cuda")
+    a["own_lens"].fill_(9)  # cut at what the tables can hold
+    check(ops, a)
+    a["prefix_pages"] = a["prefix_pages"][:0]
+    out, lse = check(ops, a)
+    assert bool((out == 0).all()) and bool((lse == -INF).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_scales(ops, dim, scale):
+    a = inputs([3, 1], 140, [70, 5], 4, 2, dim, BF16, 16, 35)
+    a["scale"] = scale
+    check(ops, a)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_rows_and_unseen_values(ops, tree):
+    """Two blocks of rows on shared tiles: infinities and NaN in the values of new tokens reach the
+    rows that see them, and only those."""
+    a = inputs([60, 50], 100, [64, 200], 4, 1, 128, F16, 16, 36, tree=tree)
+    base, _ = ops.prefix_attn(**a)
+    n, m = 60, 64
+    slot = int(a["pages"][0, (m - n + 30) // 16]), (m - n + 30) % 16  # the 30th new token's place
+    a["v_cache"][slot[0], slot[1], 0, 7] = float("nan")
+    a["v_cache"][slot[0], slot[1], 0, 8] = INF
+    out, _ = ops.prefix_attn(**a)
+    sees = torch.tensor([(int(a["tree"][r]) >> 30) & 1 == 1 if tree else r >= 30 for r in range(60)]
+                        + [False] * 50).cuda()
+    assert torch.equal(out[~sees], base[~sees])
+    assert bool(out[sees][:, :, 7].isnan().all()) and bool((out[sees][:, :, 8] == INF).all())
+    rest = [d for d in range(128) if d not in (7, 8)]
+    assert torch.equal(out[:, :, rest], base[:, :, rest])

@@ -106,7 +106,7 @@ def attn_call(capi, **kw):
 @pytest.mark.parametrize("kw", [
     dict(requests=-1), dict(requests=1025), dict(rows=-1), dict(rows=4097), dict(hq=7), dict(hk=0),
     dict(hq=2048), dict(dim=0), dict(dim=12), dict(dim=264), dict(dtype=1), dict(total=-1),
-    dict(page=0), dict(np=-1), dict(max_pages=-1), dict(scale=math.inf), dict(scale=math.nan),
+    dict(page=0), dict(np=-1), dict(max_pages=-1), dict(scale=math.inf), dict(scale=math.nan), dict(scale=-3e38),
     dict(q=None), dict(k=None), dict(v=None), dict(pp=None), dict(pl=None), dict(pages=None),
     dict(own=None), dict(starts=None), dict(out=None), dict(lse=None), dict(qs=None), dict(ks=None),
     dict(vs=None), dict(k=_AT + 2), dict(v=_AT + 8), dict(q=_AT + 2),
