@@ -14,7 +14,7 @@
 // memory. It reads the row's whole history (from L2, which the CTAs of the row share) and counts the
 // tokens of its slice in its own memory; then the slice of logits, loaded into registers ahead of
 // everything else, goes through the words and the mask to the output. The other splits measured, on
-// 128 rows of 151936 logits with histories of up to 16384 tokens (this one: 50 us): a cluster whose
+// 128 rows of 151936 logits with histories of up to 16384 tokens (this one then: 57 us, now 44): a cluster whose
 // CTAs read a part of the history each and post the counts to one another's memory, 84 us (the posts
 // of a token that a text repeats queue at one CTA); the words applied behind the stream, by a second
 // look at the history 85 us, by a list of the touched columns 64 us; a launch of its own for the
@@ -30,10 +30,11 @@
 //
 // Bound: memory where histories are short (logits once, fp32 out once): 128 rows of 151936 fp16
 // logits alone take 19.1 us, 6.1 TB/s; with biases and masks 25 us; with histories of 300 tokens as
-// well 31 us. Long histories add their read out of L2 by each of a row's eight CTAs (10300 tokens per
-// row on average: 14 us of instructions and latency; with a load per token 21 us) and the atomics in
-// shared memory (14 us), in all 50 us. Few rows are bound by the latency of lengths -> history ->
-// words -> stream: one row 3.2 us; 8 rows of 151936 logits with 300 biases each 8.4 us.
+// well 30 us. Long histories add their read out of L2 by each of a row's eight CTAs (10300 tokens per
+// row on average: 13 us of instructions and latency; with a load per token 21 us), the atomics in
+// shared memory and the touched tokens' arithmetic, in all 44 us (49 with all eight tokens of a vector
+// going through it where one is touched). Few rows are bound by the latency of lengths -> history ->
+// words -> stream: one row 3.2 us; 8 rows of 151936 logits with 300 biases each 8.0 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -119,6 +120,18 @@ __device__ __forceinline__ float process(float x, uint32_t word, const RowParams
   x = n != 0 ? less : x;
   if (bias != 0) x += bias_sums[bias - 1];
   return x;
+}
+
+// Element j of a vector in registers.
+template <typename T>
+__device__ __forceinline__ float element(const uint4 (&v)[kVec * sizeof(T) / 16], int j) {
+  auto pick = [](const uint4& w, int k) { return k & 2 ? (k & 1 ? w.w : w.z) : (k & 1 ? w.y : w.x); };
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t half = (uint16_t)(pick(v[0], j >> 1) >> (j & 1) * 16);
+    return lo_f(*reinterpret_cast<const T*>(&half));
+  } else {
+    return __uint_as_float(j & 4 ? pick(v[1], j & 3) : pick(v[0], j & 3));
+  }
 }
 
 // kVector: vectors of 8 columns (see above); otherwise element by element, for any strides.
@@ -292,14 +305,26 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs p) 
 #pragma unroll
       for (int j = 0; j < kVec; ++j) x[j] = lo_f(e[j]);
       if (touches) {
+        // A touched token's result takes the place of its word. A thread has few of them: one at a
+        // time, all threads of a warp together.
+        uint32_t touched = 0;
 #pragma unroll
         for (int h = 0; h < kVec; h += 4) {
           const uint4 w = *reinterpret_cast<const uint4*>(words + i + h);
-          if ((w.x | w.y) | (w.z | w.w)) {
-            x[h] = w.x ? process(x[h], w.x, rp, bias_sums) : x[h];
-            x[h + 1] = w.y ? process(x[h + 1], w.y, rp, bias_sums) : x[h + 1];
-            x[h + 2] = w.z ? process(x[h + 2], w.z, rp, bias_sums) : x[h + 2];
-            x[h + 3] = w.w ? process(x[h + 3], w.w, rp, bias_sums) : x[h + 3];
+          touched |= (w.x ? 1u << h : 0) | (w.y ? 2u << h : 0) | (w.z ? 4u << h : 0) | (w.w ? 8u << h : 0);
+        }
+        for (uint32_t left = touched; left; left &= left - 1) {
+          const int j = __ffs(left) - 1;
+          words[i + j] = __float_as_uint(process(element<T>(raw[s], j), words[i + j], rp, bias_sums));
+        }
+        if (touched) {
+#pragma unroll
+          for (int h = 0; h < kVec; h += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(words + i + h);
+            x[h] = touched & 1u << h ? y.x : x[h];
+            x[h + 1] = touched & 2u << h ? y.y : x[h + 1];
+            x[h + 2] = touched & 4u << h ? y.z : x[h + 2];
+            x[h + 3] = touched & 8u << h ? y.w : x[h + 3];
           }
         }
       }
