@@ -34,7 +34,7 @@
 // row on average: 13 us of instructions and latency; with a load per token 21 us), the atomics in
 // shared memory and the touched tokens' arithmetic, in all 44 us (49 with all eight tokens of a vector
 // going through it where one is touched). Few rows are bound by the latency of lengths -> history ->
-// words -> stream: one row 3.2 us; 8 rows of 151936 logits with 300 biases each 6.2 us.
+// words -> stream: one row 2.6 us; 8 rows of 151936 logits with 300 biases each 6.2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -46,13 +46,13 @@
 namespace b2 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kMostThreads = 512;
 constexpr int kVec = 8;                                // tokens per thread and step
 // Steps of a slice. Five at two CTAs per SM (64 registers) keep 128 rows' stream at 19.1 us; four at
 // three CTAs spill at 40 registers, 23.7 us. Smaller CTAs read the history more often: 256 threads
-// took 73 us for the long histories where 512 took 56, and 2.6 instead of 3.3 us for one row.
+// took 73 us for the long histories where 512 took 56.
 constexpr int kSteps = 5;
-constexpr int kMaxSlice = kThreads * kVec * kSteps;    // words of shared memory per CTA
+constexpr int kMaxSlice = kMostThreads * kVec * kSteps;    // words of shared memory per CTA
 constexpr int kAhead = 8;                              // tokens of the history a thread loads at a time
 constexpr int kMaxBias = 2047;                         // 11 bits of the word
 constexpr int kMaxHistory = (1 << 20) - 1;             // 20 bits
@@ -135,7 +135,7 @@ __device__ __forceinline__ float element(const uint4 (&v)[kVec * sizeof(T) / 16]
 }
 
 // kVector: vectors of 8 columns (see above); otherwise element by element, for any strides.
-template <typename T, bool kVector, int kCtas>
+template <typename T, bool kVector, int kThreads, int kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs p) {
   extern __shared__ __align__(16) uint32_t words[];
   const int row = blockIdx.x / p.slices;
@@ -361,11 +361,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs
   }
 }
 
-template <typename T, bool kVector, int kCtas>
+template <typename T, bool kVector, int kThreads, int kCtas>
 int launch_sized(const LogitArgs& p, int grid, cudaStream_t stream) {
   const bool touches = p.tokens || p.n_bias > 0;
   const size_t smem = touches ? sizeof(uint32_t) * ((size_t)p.slice + 2 * (size_t)p.n_bias) : 0;
-  auto kernel = logits_kernel<T, kVector, kCtas>;
+  auto kernel = logits_kernel<T, kVector, kThreads, kCtas>;
   static bool configured[64] = {};
   int dev = 0;
   B2_CUDA_TRY(cudaGetDevice(&dev));
@@ -385,17 +385,26 @@ int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
   // Enough slices per row to give every SM a CTA and none two (8 rows of 151936 with 19 slices, 4 more
   // CTAs than SMs: 8.0 us, with 18: 6.6), as long as a CTA keeps a whole step.
   const int columns = p.vocab + kVec - 1;  // with the shift
-  const int steps = (columns + kThreads * kVec - 1) / (kThreads * kVec);
+  auto steps_of = [&](int threads) { return (columns + threads * kVec - 1) / (threads * kVec); };
+  const int each = std::max(di.sm_count / rows, 1);
+  // Half the threads where that puts more SMs to work and a history takes them one batch of loads: a
+  // row of 18992, 10 CTAs instead of 5, 2.6 us instead of 3.1; with histories of 4000 a row of 151936
+  // would take 4.5 us instead of 4.1, of 16384 8.4 instead of 6.4.
+  const bool half = steps_of(kMostThreads) < each &&
+                    (!p.tokens || p.max_tokens <= kAhead * kMostThreads / 2);
+  const int steps = steps_of(half ? kMostThreads / 2 : kMostThreads);
   const int need = (columns + kMaxSlice - 1) / kMaxSlice;
-  p.slices = std::max(need, std::min(std::max(di.sm_count / rows, 1), steps));
+  p.slices = std::max(need, std::min(each, steps));
   const int slice = (columns + p.slices - 1) / p.slices;
   p.slice = (slice + kVec - 1) / kVec * kVec;
   const int64_t grid = (int64_t)rows * p.slices;
   if (grid > 0x7fffffff)
     return fail(B2_ERR_INVALID_ARG, "logits_process: %d rows of %d logits are too many", rows, p.vocab);
   // Where an SM has one CTA it may have all the registers: 8 rows 6.2 us instead of 6.6.
-  if (grid <= di.sm_count) return launch_sized<T, kVector, 1>(p, (int)grid, stream);
-  return launch_sized<T, kVector, 2>(p, (int)grid, stream);
+  if (half && p.slice <= kMaxSlice / 2)
+    return launch_sized<T, kVector, kMostThreads / 2, 1>(p, (int)grid, stream);
+  if (grid <= di.sm_count) return launch_sized<T, kVector, kMostThreads, 1>(p, (int)grid, stream);
+  return launch_sized<T, kVector, kMostThreads, 2>(p, (int)grid, stream);
 }
 
 }  // namespace

@@ -106,6 +106,13 @@ def test_counts_and_repeated_biases(ops):
     assert torch.equal(out, ops.logits_process(**a))
 
 
+@pytest.mark.parametrize("history", [2048, 2049])
+@pytest.mark.parametrize("rows,vocab", [(1, 18992), (1, 151936), (2, 20480), (3, 100003), (14, 151936)])
+def test_few_rows(ops, rows, vocab, history):
+    """Sizes around the choices of threads and blocks for few rows."""
+    check(ops, inputs(rows, vocab, history, F16, 41, biases=20, mask=True))
+
+
 def test_special_values(ops):
     """Infinities and NaN pass through; masked ones become -inf; a row may be masked whole."""
     a = inputs(3, 640, 50, F16, 7, mask=True)
