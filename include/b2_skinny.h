@@ -387,6 +387,18 @@ int b2_logits_process(const void* logits, int64_t row_stride, int dtype, float* 
                       const float* repetition, const float* frequency, const float* presence,
                       const int32_t* bias_ids, const float* bias_values, int n_bias,
                       const uint32_t* mask, int64_t mask_stride, int mask_words, void* stream);
+/* The same with the biases added before the penalties (so that a repetition penalty scales them and
+ * looks at the sign behind them), which is the order of vLLM's sampler:
+ *   biases -> repetition -> frequency and presence -> mask. */
+int b2_logits_process_bias_first(const void* logits, int64_t row_stride, int dtype, float* out,
+                                 int rows, int vocab, int vocab_start, const void* tokens,
+                                 int tokens_64, int64_t tokens_stride, int n_seqs, int max_tokens,
+                                 const int32_t* row_seq, const int32_t* prompt_lens,
+                                 const int32_t* total_lens, const float* repetition,
+                                 const float* frequency, const float* presence,
+                                 const int32_t* bias_ids, const float* bias_values, int n_bias,
+                                 const uint32_t* mask, int64_t mask_stride, int mask_words,
+                                 void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Tuning (process-wide; for measurement sweeps). B2_TUNE="key=value,..." in the environment

@@ -95,6 +95,8 @@ _SIGS = {
                             _vp]),
     "b2_logits_process": (_i, [_vp, _i64, _i, _vp, _i, _i, _i, _vp, _i, _i64, _i, _i, _vp, _vp, _vp,
                                _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
+    "b2_logits_process_bias_first": (_i, [_vp, _i64, _i, _vp, _i, _i, _i, _vp, _i, _i64, _i, _i, _vp,
+                                          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
     "b2_set_tuning": (_i, [_i, _i]),
     "b2_get_tuning": (_i, [_i]),
     "b2_w4_plan": (_i, [_i, _i, _i, _i, _i, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),

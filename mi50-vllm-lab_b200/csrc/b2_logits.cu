@@ -7,7 +7,7 @@
 //   x = float(logit)
 //   seen:   x = x > 0 ? x / repetition : x * repetition
 //   n > 0:  x = x - frequency * n - presence
-//   x += sum of the row's biases for v
+//   x += sum of the row's biases for v       (before the penalties where the caller asks for it)
 //   mask bit of v clear: x = -inf
 //
 // A CTA owns a slice of a row's vocabulary and keeps one 32-bit word per token of it in shared
@@ -108,9 +108,11 @@ __device__ __forceinline__ RowParams row_params(const LogitArgs& p, int row) {
   return r;  // inv and plain are the caller's, once rep is here
 }
 
+template <bool kBiasFirst>
 __device__ __forceinline__ float process(float x, uint32_t word, const RowParams& rp,
                                          const float* bias_sums) {
   const uint32_t n = word & (uint32_t)kMaxHistory, bias = (word >> 20) & 2047u;
+  if (kBiasFirst && bias != 0) x += bias_sums[bias - 1];
   const float q = __fmul_rn(x, rp.inv), residual = __fmaf_rn(-q, rp.rep, x);
   float quotient = isfinite(residual) ? __fmaf_rn(residual, rp.inv, q) : q;
   if (rp.plain) quotient = __fdiv_rn(x, rp.rep);
@@ -118,7 +120,7 @@ __device__ __forceinline__ float process(float x, uint32_t word, const RowParams
   x = n != 0 || (word & kPromptBit) ? y : x;
   const float less = __fsub_rn(__fsub_rn(x, __fmul_rn(rp.freq, (float)n)), rp.pres);
   x = n != 0 ? less : x;
-  if (bias != 0) x += bias_sums[bias - 1];
+  if (!kBiasFirst && bias != 0) x += bias_sums[bias - 1];
   return x;
 }
 
@@ -134,8 +136,10 @@ __device__ __forceinline__ float element(const uint4 (&v)[kVec * sizeof(T) / 16]
   }
 }
 
-// kVector: vectors of 8 columns (see above); otherwise element by element, for any strides.
-template <typename T, bool kVector, int kThreads, int kCtas>
+// kVector: vectors of 8 columns (see above); otherwise element by element, for any strides. kBiasFirst:
+// an instance of its own, since a choice made per touched token took 128 rows with histories and
+// biases from 44.1 us to 45.3.
+template <typename T, bool kVector, bool kBiasFirst, int kThreads, int kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs p) {
   extern __shared__ __align__(16) uint32_t words[];
   const int row = blockIdx.x / p.slices;
@@ -315,7 +319,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs
         }
         for (uint32_t left = touched; left; left &= left - 1) {
           const int j = __ffs(left) - 1;
-          words[i + j] = __float_as_uint(process(element<T>(raw[s], j), words[i + j], rp, bias_sums));
+          words[i + j] =
+              __float_as_uint(process<kBiasFirst>(element<T>(raw[s], j), words[i + j], rp, bias_sums));
         }
         if (touched) {
 #pragma unroll
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs
       for (int j = 0; j < kVec; ++j) {
         const int i = i0 + j * kThreads;
         if (i >= to) continue;
-        if (touches && words[i]) x[j] = process(x[j], words[i], rp, bias_sums);
+        if (touches && words[i]) x[j] = process<kBiasFirst>(x[j], words[i], rp, bias_sums);
         if (mask && !(mask_bits(mask, p.mask_words, bit0 + i) & 1u)) x[j] = ninf;
         out[i] = x[j];
       }
@@ -361,11 +366,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) logits_kernel(const LogitArgs
   }
 }
 
-template <typename T, bool kVector, int kThreads, int kCtas>
+template <typename T, bool kVector, bool kBiasFirst, int kThreads, int kCtas>
 int launch_sized(const LogitArgs& p, int grid, cudaStream_t stream) {
   const bool touches = p.tokens || p.n_bias > 0;
   const size_t smem = touches ? sizeof(uint32_t) * ((size_t)p.slice + 2 * (size_t)p.n_bias) : 0;
-  auto kernel = logits_kernel<T, kVector, kThreads, kCtas>;
+  auto kernel = logits_kernel<T, kVector, kBiasFirst, kThreads, kCtas>;
   static bool configured[64] = {};
   int dev = 0;
   B2_CUDA_TRY(cudaGetDevice(&dev));
@@ -377,7 +382,7 @@ int launch_sized(const LogitArgs& p, int grid, cudaStream_t stream) {
   return launch_kernel(kernel, grid, kThreads, smem, stream, /*early=*/true, p);
 }
 
-template <typename T, bool kVector>
+template <typename T, bool kVector, bool kBiasFirst>
 int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
   DeviceInfo di;
   int rc = device_info(&di);
@@ -402,24 +407,29 @@ int launch_typed(LogitArgs& p, int rows, cudaStream_t stream) {
     return fail(B2_ERR_INVALID_ARG, "logits_process: %d rows of %d logits are too many", rows, p.vocab);
   // Where an SM has one CTA it may have all the registers: 8 rows 6.2 us instead of 6.6.
   if (half && p.slice <= kMaxSlice / 2)
-    return launch_sized<T, kVector, kMostThreads / 2, 1>(p, (int)grid, stream);
-  if (grid <= di.sm_count) return launch_sized<T, kVector, kMostThreads, 1>(p, (int)grid, stream);
-  return launch_sized<T, kVector, kMostThreads, 2>(p, (int)grid, stream);
+    return launch_sized<T, kVector, kBiasFirst, kMostThreads / 2, 1>(p, (int)grid, stream);
+  if (grid <= di.sm_count)
+    return launch_sized<T, kVector, kBiasFirst, kMostThreads, 1>(p, (int)grid, stream);
+  return launch_sized<T, kVector, kBiasFirst, kMostThreads, 2>(p, (int)grid, stream);
 }
 
-}  // namespace
-}  // namespace b2
 
-extern "C" int b2_logits_process(const void* logits, int64_t row_stride, int dtype, float* out,
-                                 int rows, int vocab, int vocab_start, const void* tokens,
-                                 int tokens_64, int64_t tokens_stride, int n_seqs, int max_tokens,
-                                 const int32_t* row_seq, const int32_t* prompt_lens,
-                                 const int32_t* total_lens, const float* repetition,
-                                 const float* frequency, const float* presence,
-                                 const int32_t* bias_ids, const float* bias_values, int n_bias,
-                                 const uint32_t* mask, int64_t mask_stride, int mask_words,
-                                 void* stream) {
-  using namespace b2;
+template <typename T>
+int launch_type(LogitArgs& p, int rows, bool vector, bool bias_first, cudaStream_t stream) {
+  if (bias_first)
+    return vector ? launch_typed<T, true, true>(p, rows, stream)
+                  : launch_typed<T, false, true>(p, rows, stream);
+  return vector ? launch_typed<T, true, false>(p, rows, stream)
+                : launch_typed<T, false, false>(p, rows, stream);
+}
+
+int check_and_launch(const void* logits, int64_t row_stride, int dtype, float* out, int rows, int vocab,
+                     int vocab_start, const void* tokens, int tokens_64, int64_t tokens_stride,
+                     int n_seqs, int max_tokens, const int32_t* row_seq, const int32_t* prompt_lens,
+                     const int32_t* total_lens, const float* repetition, const float* frequency,
+                     const float* presence, const int32_t* bias_ids, const float* bias_values,
+                     int n_bias, const uint32_t* mask, int64_t mask_stride, int mask_words,
+                     bool bias_first, void* stream) {
   const char* op = "logits_process";
   if (rows < 0 || vocab < 1) return fail(B2_ERR_INVALID_ARG, "%s: %d rows of %d logits", op, rows, vocab);
   if (vocab_start < 0 || (int64_t)vocab_start + vocab > 0x7fffffff - 64)
@@ -460,10 +470,40 @@ extern "C" int b2_logits_process(const void* logits, int64_t row_stride, int dty
   const bool vector = (reinterpret_cast<uintptr_t>(logits) & 15u) == 0 &&
                       (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && (row_stride - vocab) % kVec == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == B2_DTYPE_F16)
-    return vector ? launch_typed<__half, true>(p, rows, s) : launch_typed<__half, false>(p, rows, s);
-  if (dtype == B2_DTYPE_BF16)
-    return vector ? launch_typed<__nv_bfloat16, true>(p, rows, s)
-                  : launch_typed<__nv_bfloat16, false>(p, rows, s);
-  return vector ? launch_typed<float, true>(p, rows, s) : launch_typed<float, false>(p, rows, s);
+  // The order matters to a biased token that the penalties touch.
+  const bool first = bias_first && p.tokens && n_bias > 0;
+  if (dtype == B2_DTYPE_F16) return launch_type<__half>(p, rows, vector, first, s);
+  if (dtype == B2_DTYPE_BF16) return launch_type<__nv_bfloat16>(p, rows, vector, first, s);
+  return launch_type<float>(p, rows, vector, first, s);
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" int b2_logits_process(const void* logits, int64_t row_stride, int dtype, float* out,
+                                 int rows, int vocab, int vocab_start, const void* tokens,
+                                 int tokens_64, int64_t tokens_stride, int n_seqs, int max_tokens,
+                                 const int32_t* row_seq, const int32_t* prompt_lens,
+                                 const int32_t* total_lens, const float* repetition,
+                                 const float* frequency, const float* presence,
+                                 const int32_t* bias_ids, const float* bias_values, int n_bias,
+                                 const uint32_t* mask, int64_t mask_stride, int mask_words,
+                                 void* stream) {
+  return b2::check_and_launch(logits, row_stride, dtype, out, rows, vocab, vocab_start, tokens, tokens_64,
+                              tokens_stride, n_seqs, max_tokens, row_seq, prompt_lens, total_lens,
+                              repetition, frequency, presence, bias_ids, bias_values, n_bias, mask,
+                              mask_stride, mask_words, /*bias_first=*/false, stream);
+}
+
+extern "C" int b2_logits_process_bias_first(
+    const void* logits, int64_t row_stride, int dtype, float* out, int rows, int vocab, int vocab_start,
+    const void* tokens, int tokens_64, int64_t tokens_stride, int n_seqs, int max_tokens,
+    const int32_t* row_seq, const int32_t* prompt_lens, const int32_t* total_lens,
+    const float* repetition, const float* frequency, const float* presence, const int32_t* bias_ids,
+    const float* bias_values, int n_bias, const uint32_t* mask, int64_t mask_stride, int mask_words,
+    void* stream) {
+  return b2::check_and_launch(logits, row_stride, dtype, out, rows, vocab, vocab_start, tokens, tokens_64,
+                              tokens_stride, n_seqs, max_tokens, row_seq, prompt_lens, total_lens,
+                              repetition, frequency, presence, bias_ids, bias_values, n_bias, mask,
+                              mask_stride, mask_words, /*bias_first=*/true, stream);
 }

@@ -640,16 +640,17 @@ const T* row_parameter(const std::optional<at::Tensor>& t, const at::Tensor& lik
   return t->data_ptr<T>();
 }
 
-at::Tensor logits_process(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
-                          const std::optional<at::Tensor>& row_seq,
-                          const std::optional<at::Tensor>& prompt_lens,
-                          const std::optional<at::Tensor>& total_lens,
-                          const std::optional<at::Tensor>& repetition,
-                          const std::optional<at::Tensor>& frequency,
-                          const std::optional<at::Tensor>& presence,
-                          const std::optional<at::Tensor>& bias_ids,
-                          const std::optional<at::Tensor>& bias_values,
-                          const std::optional<at::Tensor>& mask, int64_t vocab_start) {
+at::Tensor logits_process_order(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                                const std::optional<at::Tensor>& row_seq,
+                                const std::optional<at::Tensor>& prompt_lens,
+                                const std::optional<at::Tensor>& total_lens,
+                                const std::optional<at::Tensor>& repetition,
+                                const std::optional<at::Tensor>& frequency,
+                                const std::optional<at::Tensor>& presence,
+                                const std::optional<at::Tensor>& bias_ids,
+                                const std::optional<at::Tensor>& bias_values,
+                                const std::optional<at::Tensor>& mask, int64_t vocab_start,
+                                bool bias_first) {
   const char* op = "logits_process";
   TORCH_CHECK(logits.is_cuda(), op, ": logits must be a CUDA tensor");
   const int dt = dtype_code(logits, op, "logits", true);
@@ -716,7 +717,7 @@ at::Tensor logits_process(const at::Tensor& logits, const std::optional<at::Tens
   }
   c10::cuda::CUDAGuard guard(logits.device());
   auto out = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));
-  const int rc = b2_logits_process(
+  const int rc = (bias_first ? b2_logits_process_bias_first : b2_logits_process)(
       logits.data_ptr(), stride_of(logits, 0, vocab), dt, out.data_ptr<float>(), (int)rows, (int)vocab,
       (int)vocab_start, tok, tok64, tok_stride, (int)seqs, (int)most, seq, prompt, total, rep, freq,
       pres, n_bias ? bias_ids->data_ptr<int32_t>() : nullptr,
@@ -726,12 +727,35 @@ at::Tensor logits_process(const at::Tensor& logits, const std::optional<at::Tens
   return out;
 }
 
+at::Tensor logits_process(const at::Tensor& logits, const std::optional<at::Tensor>& tokens,
+                          const std::optional<at::Tensor>& row_seq,
+                          const std::optional<at::Tensor>& prompt_lens,
+                          const std::optional<at::Tensor>& total_lens,
+                          const std::optional<at::Tensor>& repetition,
+                          const std::optional<at::Tensor>& frequency,
+                          const std::optional<at::Tensor>& presence,
+                          const std::optional<at::Tensor>& bias_ids,
+                          const std::optional<at::Tensor>& bias_values,
+                          const std::optional<at::Tensor>& mask, int64_t vocab_start) {
+  return logits_process_order(logits, tokens, row_seq, prompt_lens, total_lens, repetition, frequency,
+                              presence, bias_ids, bias_values, mask, vocab_start, false);
+}
+
 at::Tensor logits_process_meta(const at::Tensor& logits, const std::optional<at::Tensor>&,
                                const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                                const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                                const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                                const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                                const std::optional<at::Tensor>&, int64_t) {
+  return at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
+}
+
+at::Tensor logits_process_order_meta(
+    const at::Tensor& logits, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+    const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+    const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+    const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+    const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, int64_t, bool) {
   return at::empty(logits.sizes(), logits.options().dtype(at::kFloat));
 }
 
@@ -808,6 +832,11 @@ TORCH_LIBRARY(gfx906_skinny, m) {
         "Tensor? prompt_lens=None, Tensor? total_lens=None, Tensor? repetition=None, "
         "Tensor? frequency=None, Tensor? presence=None, Tensor? bias_ids=None, "
         "Tensor? bias_values=None, Tensor? mask=None, int vocab_start=0) -> Tensor");
+  // the same with a choice of the order: biases before the penalties, or (as above) behind them
+  m.def("logits_process.order(Tensor logits, Tensor? tokens, Tensor? row_seq, Tensor? prompt_lens, "
+        "Tensor? total_lens, Tensor? repetition, Tensor? frequency, Tensor? presence, "
+        "Tensor? bias_ids, Tensor? bias_values, Tensor? mask, int vocab_start, bool bias_first) "
+        "-> Tensor");
   m.def("nvar_status(int handle, bool clear=False) -> int");
   m.def("nvar_set_timeout_ms(int handle, int ms) -> ()");
   m.def("workspace_status(bool clear=False) -> int");
@@ -829,6 +858,7 @@ TORCH_LIBRARY_IMPL(gfx906_skinny, CUDA, m) {
   m.impl("rope_cache", &rope_cache);
   m.impl("prefix_attn", &prefix_attn);
   m.impl("logits_process", &logits_process);
+  m.impl("logits_process.order", &logits_process_order);
 }
 
 TORCH_LIBRARY_IMPL(gfx906_skinny, Meta, m) {
@@ -840,6 +870,7 @@ TORCH_LIBRARY_IMPL(gfx906_skinny, Meta, m) {
   m.impl("rope_cache", &rope_cache_meta);
   m.impl("prefix_attn", &prefix_attn_meta);
   m.impl("logits_process", &logits_process_meta);
+  m.impl("logits_process.order", &logits_process_order_meta);
 }
 
 TORCH_LIBRARY_IMPL(gfx906_skinny, CompositeExplicitAutograd, m) {

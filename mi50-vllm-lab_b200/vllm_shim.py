@@ -176,10 +176,10 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
 def process_logits(logits: torch.Tensor, tokens=None, row_seq=None, prompt_lens=None,
                    total_lens=None, repetition=None, frequency=None, presence=None, bias_ids=None,
                    bias_values=None, mask=None, vocab_start: int = 0, ops=None):
-    """fp32 logits [rows, vocab] behind vLLM's penalties (repetition, then frequency and presence),
-    logit biases and grammar bitmask, in one pass, or None. ``tokens`` holds the requests' prompts
-    and outputs, ``row_seq`` each row's request; ``vocab_start`` is a tensor-parallel shard's
-    first token."""
+    """fp32 logits [rows, vocab] behind vLLM's logit biases, penalties (repetition, then frequency and
+    presence) and grammar bitmask, in this order (its sampler's: biases come before the penalties) and
+    in one pass, or None. ``tokens`` holds the requests' prompts and outputs, ``row_seq`` each row's
+    request; ``vocab_start`` is a tensor-parallel shard's first token."""
     if logits.dtype not in _FLOATS or logits.dim() != 2 or logits.stride(1) != 1:
         return None
     if tokens is not None and tokens.shape[1] >= 1 << 20:
@@ -188,7 +188,7 @@ def process_logits(logits: torch.Tensor, tokens=None, row_seq=None, prompt_lens=
         return None
     return (ops or _ops()).logits_process(logits, tokens, row_seq, prompt_lens, total_lens,
                                           repetition, frequency, presence, bias_ids, bias_values,
-                                          mask, vocab_start)
+                                          mask, vocab_start, True)
 
 
 class NvlinkAllReduce:

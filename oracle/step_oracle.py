@@ -141,9 +141,11 @@ def attn_ref(q, k_cache, v_cache, prefix_pages, prefix_len, pages, own_lens, row
 # ------------------------------------------------------------------------------------------------
 def logits_ref(logits, tokens=None, row_seq=None, prompt_lens=None, total_lens=None, repetition=None,
                frequency=None, presence=None, bias_ids=None, bias_values=None, mask=None,
-               vocab_start=0):
+               vocab_start=0, bias_first=False):
     """Processed logits in 64 bits and the bound on a kernel's error: each of the five fp32
-    operations rounds its result once (2^-24 of the running magnitude), and the biases' sum once."""
+    operations rounds its result once (2^-24 of the running magnitude), and the biases' sum once.
+    With `bias_first` the errors of the biased logit go through the repetition penalty, which scales
+    them by max(rep, 1 / rep) at most."""
     dev = lambda t: None if t is None else t.detach().cpu()  # noqa: E731
     x = dev(logits).double()
     rows, v = x.shape
@@ -153,6 +155,16 @@ def logits_ref(logits, tokens=None, row_seq=None, prompt_lens=None, total_lens=N
     for r in range(rows):
         y = x[r].clone()
         mag = torch.zeros(v, dtype=torch.float64)
+
+        def add_biases():
+            for e in range(bias_ids.shape[1]):
+                col = int(bias_ids[r, e]) - vocab_start
+                if int(bias_ids[r, e]) >= 0 and 0 <= col < v:
+                    y[col] += float(bias_values[r, e])
+                    mag[col] += abs(float(bias_values[r, e])) + y[col].abs() + abs(float(x[r, col]))
+
+        if bias_ids is not None and bias_first:
+            add_biases()
         if penalties and tokens is not None:
             seq = r if row_seq is None else int(row_seq[r])
             if 0 <= seq < tokens.shape[0]:
@@ -167,18 +179,16 @@ def logits_ref(logits, tokens=None, row_seq=None, prompt_lens=None, total_lens=N
                 rep = 1.0 if repetition is None else float(repetition[r])
                 fr = 0.0 if frequency is None else float(frequency[r])
                 pr = 0.0 if presence is None else float(presence[r])
+                if rep > 0:  # what was off before the penalty
+                    mag = torch.where(seen, mag * max(rep, 1 / rep), mag)
                 y = torch.where(seen, torch.where(y > 0, y / rep, y * rep), y)
                 mag += torch.where(seen, y.abs(), 0.0)
                 hit = count > 0
                 mag += torch.where(hit, 2 * (fr * count).abs() + y.abs() + abs(pr), 0.0)
                 y = torch.where(hit, y - fr * count - pr, y)
                 mag += torch.where(hit, y.abs(), 0.0)
-        if bias_ids is not None:
-            for e in range(bias_ids.shape[1]):
-                col = int(bias_ids[r, e]) - vocab_start
-                if int(bias_ids[r, e]) >= 0 and 0 <= col < v:
-                    y[col] += float(bias_values[r, e])
-                    mag[col] += abs(float(bias_values[r, e])) + y[col].abs() + abs(float(x[r, col]))
+        if bias_ids is not None and not bias_first:
+            add_biases()
         tol[r] = torch.where(mag.isfinite(), mag, 0.0) * F32 * 2
         if mask is not None:
             ids = torch.arange(v) + vocab_start

@@ -225,3 +225,46 @@ def test_refusals(ops):
     for change in bad:
         with pytest.raises(RuntimeError):
             ops.logits_process(**{**a, **change})
+
+
+ARGS = ("logits", "tokens", "row_seq", "prompt_lens", "total_lens", "repetition", "frequency",
+        "presence", "bias_ids", "bias_values", "mask", "vocab_start")
+
+
+def ordered(ops, a, bias_first=True):
+    """The overload with a choice of the order: every argument in its place."""
+    return ops.logits_process(*(a.get(n) for n in ARGS), bias_first)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab,history,biases,mask", [
+    (1, 7, 5, 2, True), (3, 1000, 300, 40, False), (8, 50257, 700, 17, True), (2, 4100, 4097, 300, True),
+    (5, 333, 64, 64, True),
+])
+def test_biases_before_penalties(ops, rows, vocab, history, biases, mask, dtype):
+    """Biased tokens of the history: the penalties scale and look at the sum. Without a bias, or
+    without penalties, both orders give the same bits."""
+    a = inputs(rows, vocab, history, dtype, 50, biases=biases, mask=mask)
+    a["bias_ids"][:, ::2] = a["tokens"][a["row_seq"].long()].gather(
+        1, torch.randint(0, history, (rows, biases), device="cuda"))[:, ::2]
+    out = ordered(ops, a)
+    ref, tol = so.logits_ref(**a, bias_first=True)
+    assert so.worst(out, ref, tol) <= 1
+    assert torch.equal(ordered(ops, a, False), ops.logits_process(**a))
+    for drop in (("bias_ids", "bias_values"), ("repetition", "frequency", "presence", "tokens")):
+        b = {k: v for k, v in a.items() if k not in drop}
+        assert torch.equal(ordered(ops, b), ops.logits_process(**b))
+
+
+def test_call_site_takes_the_samplers_order(ops):
+    """By hand: logits 2 and -1 with a bias of 5 and a repetition penalty of 1.3, through the call
+    site: 7 / 1.3 and 4 / 1.3."""
+    from mi50_vllm_lab_b200 import vllm_shim
+
+    a = {k: torch.tensor(v, dtype=t, device="cuda") for k, v, t in (
+        ("logits", [[2.0, -1.0, 0.5]], F32), ("tokens", [[0, 1]], torch.int32),
+        ("prompt_lens", [2], torch.int32), ("total_lens", [2], torch.int32), ("repetition", [1.3], F32),
+        ("bias_ids", [[0, 1]], torch.int32), ("bias_values", [[5.0, 5.0]], F32))}
+    out = vllm_shim.process_logits(**a, ops=ops)
+    want = torch.tensor([[7 / 1.3, 4 / 1.3, 0.5]])
+    assert bool(((out.cpu() - want).abs() <= 2.0 ** -21).all())

@@ -200,3 +200,32 @@ def test_oracle_logits_by_hand():
                              mask=torch.tensor([[0b111110 << 10 >> 1 & ~(1 << 14)]]), vocab_start=10)
     assert out[0].tolist() == [1.0, -2.0 - 1.0 - 0.25, 2.0, 1.5 - 0.5 - 0.25, -math.inf]
     assert bool((tol >= 0).all())
+
+
+def test_order_overload(ops):
+    assert str(ops.logits_process.order._schema) == (
+        "gfx906_skinny::logits_process.order(Tensor logits, Tensor? tokens, Tensor? row_seq, "
+        "Tensor? prompt_lens, Tensor? total_lens, Tensor? repetition, Tensor? frequency, "
+        "Tensor? presence, Tensor? bias_ids, Tensor? bias_values, Tensor? mask, int vocab_start, "
+        "bool bias_first) -> Tensor")
+    x = torch.empty(7, 1000, dtype=torch.float16, device="meta")
+    y = ops.logits_process(x, *[None] * 10, 0, True)
+    assert y.shape == (7, 1000) and y.dtype == torch.float32
+
+
+def test_bias_first_refuses_the_same(capi):
+    """One set of checks for both orders of the C ABI."""
+    call = lambda rows, words: capi.lib().b2_logits_process_bias_first(  # noqa: E731
+        _AT, 1000, 0, _AT, rows, 1000, 0, _AT, 0, 100, 4, 100, None, _AT, _AT, _AT, None, None, None,
+        None, 0, _AT, words, words, None)
+    assert call(0, 32) == 0
+    assert call(-1, 32) == capi.B2_ERR_INVALID_ARG and call(4, 31) == capi.B2_ERR_INVALID_ARG
+
+
+def test_oracle_biases_first_by_hand():
+    a = dict(tokens=torch.tensor([[0, 1]]), prompt_lens=torch.tensor([1]), total_lens=torch.tensor([2]),
+             repetition=torch.tensor([2.0]), presence=torch.tensor([0.25]),
+             bias_ids=torch.tensor([[0, 1, 2]]), bias_values=torch.tensor([[5.0, 5.0, 1.0]]))
+    x = torch.tensor([[2.0, -1.0, 0.5]])
+    assert so.logits_ref(x, **a, bias_first=True)[0][0].tolist() == [3.5, 1.75, 1.5]
+    assert so.logits_ref(x, **a)[0][0].tolist() == [6.0, 2.75, 1.5]

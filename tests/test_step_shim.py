@@ -102,3 +102,13 @@ def test_logits(shim):
                                bias_values=torch.zeros(3, 2048), ops=r) is None
     assert shim.process_logits(x, tokens=torch.zeros(1, 1 << 20, dtype=torch.int32), ops=r) is None
     assert len(r.calls) == n
+
+
+def test_logits_in_the_samplers_order(shim):
+    """The call site asks for biases before the penalties, as vLLM's sampler applies them."""
+    r = Recorder()
+    x = torch.randn(3, 100).half()
+    shim.process_logits(x, bias_ids=torch.zeros(3, 2, dtype=torch.int32), bias_values=torch.zeros(3, 2),
+                        ops=r)
+    name, args = r.calls[-1]
+    assert name == "logits_process" and len(args) == 13 and args[12] is True
