@@ -67,6 +67,7 @@ struct AttnArgs {
   int box_rows;  // tokens per TMA box: a power of two that divides the page size
   FastDiv by_page, by_group;
   float scale_log2;
+  uint64_t minus_zero;  // two of them: a * b + -0 is a rounded product that no sum is fused with
 };
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
@@ -1143,7 +1144,11 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
             }
 #pragma unroll
             for (int j = 0; j < 64; j += 2) {
-              const uint64_t e = fma_pair((uint64_t)s[j + 1] << 32 | s[j], mul2, ref2);
+              // The product is rounded, as the maximum was, before the difference: left exact, as by one
+              // fma, it may lie above the rounded maximum by half a step, which is more than 1 from 2^25
+              // on, and weights of large scores have no bound then. 64 requests on a prefix take 99.7 us
+              // instead of 98.4 for it.
+              const uint64_t e = add_pair(fma_pair((uint64_t)s[j + 1] << 32 | s[j], mul2, p.minus_zero), ref2);
               const float x = ex2(__uint_as_float((uint32_t)e)), y = ex2(__uint_as_float((uint32_t)(e >> 32)));
               sum2[(j >> 1) & 1] = add_pair(sum2[(j >> 1) & 1], pair_of(x, y));
               s[j / 2] = Pair<T>::pack(x, y);
@@ -1639,6 +1644,7 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.requests = requests, p.rows = rows, p.q_heads = q_heads, p.kv_heads = kv_heads, p.group = group;
   p.dim = head_dim;
   p.scale_log2 = scale * kLog2e;
+  p.minus_zero = 0x8000000080000000ull;
   p.row_plan = static_cast<RowPlan*>(ws);
   p.part_ml = reinterpret_cast<float2*>(p.row_plan + rows);
   const size_t ml_bytes = ((size_t)rows * sizeof(RowPlan) + (size_t)partials_for(requests, rows, group, kv_heads) * sizeof(float2) + 255) & ~(size_t)255;

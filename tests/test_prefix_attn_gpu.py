@@ -402,3 +402,34 @@ def test_many_rows_and_unseen_values(ops, tree):
     assert bool(out[sees][:, :, 7].isnan().all()) and bool((out[sees][:, :, 8] == INF).all())
     rest = [d for d in range(128) if d not in (7, 8)]
     assert torch.equal(out[:, :, rest], base[:, :, rest])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (256, 16), (128, 5)])
+@pytest.mark.parametrize("scale", [1e4, 1e7, 3e9, -3e9])
+def test_large_scores(ops, scale, dim, page, dtype):
+    """Scores whose neighbours in fp32 are further apart than 1: the largest takes all the weight. The
+    products q k are exact here; their gaps are above the rounding of the scores, so that the output is
+    the value at the largest, rounded as a weight and as an output (half a step each)."""
+    n = 700
+    a = inputs([1], 0, [n], 4, 2, dim, dtype, page, 41)
+    g = torch.Generator().manual_seed(42)
+    a["scale"] = scale
+    a["q"].zero_()
+    a["q"][..., 0] = 1.0
+    pages, tok = a["pages"][0].long(), torch.arange(n, device="cuda")
+    at = pages[tok // page], tok % page
+    order = torch.stack([torch.randperm(n, generator=g) for _ in range(2)], 1)
+    # 256 levels are exact in bf16; the first is held by one token alone
+    level = (order.clamp(max=254) * 8.0 + torch.where(order == n - 1, 8.0, 0.0)) / 256 - 4.0
+    k = torch.zeros(n, 2, dim)
+    k[..., 0] = level * (1.0 if scale > 0 else -1.0)
+    a["k_cache"][at] = k.to(dtype).cuda()
+    assert torch.equal(a["k_cache"][at].float().cpu(), k)
+    out, lse = ops.prefix_attn(**a)
+    best = order.argmax(0)
+    want = a["v_cache"][at][best.cuda(), torch.arange(2, device="cuda")].double().repeat_interleave(2, 0)
+    bound = 2.002 * so.half_step(dtype) * want.abs() + so.smallest(dtype)
+    assert bool(((out[0].double() - want).abs() <= bound).all())
+    top = abs(scale) * level.max().item()
+    assert bool(((lse - top).abs() <= 2.0 ** -21 * abs(top) + 1e-6).all())
