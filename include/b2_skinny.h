@@ -346,7 +346,8 @@ int b2_rope_cache(const void* q, const int64_t* q_strides, const void* k, const 
  * (even); caches [total_pages, page_size, kv_heads, head_dim] with {page, token, head} strides
  * (multiples of 8); out [rows, q_heads, head_dim] and lse (fp32, [rows, q_heads]) contiguous.
  * head_dim a multiple of 8 up to 256, at most 1024 requests and 4096 rows, fp16 or bf16.
- * Scores, statistics and sums are fp32; the weights are rounded to the type for the second product.
+ * Scores, statistics and sums are fp32; the weights are rounded to the type for the second product
+ * (in fp16 those that lie more than 2^25 below the largest of their run of tokens lose bits).
  * ws: b2_prefix_attn_workspace() bytes, 256-byte aligned, no initialisation; calls that overlap on
  * the GPU need one each. Equal calls give equal bits.
  * ---------------------------------------------------------------------------------------- */

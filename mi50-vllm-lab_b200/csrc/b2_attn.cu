@@ -98,6 +98,7 @@ template <>
 struct Pair<__half> {
   static constexpr uint32_t kExp = 0x7c00u;  // exponent bits: all set in infinities and NaN
   static constexpr uint32_t kFormat = 0;     // operand format of the instruction descriptor
+  static constexpr float kTop = 11.f, kGrow = 4.f;  // of the weights, see the main kernel
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -107,6 +108,7 @@ template <>
 struct Pair<__nv_bfloat16> {
   static constexpr uint32_t kExp = 0x7f80u;
   static constexpr uint32_t kFormat = 1;
+  static constexpr float kTop = 0.f, kGrow = 8.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -453,9 +455,17 @@ struct Cursor {
 //   next warp        issues the products, in the order in which their operands become ready
 //   next 2 warps     (kTma) K and V: one TMA box per group of tokens of one page and 64 dimensions
 //   next 4 warps     (otherwise) 16 bytes per cp.async, for any page size and strides
-// O is rescaled only when a row's maximum has grown by more than 2^8 over the one its weights refer
-// to (the weights stay below 2^8, in range of fp16, with the same relative rounding); the sum l and
-// the partial refer to the same maximum, so nothing is approximated.
+// The weights of the second product are rounded to the operands' type, the sum l is of the weights
+// before that: the tensor cores take 16 bits, and the remainders as a second operand would double the
+// product and the stores of P. Their error is that of the output's own rounding.
+// A weight is 2^(s - m_ref), where m_ref is kTop below the row's maximum when it is set. O is rescaled,
+// and m_ref set again, only when the maximum has grown by more than kGrow since: weights stay below
+// 2^(kTop + kGrow), and O, l and the partial refer to the same m_ref, so nothing is approximated.
+// bf16 has the exponents of fp32: 0 and 8. fp16 ends at 2^16 and loses bits from 2^-14 down: with 11
+// and 4 that begins 2^-25 below the largest weight, with 0 and 8 at 2^-14, where thousands of keys
+// behind one that stands 10 to 18 nats above them count for much and were lost. 7 and 8 would lose
+// some of them and save 0.4 us of the 33.6 that 8 rows on 32775 tokens take (24 query and 4 KV heads of
+// 256), which rescale more often; 13 and 2 take 34.7.
 // ------------------------------------------------------------------------------------------------
 template <int kDim, bool kTma>
 struct Shape {
@@ -1110,10 +1120,12 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
           }
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
           if constexpr (kChains > 1 && kTok == 64) give_back();
-          const bool grow = mx > m_ref + 8.f || (m_ref == neg_inf() && mx > neg_inf());
+          const bool grow = mx > m_ref + (Pair<T>::kTop + Pair<T>::kGrow) ||
+                            (m_ref == neg_inf() && mx > neg_inf());
           if (__any_sync(~0u, grow)) {
-            const float f = grow ? ex2(m_ref - mx) : 1.f;
-            if (grow) m_ref = mx;
+            // (rounded up: the largest weight is 2^kTop at most, however large the scores are)
+            const float to = __fadd_ru(mx, -Pair<T>::kTop), f = grow ? ex2(m_ref - to) : 1.f;
+            if (grow) m_ref = to;
             l *= f;
             if (k > 0) {  // O holds the chain's tiles so far
               const int last = task - 1;
@@ -1307,8 +1319,12 @@ __device__ __forceinline__ void write_row(const AttnArgs& p, int t, int h, int c
   T* out = static_cast<T*>(p.out) + ((int64_t)t * p.q_heads + h) * p.dim + col * 4;
   out[0] = T(acc.x * inv), out[1] = T(acc.y * inv), out[2] = T(acc.z * inv), out[3] = T(acc.w * inv);
 }
+template <typename T>
 __device__ __forceinline__ void write_lse(const AttnArgs& p, int t, int h, float top, float sum) {
-  p.lse[(int64_t)t * p.q_heads + h] = sum == 0.f ? neg_inf() : (top + log2f(sum)) * kLn2;
+  // log2(sum) near its smallest, where the maxima were: the scaling is exact
+  constexpr float kScale = Pair<T>::kTop == 0.f ? 1.f : 1.f / (float)(1 << (int)Pair<T>::kTop);
+  p.lse[(int64_t)t * p.q_heads + h] =
+      sum == 0.f ? neg_inf() : ((top + Pair<T>::kTop) + log2f(sum * kScale)) * kLn2;
 }
 
 // Few rows, many partials: one block per (row, query head). kThreads / kCols threads (8, or 16 at
@@ -1392,7 +1408,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs p, int gr
     }
     write_row<T>(p, t, h, col, acc, sum);
   }
-  if (threadIdx.x == 0) write_lse(p, t, h, top, sum);
+  if (threadIdx.x == 0) write_lse<T>(p, t, h, top, sum);
 }
 
 // Many rows, few partials each: one warp per (row, query head), 32 partials at a time.
@@ -1454,7 +1470,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const AttnAr
 #pragma unroll
   for (int c = 0; c < kMine; ++c)
     if ((lane + 32 * c) * 4 < p.dim) write_row<T>(p, t, h, lane + 32 * c, acc[c], sum);
-  if (lane == 0) write_lse(p, t, h, top, sum);
+  if (lane == 0) write_lse<T>(p, t, h, top, sum);
 }
 
 int round_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }

@@ -74,7 +74,9 @@ def attn_ref(q, k_cache, v_cache, prefix_pages, prefix_len, pages, own_lens, row
     """(out, lse) in 64 bits and the bounds on a kernel's error.
 
     With A = sum_j w_j |v_j| (w: the softmax weights), u = half a step of the type:
-      * the weights are rounded to the type for the second product: u A;
+      * the weights are rounded to the type for the second product: u A, and in fp16, of which the
+        kernel lets the largest weight of a run of tokens be 2^11, or a little less where its
+        logarithm was rounded, half a subnormal step each: 2^-25 / 2^10 of it, n times |v|;
       * a score is a sum of dim exact products in fp32, in any order: at most
         e = 2 dim 2^-24 scale sum|q k| + 2^-22 |s| off (the tensor cores may cut where fp32 would
         round: twice the usual bound; the factor scale * log2(e) and the difference to the maximum
@@ -131,7 +133,8 @@ def attn_ref(q, k_cache, v_cache, prefix_pages, prefix_len, pages, own_lens, row
                 a = w @ v[:, h].abs()
                 cnt = k.shape[0]
                 out_tol[row, h * g:(h + 1) * g] = (u + 2 * e[:, None] + 2.0 ** -21 + 2 * cnt * F32) * a \
-                    + u * o.abs() * (1 + 1e-3) + smallest(q.dtype)
+                    + u * o.abs() * (1 + 1e-3) + smallest(q.dtype) \
+                    + (2.0 ** -35 * v[:, h].abs().sum(0) if q.dtype == torch.float16 else 0.0)
                 lse_tol[row, h * g:(h + 1) * g] = e + 2.0 ** -21 + cnt * F32 + 2.0 ** -22 * le.abs()
     return out, lse, out_tol, lse_tol
 

@@ -433,3 +433,25 @@ def test_large_scores(ops, scale, dim, page, dtype):
     assert bool(((out[0].double() - want).abs() <= bound).all())
     top = abs(scale) * level.max().item()
     assert bool(((lse - top).abs() <= 2.0 ** -21 * abs(top) + 1e-6).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (256, 16), (64, 5)])
+@pytest.mark.parametrize("nats", [10.0, 14.0, 17.0, 18.0, 22.0])
+def test_small_weights_beside_a_large_one(ops, nats, dim, page, dtype):
+    """One key far above thousands of others, its value 0: the output is the sum of the small weights.
+    160 heads, so that about a whole head is one piece and all of it refers to that key's maximum."""
+    n, heads = 4097, 160
+    a = inputs([1], 0, [n], heads, heads, dim, dtype, page, 40)
+    a["scale"] = 1.0
+    a["q"].zero_()
+    a["q"][..., 0] = 4.0
+    pages, tok = a["pages"][0].long(), torch.arange(n, device="cuda")
+    at = pages[tok // page], tok % page
+    k = torch.zeros(n, heads, dim, device="cuda")
+    k[0, :, 0] = nats / 4
+    a["k_cache"][at] = k.to(dtype)
+    v = a["v_cache"][at].float().abs() + 0.5
+    v[0] = 0
+    a["v_cache"][at] = v.to(dtype)
+    check(ops, a)
