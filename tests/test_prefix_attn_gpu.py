@@ -455,3 +455,51 @@ def test_small_weights_beside_a_large_one(ops, nats, dim, page, dtype):
     v[0] = 0
     a["v_cache"][at] = v.to(dtype)
     check(ops, a)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (256, 16), (128, 5)])
+def test_infinite_keys(ops, dim, page, dtype):
+    """An infinity in a key that a row sees: a score of -inf takes no weight, and the row is as without
+    the key; a score of +inf leaves no number. Heads and rows that do not see it keep their bits."""
+    a = inputs([3], 100, [90], 8, 2, dim, dtype, page, 43)
+    slot = int(a["pages"][0, 88 // page]), 88 % page  # the second new row's own key
+    a["tree"] = torch.tensor([1, 1, 5], device="cuda")  # nobody sees it
+    without, lse0 = ops.prefix_attn(**a)
+    a["tree"] = torch.tensor([1, 3, 5], device="cuda")  # its own row does
+    seen, lse1 = ops.prefix_attn(**a)
+    a["k_cache"][slot[0], slot[1], 1, 3] = INF  # of the second KV head
+    got, lse = ops.prefix_attn(**a)
+    other = torch.tensor([0, 2], device="cuda")
+    assert torch.equal(got[other], seen[other]) and torch.equal(lse[other], lse1[other])
+    assert torch.equal(got[1, :4], seen[1, :4]) and torch.equal(lse[1, :4], lse1[1, :4])
+    for h in range(4, 8):
+        if a["q"][1, h, 3] < 0:
+            assert torch.equal(got[1, h], without[1, h]) and lse[1, h] == lse0[1, h]
+        else:
+            assert bool(got[1, h].isnan().all()) and not bool(lse[1, h].isfinite())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,prefix,hq,hk,dim,page,tree", [
+    (40, 6000, 32, 8, 128, 16, False),    # 160 rows per KV head on 752 tiles: one group of two blocks
+    (75, 6000, 16, 4, 128, 16, True),     # 300: a second group, of one block
+    (70, 12000, 16, 4, 64, 32, False),    # tiles of 128 tokens
+    (40, 6000, 16, 4, 256, 16, True),     # one chain: groups of 128
+    (40, 6000, 16, 4, 128, 5, False),     # pages that no box fits
+    (6, 24000, 8, 2, 128, 64, False),     # few rows, long pieces
+])
+def test_uneven_costs(ops, rows, prefix, hq, hk, dim, page, tree, dtype):
+    """More than two tiles per block: costs by tile and group, and groups split between blocks in
+    their middle. Ragged requests behind the prefix; equal calls give equal bits."""
+    rows_of, left = [], rows
+    while left:
+        rows_of.append(min(left, 1 + 3 * len(rows_of) % 7))
+        left -= rows_of[-1]
+    own = [n + 131 * i % 400 for i, n in enumerate(rows_of)]
+    tile = 128 if dim <= 64 else 64
+    assert hk * -(-prefix // tile) > 296
+    a = inputs(rows_of, prefix, own, hq, hk, dim, dtype, page, 44, tree=tree)
+    out, lse = check(ops, a)
+    again = ops.prefix_attn(**a)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
