@@ -349,7 +349,9 @@ int b2_rope_cache(const void* q, const int64_t* q_strides, const void* k, const 
  * Scores, statistics and sums are fp32; the weights are rounded to the type for the second product
  * (in fp16 those that lie more than 2^25 below the largest of their run of tokens lose bits).
  * ws: b2_prefix_attn_workspace() bytes, 256-byte aligned, no initialisation; calls that overlap on
- * the GPU need one each. Equal calls give equal bits.
+ * the GPU need one each; with c = 2 up to head_dim 128, else 1, it is about 2c * rows * q_heads
+ * + 160 * min(128c, c * rows * q_heads / kv_heads) rows of head_dim + 2 floats. Equal calls give equal
+ * bits.
  * ---------------------------------------------------------------------------------------- */
 /* A device-side wait that gave up (a fault of the library or the device; outputs of that call are
  * undefined) is recorded per device: 0 or B2_ERR_TIMEOUT, cleared when `clear` is non-zero.

@@ -13,8 +13,10 @@
 // for one group of rows and one KV head over all segments (segment 0 = the prefix, segment b+1 =
 // request b's own tokens), whatever the lengths on the device say, so a captured graph follows
 // growing lengths. A range's piece of one (segment, head, rows) group ends in unnormalised fp32
-// partials (O, m, l) in the workspace, at slot cta + group (no two pieces share one); a second
-// launch joins the partials of each row in a fixed order, so results do not depend on timing.
+// partials (O, m, l) in the workspace; a second launch joins the partials of each row in a fixed order,
+// so results do not depend on timing. The partials of CTA c's piece of group g begin at row
+// (rows of all groups before g) + c * (rows of the largest group): from one piece to the next the
+// group, the CTA or both go up by one, so no two pieces share a row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -40,12 +42,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Where the partials of a row are: written by the main launch, read by the one that joins them.
 struct RowPlan {
   int cost;                                       // of the whole call
-  int prefix_tiles, prefix_first, prefix_count;   // of the prefix
-  int tiles, first, count;                        // of the row's request; tiles = 0: none
-  int cost0, group0;                              // cost and groups before the request's
+  int prefix_tiles, prefix_first, prefix_count, prefix_span;  // of the prefix
+  int tiles, first, count, span;                  // of the row's request; tiles = 0: none
+  int cost0, rows0;                               // cost and rows of partials before the request's
   int owned;                                      // the row belongs to a request
   int even;                                       // every tile costs the same (Cost)
-  int pad;
 };
 
 struct AttnArgs {
@@ -56,13 +57,13 @@ struct AttnArgs {
   const int64_t* tree;
   void* out;
   float* lse;
-  float* part_o;    // [slots][chains][rows per block][dim]
-  float2* part_ml;  // [slots][chains][rows per block]
+  float* part_o;    // [part_rows][dim]
+  float2* part_ml;  // [part_rows]
   RowPlan* row_plan;  // [rows]
   int64_t pages_stride;
   int total_pages, page_size, n_prefix_pages, max_pages;
   int requests, rows, q_heads, kv_heads, group, dim;
-  int slots;
+  int part_rows, piece_rows;  // rows of partials, of the largest piece
   int q_vec;     // queries allow 16-byte loads
   int box_rows;  // tokens per TMA box: a power of two that divides the page size
   FastDiv by_page, by_group;
@@ -260,7 +261,7 @@ struct Cost {
 };
 struct Plan {
   int cost_end[kMaxRequests + 1];    // running sum of costs up to and with segment s
-  int groups_end[kMaxRequests + 1];  // running sum of groups
+  int rows_end[kMaxRequests + 1];    // running sum of rows of partials, one CTA's for each group
   int first[kMaxRequests + 1];       // first row of the segment
   int count[kMaxRequests + 1];       // and how many
   int len[kMaxRequests + 1];         // tokens
@@ -280,6 +281,18 @@ __device__ __forceinline__ int tile_cost(const Cost& cost, int count, int group)
 template <int kChains>
 __device__ __forceinline__ int group_rows(int count, int group, int g) {
   return min(kChains * kBlockRows, count * group - g * kChains * kBlockRows);
+}
+// Rows of partials of a CTA's piece of a group with so many rows: one for each, or one for each and
+// chain where the chains take its tiles in turn; and of one CTA's pieces of all groups of a head.
+template <int kChains>
+__device__ __forceinline__ int piece_rows(int rows) {
+  return kChains > 1 && rows <= kBlockRows ? kChains * rows : rows;
+}
+template <int kChains>
+__device__ __forceinline__ int head_rows(int count, int group) {
+  constexpr int kWhole = kChains * kBlockRows;
+  const int whole = count * group / kWhole * kWhole;
+  return whole + piece_rows<kChains>(count * group - whole);
 }
 
 // Lengths and rows of every segment, cut at the tables and at the rows there are, and the running
@@ -307,23 +320,23 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
     all = __reduce_add_sync(~0u, all);
     const bool even = all <= 2 * (int)gridDim.x;
     const Cost cost(even);
-    int c_base = 0, g_base = 0;
+    int c_base = 0, r_base = 0;
     for (int s0 = 0; s0 <= p.requests; s0 += 32) {
       const int s = s0 + threadIdx.x;
-      int c = 0, g = 0;
-      if (s <= p.requests && plan.len[s] > 0) {
-        g = groups(s);
-        c = g * (cost.open + tiles(s) * tile_cost<kChains>(cost, plan.count[s], p.group));
+      int c = 0, r = 0;
+      if (s <= p.requests && plan.len[s] > 0 && !bad) {
+        c = groups(s) * (cost.open + tiles(s) * tile_cost<kChains>(cost, plan.count[s], p.group));
+        r = p.kv_heads * head_rows<kChains>(plan.count[s], p.group);
       }
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
-        const int cc = __shfl_up_sync(~0u, c, d), gg = __shfl_up_sync(~0u, g, d);
-        if ((int)threadIdx.x >= d) c += cc, g += gg;
+        const int cc = __shfl_up_sync(~0u, c, d), rr = __shfl_up_sync(~0u, r, d);
+        if ((int)threadIdx.x >= d) c += cc, r += rr;
       }
-      c += c_base, g += g_base;
-      if (s <= p.requests) plan.cost_end[s] = c, plan.groups_end[s] = g;
+      c += c_base, r += r_base;
+      if (s <= p.requests) plan.cost_end[s] = c, plan.rows_end[s] = r;
       c_base = __shfl_sync(~0u, c, 31);
-      g_base = __shfl_sync(~0u, g, 31);
+      r_base = __shfl_sync(~0u, r, 31);
     }
     if (threadIdx.x == 0) plan.even = even;
   }
@@ -331,6 +344,7 @@ __device__ __forceinline__ void make_plan(const AttnArgs& p, int tok, Plan& plan
 }
 
 // The plan of row t for the launch that joins its partials.
+template <int kChains>
 __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const Plan& plan, int t) {
   RowPlan r = {};
   r.cost = plan.cost_end[p.requests];
@@ -338,6 +352,7 @@ __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const
   r.prefix_tiles = (plan.len[0] + tok - 1) / tok;
   r.prefix_first = plan.first[0];
   r.prefix_count = plan.count[0];
+  r.prefix_span = head_rows<kChains>(plan.count[0], p.group);
   // the last request that starts at or before t: requests without rows share a start with the next
   int lo = 0, hi = p.requests;
   while (lo < hi) {
@@ -349,8 +364,9 @@ __device__ __forceinline__ void write_row_plan(const AttnArgs& p, int tok, const
     r.tiles = (plan.len[lo] + tok - 1) / tok;
     r.first = plan.first[lo];
     r.count = plan.count[lo];
+    r.span = head_rows<kChains>(plan.count[lo], p.group);
     r.cost0 = plan.cost_end[lo - 1];
-    r.group0 = plan.groups_end[lo - 1];
+    r.rows0 = plan.rows_end[lo - 1];
   }
   p.row_plan[t] = r;
 }
@@ -371,7 +387,7 @@ __device__ __forceinline__ int plan_owner(int cost, int ctas, int at) {
 template <int kChains>
 struct Cursor {
   int seg, head, group, tile, at;  // at: the cost before it
-  int first, count, len, tiles, groups, weight;
+  int first, count, len, tiles, groups, weight, span;  // span: rows of partials of a head
   int open;
   __device__ __forceinline__ void load(const AttnArgs& p, const Plan& plan, int tok) {
     const Cost cost(plan.even);
@@ -379,9 +395,14 @@ struct Cursor {
     tiles = (len + tok - 1) / tok;
     groups = groups_of<kChains>(count, p.group);
     weight = tile_cost<kChains>(cost, count, p.group);
+    span = head_rows<kChains>(count, p.group);
     open = cost.open;
   }
-  __device__ __forceinline__ int index() const { return head * groups + group; }  // in the segment
+  // The first row of partials of this CTA's piece.
+  __device__ __forceinline__ int part_row(const AttnArgs& p, const Plan& plan) const {
+    return (seg ? plan.rows_end[seg - 1] : 0) + head * span + group * (kChains * kBlockRows) +
+           (int)blockIdx.x * p.piece_rows;
+  }
   __device__ __forceinline__ int rows(const AttnArgs& p) const {
     return group_rows<kChains>(count, p.group, group);
   }
@@ -729,7 +750,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
     // The whole warp runs this loop, so that addresses and descriptors stay in uniform registers;
     // one elected lane issues.
     for (int r = blockIdx.x + gridDim.x * lane; r < p.rows; r += gridDim.x * 32)
-      write_row_plan(p, kTok, plan, r);
+      write_row_plan<kChains>(p, kTok, plan, r);
     __syncwarp();
     if (!idle) {
       constexpr uint32_t kIdescS = instr_desc<T>(kTok, false), kIdescO = instr_desc<T>(kDim, true);
@@ -970,16 +991,15 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
     int task = 0;        // tiles this chain has taken
     int tile_index = 0;  // tiles of the CTA before the piece
     Piece piece;
-    int64_t part = 0;  // where this row's partial goes
+    int part = 0;  // where this row's partial goes
     bool room = false;
     // To the next piece that this chain takes tiles of, and open it. A single tile that is the other
     // chain's leaves an empty partial.
     auto advance = [&] {
       while (cur.at < c_hi) {
         piece = piece_at(cur, tile_index);
-        const int slot = (int)blockIdx.x + (cur.seg ? plan.groups_end[cur.seg - 1] : 0) + cur.index();
-        part = ((int64_t)slot * kChains + w) * kBlockRows + row;
-        room = slot >= 0 && slot < p.slots;
+        part = cur.part_row(p, plan) + w * (piece.both ? kBlockRows : cur.rows(p)) + row;
+        room = part < p.part_rows;
         if (kChains == 1 || piece.mine > 0) {
           open_piece(cur, piece.both);
           return true;
@@ -1230,7 +1250,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 
       // ---- end of a piece: the next one's queries first, then O out
       const int done_rows = my_rows, last = task - 1;
-      const int64_t done_part = part;
+      const int done_part = part;
       const bool done_room = room;
       tile_index += piece.tiles;
       cur.skip(p, plan, piece.tiles, kTok);
@@ -1241,7 +1261,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
       __syncwarp();
       if ((warp & 3) * 32 < done_rows) {
         const bool act = row < done_rows && done_room;
-        float* dst = p.part_o + done_part * p.dim;
+        float* dst = p.part_o + (int64_t)done_part * p.dim;
 #pragma unroll 1
         for (int c0 = 0; c0 < p.dim; c0 += 32) {
           uint32_t x[32];
@@ -1276,39 +1296,39 @@ __global__ void __launch_bounds__(Shape<kDim, kTma>::kThreads, 1)
 constexpr int kMaxPartials = 4 * kMaxCtas;
 
 // Where the partials of (row t, query head h) are: n[0] of the prefix, then n[1] of the request; two
-// in each slot where the chains took turns.
+// of each CTA, `chain` rows apart, where the chains took turns.
 template <int kChains>
 struct Partials {
-  int n[2], from[2], row[2], both[2];
+  int n[2], from[2], chain[2], step;
   __device__ __forceinline__ Partials(const AttnArgs& p, const RowPlan& r, int grid, int t, int h) {
     const int head = p.by_group.div(h), g = h - head * p.group;
     const Cost cost(r.even);
     const int ctas = cost.ctas(r.cost, grid);
+    step = p.piece_rows;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      n[i] = from[i] = row[i] = 0;
-      both[i] = 1;
+      n[i] = from[i] = chain[i] = 0;
       const int tiles = i ? r.tiles : r.prefix_tiles, count = i ? r.count : r.prefix_count;
+      const int span = i ? r.span : r.prefix_span;  // rows of partials of a head
       if (!r.owned || tiles == 0) continue;
       const int f = (t - (i ? r.first : r.prefix_first)) * p.group + g;
       const int index = f / (kChains * kBlockRows);
       const int group = head * groups_of<kChains>(count, p.group) + index;
-      both[i] = kChains == 1 || group_rows<kChains>(count, p.group, index) > kBlockRows;
-      row[i] = f % (kChains * kBlockRows);
+      const int rows = group_rows<kChains>(count, p.group, index);
+      if (kChains > 1 && rows <= kBlockRows) chain[i] = rows;
       const int weight = tile_cost<kChains>(cost, count, p.group);
       const int at = (i ? r.cost0 : 0) + group * (cost.open + tiles * weight);
       const int last = at + (tiles > 1 ? cost.open + (tiles - 1) * weight : 0);
       const int c0 = plan_owner(r.cost, ctas, at), c1 = plan_owner(r.cost, ctas, last);
-      from[i] = c0 + (i ? r.group0 : 0) + group;
-      n[i] = min(min(c1 - c0 + 1, kMaxCtas), max(0, p.slots - from[i])) * (both[i] ? 1 : 2);
+      const int n_ctas = min(c1 - c0 + 1, kMaxCtas);
+      from[i] = (i ? r.rows0 : 0) + head * span + f + c0 * step;
+      if (from[i] + (n_ctas - 1) * step + chain[i] < p.part_rows) n[i] = n_ctas * (chain[i] ? 2 : 1);
     }
   }
   __device__ __forceinline__ int64_t place(int j) const {
-    const bool own = j >= n[0], whole = own ? both[1] : both[0];
-    const int k = own ? j - n[0] : j, f = own ? from[1] : from[0], r = own ? row[1] : row[0];
-    // a whole group's rows run over its chains; a shared block of rows is in each
-    return (int64_t)(f + (whole ? k : k >> 1)) * (kChains * kBlockRows) + r +
-           (whole ? 0 : (k & 1) * kBlockRows);
+    const bool own = j >= n[0];
+    const int k = own ? j - n[0] : j, f = own ? from[1] : from[0], c = own ? chain[1] : chain[0];
+    return c ? f + (k >> 1) * step + (k & 1) * c : f + k * step;
   }
 };
 
@@ -1474,15 +1494,26 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const AttnAr
 }
 
 int round_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Slots, and partials in all, of the variant with `chains` chains.
-int64_t slots_for(int requests, int rows, int group, int kv_heads, int chains) {
-  const int64_t groups = ((int64_t)rows * group + chains * kBlockRows - 1) / (chains * kBlockRows);
-  return kMaxCtas + kv_heads * (2 * groups + requests);
+// Rows of the largest piece, and of partials in all, with so many chains: every row is in a group of the
+// prefix and in one of its request, and has a partial for each chain at most.
+int piece_rows_for(int rows, int group, int chains) {
+  return std::min(chains * kBlockRows, chains * rows * group);
 }
-int64_t partials_for(int requests, int rows, int group, int kv_heads) {
-  return kBlockRows * std::max(slots_for(requests, rows, group, kv_heads, 1),
-                               2 * slots_for(requests, rows, group, kv_heads, 2));
+int part_rows_for(int rows, int group, int kv_heads, int chains) {
+  return 2 * chains * rows * group * kv_heads + kMaxCtas * piece_rows_for(rows, group, chains);
 }
+// The workspace: row plans, statistics and outputs of the partials. Two chains, where the head
+// dimension allows them, take the more of it.
+struct Layout {
+  size_t ml, o, bytes;
+  Layout(int rows, int q_heads, int kv_heads, int dim) {
+    const size_t n = part_rows_for(rows, q_heads / kv_heads, kv_heads, round_dim(dim) <= 128 ? 2 : 1);
+    auto aligned = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    ml = aligned(rows * sizeof(RowPlan));
+    o = ml + aligned(n * sizeof(float2));
+    bytes = o + n * dim * sizeof(float);
+  }
+};
 
 template <typename T, int kDim, bool kTma>
 int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int ctas,
@@ -1491,7 +1522,8 @@ int launch_typed(const CUtensorMap& mk, const CUtensorMap& mv, AttnArgs& p, int 
   constexpr int kChains = S::kChains;
   constexpr size_t smem = attn_smem<kDim, kTma>();
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  p.slots = (int)slots_for(p.requests, p.rows, p.group, p.kv_heads, kChains);
+  p.part_rows = part_rows_for(p.rows, p.group, p.kv_heads, kChains);
+  p.piece_rows = piece_rows_for(p.rows, p.group, kChains);
   auto kernel = attn_kernel<T, kDim, kTma>;
   static bool configured[64] = {};
   int dev = 0;
@@ -1591,9 +1623,7 @@ extern "C" size_t b2_prefix_attn_workspace(int requests, int rows, int q_heads, 
                                            int head_dim) {
   using namespace b2;
   if (check_shape(requests, rows, q_heads, kv_heads, head_dim)) return 0;
-  return (size_t)partials_for(requests, rows, q_heads / kv_heads, kv_heads) *
-             (head_dim * sizeof(float) + sizeof(float2)) +
-         (size_t)rows * sizeof(RowPlan) + 256;
+  return Layout(rows, q_heads, kv_heads, head_dim).bytes;
 }
 
 extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
@@ -1662,9 +1692,9 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   p.scale_log2 = scale * kLog2e;
   p.minus_zero = 0x8000000080000000ull;
   p.row_plan = static_cast<RowPlan*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(p.row_plan + rows);
-  const size_t ml_bytes = ((size_t)rows * sizeof(RowPlan) + (size_t)partials_for(requests, rows, group, kv_heads) * sizeof(float2) + 255) & ~(size_t)255;
-  p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + ml_bytes);
+  const Layout layout(rows, q_heads, kv_heads, head_dim);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + layout.ml);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + layout.o);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == B2_DTYPE_F16 ? launch_type<__half>(p, ctas, s)
                                : launch_type<__nv_bfloat16>(p, ctas, s);

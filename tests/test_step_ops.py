@@ -229,3 +229,18 @@ def test_oracle_biases_first_by_hand():
     x = torch.tensor([[2.0, -1.0, 0.5]])
     assert so.logits_ref(x, **a, bias_first=True)[0][0].tolist() == [3.5, 1.75, 1.5]
     assert so.logits_ref(x, **a)[0][0].tolist() == [6.0, 2.75, 1.5]
+
+
+@pytest.mark.parametrize("requests,rows,hq,hk,dim", [
+    (1, 1, 24, 4, 256), (64, 64, 32, 8, 128), (256, 256, 32, 32, 128), (1024, 1024, 32, 8, 128),
+    (256, 256, 24, 4, 256), (1, 8, 48, 8, 128), (16, 4096, 32, 8, 64), (1, 1, 1, 1, 8),
+])
+def test_workspace_follows_the_rows(capi, requests, rows, hq, hk, dim):
+    """A row's partials of the prefix and of its request, two each where two chains share the tiles (up
+    to dimension 128), and those of one group more for each of at most 160 blocks: all in fp32 with two
+    statistics."""
+    chains = 2 if dim <= 128 else 1
+    group = min(chains * 128, chains * rows * hq // hk)
+    most = (2 * chains * rows * hq + 160 * group) * (4 * dim + 8) + 64 * rows + 1024
+    need = capi.lib().b2_prefix_attn_workspace(requests, rows, hq, hk, dim)
+    assert 4 * rows * hq * dim <= need <= most
