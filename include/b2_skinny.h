@@ -339,7 +339,7 @@ int b2_rope_cache(const void* q, const int64_t* q_strides, const void* k, const 
  * A row that sees nothing, and a row of no request, gets out = 0 and lse = -inf. Tokens a row does
  * not see do not reach it, whatever they hold (NaN, infinities); neither do places of a page
  * behind a length. Tokens on a page whose id is outside [0, total_pages) are left out; lengths are
- * cut at what the tables can hold.
+ * cut at what the tables can hold, at most 2^31 - 256 tokens each.
  *
  * Lengths, tables and row starts are read on the device: a captured call follows them. Query head
  * h reads KV head h / (q_heads / kv_heads). q [rows, q_heads, head_dim] with {row, head} strides

@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kMaxRequests = 1024;
 constexpr int kMaxRows = 4096;
+constexpr int kMaxTokens = 0x7fffff00;  // a tile that begins below it ends below 2^31
 constexpr int kLoadThreads = 128;
 constexpr int kBlockRows = 128;  // rows of one product: the lanes of tensor memory
 constexpr unsigned int kMaxPolls = 1u << 20;  // of two barriers in turn, before the wait with a clock
@@ -1651,8 +1652,8 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
       (requests > 0 && !own_lens) || !row_start || !out || !lse || (n_prefix_pages > 0 && !prefix_pages) ||
       (max_pages > 0 && !pages))
     return fail(B2_ERR_INVALID_ARG, "%s: null pointer", op);
-  if ((int64_t)n_prefix_pages * page_size > 0x7ffffff0 || (int64_t)max_pages * page_size > 0x7ffffff0)
-    return fail(B2_ERR_INVALID_ARG, "%s: tables of more than 2^31 tokens", op);
+  if ((int64_t)n_prefix_pages * page_size > kMaxTokens || (int64_t)max_pages * page_size > kMaxTokens)
+    return fail(B2_ERR_INVALID_ARG, "%s: tables of more than %d tokens", op, kMaxTokens);
   if (!aligned16(k_cache) || !aligned16(v_cache) || (reinterpret_cast<uintptr_t>(q) & 3u) != 0)
     return fail(B2_ERR_INVALID_ARG, "%s: caches must be 16-byte and q 4-byte aligned", op);
   if (q_strides[0] % 2 != 0 || q_strides[1] % 2 != 0)

@@ -244,3 +244,13 @@ def test_workspace_follows_the_rows(capi, requests, rows, hq, hk, dim):
     most = (2 * chains * rows * hq + 160 * group) * (4 * dim + 8) + 64 * rows + 1024
     need = capi.lib().b2_prefix_attn_workspace(requests, rows, hq, hk, dim)
     assert 4 * rows * hq * dim <= need <= most
+
+
+def test_prefix_attn_longest_tables(capi):
+    """Tables of 2^31 - 256 tokens are taken (no workspace is given: the call ends there), longer ones
+    refused: positions in the last tile would pass 31 bits."""
+    most = (2**31 - 256) // 16
+    assert attn_call(capi, np=most, ws=None) == capi.B2_ERR_WORKSPACE
+    assert attn_call(capi, max_pages=most, ws=None) == capi.B2_ERR_WORKSPACE
+    assert attn_call(capi, np=most + 1, ws=None) == capi.B2_ERR_INVALID_ARG
+    assert attn_call(capi, max_pages=most + 1, ws=None) == capi.B2_ERR_INVALID_ARG
