@@ -268,7 +268,6 @@ struct Plan {
   int len[kMaxRequests + 1];         // tokens
   int even;
 };
-constexpr int kMaxCost = 8;  // of a tile, with the opening of its group
 
 template <int kChains>
 __device__ __forceinline__ int groups_of(int count, int group) {
@@ -1590,6 +1589,17 @@ int launch_type(AttnArgs& p, int ctas, cudaStream_t stream) {
   }
 }
 
+// Costs are counted in 32 bits, for whatever lengths the tables can hold. With b blocks of 128 rows per
+// KV head: of the prefix, b groups of 2 a tile, or with two chains half as many, rounded up, of 4; of
+// a request with x rows 2 a tile up to 128 rows, else 4 for every 256 begun, both at most 2 + 4 x / 128
+// (x = 257: 8 of 10). The opening of a group costs two such tiles at most.
+bool costs_fit(int requests, int rows, int q_heads, int kv_heads, int dim, int64_t prefix, int64_t own) {
+  const int tok = round_dim(dim) == 64 ? 128 : 64;
+  const int64_t b = ((int64_t)rows * (q_heads / kv_heads) + kBlockRows - 1) / kBlockRows;
+  const int64_t per_prefix = 2 * b + 2, per_own = 4 * b + 2 * std::min(requests, rows);
+  return kv_heads * (per_prefix * (prefix / tok + 3) + per_own * (own / tok + 3)) <= 0x7fff0000;
+}
+
 int check_shape(int requests, int rows, int q_heads, int kv_heads, int head_dim) {
   const char* op = "prefix_attn";
   if (requests < 0 || requests > kMaxRequests)
@@ -1661,17 +1671,14 @@ extern "C" int b2_prefix_attn(const void* q, const int64_t* q_strides, const voi
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
       return fail(B2_ERR_INVALID_ARG, "%s: cache strides must be multiples of 8 elements", op);
+  if (!costs_fit(requests, rows, q_heads, kv_heads, head_dim, (int64_t)n_prefix_pages * page_size,
+                 (int64_t)max_pages * page_size))
+    return fail(B2_ERR_INVALID_ARG, "%s: tables too long for %d rows of %d requests", op, rows, requests);
   const size_t need = b2_prefix_attn_workspace(requests, rows, q_heads, kv_heads, head_dim);
   if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
     return fail(B2_ERR_WORKSPACE, "%s: workspace of %zu B, need %zu B, 256-byte aligned", op, ws_bytes,
                 need);
   const int group = q_heads / kv_heads;
-  const int tok = round_dim(head_dim) == 64 ? 128 : 64;
-  // costs are counted in 32 bits
-  const int64_t blocks = ((int64_t)rows * group + kBlockRows - 1) / kBlockRows;
-  const int64_t tiles = ((int64_t)std::max(n_prefix_pages, max_pages) * page_size + tok - 1) / tok;
-  if ((2 * blocks + requests) * kv_heads * tiles * kMaxCost > 0x7fffffff)
-    return fail(B2_ERR_INVALID_ARG, "%s: tables too long for %d rows", op, rows);
   DeviceInfo di;
   rc = device_info(&di);
   if (rc) return rc;

@@ -254,3 +254,44 @@ def test_prefix_attn_longest_tables(capi):
     assert attn_call(capi, max_pages=most, ws=None) == capi.B2_ERR_WORKSPACE
     assert attn_call(capi, np=most + 1, ws=None) == capi.B2_ERR_INVALID_ARG
     assert attn_call(capi, max_pages=most + 1, ws=None) == capi.B2_ERR_INVALID_ARG
+
+
+def longest(rows_of, hq, hk, dim, tokens):
+    """The cost of requests with so many rows over a prefix and own tokens of that length each, as the
+    plan counts it in 32 bits: the larger of one and two chains."""
+    group, tiles, worst = hq // hk, -(-tokens // (128 if dim <= 64 else 64)), 0
+    for chains in (1, 2):
+        def segment(rows):
+            x = rows * group
+            return -(-x // (128 * chains)) * (4 + tiles * (4 if chains > 1 and x > 128 else 2))
+        worst = max(worst, hk * (segment(sum(rows_of)) + sum(map(segment, rows_of))))
+    return worst
+
+
+@pytest.mark.parametrize("rows_of,hq,hk,dim", [
+    ([1] * 256, 32, 8, 128), ([8], 48, 8, 128), ([4096], 32, 8, 128), ([4] * 1024, 16, 16, 64),
+    ([1] * 1023 + [300], 64, 8, 256), ([33] * 7, 8, 1, 64), ([257], 1, 1, 128), ([0] * 50 + [129], 2, 2, 64),
+])
+def test_prefix_attn_table_limit(capi, rows_of, hq, hk, dim):
+    """Tables are refused where the costs of their lengths could pass 31 bits, however the rows are
+    spread over the requests, and not long before."""
+    def taken(tokens):
+        rc = attn_call(capi, requests=len(rows_of), rows=sum(rows_of), hq=hq, hk=hk, dim=dim,
+                       np=tokens // 16, max_pages=tokens // 16, ws=None)
+        assert rc in (capi.B2_ERR_WORKSPACE, capi.B2_ERR_INVALID_ARG)
+        return rc == capi.B2_ERR_WORKSPACE
+
+    lo, hi = 0, 2**31 - 256
+    while hi - lo > 4096:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if taken(mid) else (lo, mid)
+    assert longest(rows_of, hq, hk, dim, lo + 16) < 2**31 - 1024
+    n, t = len(rows_of), sum(rows_of)
+    spread = [t // n + (i < t % n) for i in range(n)]
+    assert lo > 2**31 - 8192 or longest(spread, hq, hk, dim, lo) > 2**31 // 4
+
+
+def test_prefix_attn_takes_wide_tables(capi):
+    """256 requests of one row with room for ten million tokens each."""
+    kw = dict(requests=256, rows=256, hq=32, hk=8, np=0, max_pages=10_000_000 // 16, ws=None)
+    assert attn_call(capi, **kw) == capi.B2_ERR_WORKSPACE
