@@ -81,6 +81,19 @@ def skinny8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor | None:
 
 _HALF = (torch.float16, torch.bfloat16)
 _FLOATS = (*_HALF, torch.float32)
+_INTS = (torch.int32, torch.int64)
+
+
+def _is_list(t: torch.Tensor, n: int, like: torch.Tensor, *dtypes) -> bool:
+    """Contiguous, with n elements of one of the types, where `like` is."""
+    return (t.dim() == 1 and t.shape[0] == n and t.dtype in dtypes and t.device == like.device
+            and t.is_contiguous())
+
+
+def _is_table(t: torch.Tensor, like: torch.Tensor, *dtypes) -> bool:
+    """Two-dimensional with contiguous rows of one of the types, where `like` is."""
+    return (t.dim() == 2 and t.dtype in dtypes and t.device == like.device
+            and (t.shape[1] <= 1 or t.stride(1) == 1))
 
 
 class RotaryPositions:
@@ -103,10 +116,16 @@ class RotaryPositions:
         t = t.unflatten(1, (-1, self.head_size)) if t.dim() == 2 else t
         return t if t.shape[-1] == self.head_size and t.stride(-1) == 1 else None
 
+    def _takes(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor) -> bool:
+        return (2 <= self.head_size <= 1024 and self.rotary_dim <= self.head_size
+                and q.dtype == k.dtype and q.device == k.device == self.inv_freq.device
+                and q.shape[0] == k.shape[0] and 1 <= q.shape[1] <= 65536 and 1 <= k.shape[1] <= 65536
+                and _is_list(positions, q.shape[0], q, *_INTS))
+
     def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor):
         """(query, key) turned, in the inputs' shapes, or None."""
         q, k = self._heads(query), self._heads(key)
-        if q is None or k is None or q.dtype != k.dtype or positions.dim() != 1:
+        if q is None or k is None or not self._takes(positions, q, k):
             return None
         q, k = self.ops.rope(q, k, positions, self.inv_freq, self.scale, self.interleaved)
         return q.view(query.shape), k.view(key.shape)
@@ -116,11 +135,19 @@ class RotaryPositions:
                           slot_mapping: torch.Tensor) -> torch.Tensor | None:
         """The turned query; the turned key and the value go to ``slot_mapping`` of the caches
         [blocks, block_size, kv_heads, head_size] (vLLM's reshape_and_cache, in the same launch;
-        -1 writes nothing). None, with the caches untouched, when the shapes are not handled."""
+        -1 writes nothing). None, with the caches untouched, when the shapes are not handled, among
+        them a ``slot_mapping`` shorter than the (padded) rows."""
         q, k, v = self._heads(query), self._heads(key), self._heads(value)
-        if q is None or k is None or v is None or positions.dim() != 1:
+        if q is None or k is None or v is None or not self._takes(positions, q, k):
             return None
-        if any(t.dtype != q.dtype for t in (k, v, key_cache, value_cache)):  # e.g. an fp8 cache
+        if v.shape != k.shape or v.dtype != q.dtype or v.device != q.device:
+            return None
+        for t in (key_cache, value_cache):  # another type: an fp8 cache, for example
+            if not (t.dtype == q.dtype and t.device == q.device and t.dim() == 4
+                    and t.shape[2:] == k.shape[1:] and t.shape == key_cache.shape
+                    and t.shape[0] and t.shape[1] and t.stride(3) == 1):
+                return None
+        if not _is_list(slot_mapping, q.shape[0], q, torch.int64):
             return None
         return self.ops.rope_cache(q, k, v, positions, self.inv_freq, slot_mapping, key_cache,
                                    value_cache, self.scale, self.interleaved).view(query.shape)
@@ -149,6 +176,18 @@ class PrefixTables:
         self.row_start = query_start_loc
 
 
+def attention_tables_fit(requests: int, rows: int, heads: int, kv_heads: int, dim: int, prefix: int,
+                         own: int) -> bool:
+    """Whether the kernel takes tables for ``prefix`` shared and ``own`` tokens of each request: it
+    plans the lengths they can hold in 32 bits (the rule of ``b2_prefix_attn``)."""
+    if max(prefix, own) > 2**31 - 256:
+        return False
+    tile, blocks = 128 if dim <= 64 else 64, -(-rows * (heads // kv_heads) // 128)
+    cost = (2 * blocks + 2) * (prefix // tile + 3) \
+        + (4 * blocks + 2 * min(requests, rows)) * (own // tile + 3)
+    return kv_heads * cost <= 0x7fff0000
+
+
 def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                      tables: PrefixTables, scale: float, tree: torch.Tensor | None = None,
                      ops=None) -> tuple[torch.Tensor, torch.Tensor] | None:
@@ -156,17 +195,29 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     own blocks: (output, log-sum-exp [rows, heads] in fp32), or None when the kernel does not take
     the shapes. ``tree`` (int64 [rows]) replaces the causal order among a request's new rows: bit m
     lets a row see the m-th of them."""
+    if query.dim() != 3 or key_cache.dim() != 4 or key_cache.shape != value_cache.shape:
+        return None
     rows, heads, dim = query.shape
-    kv_heads = key_cache.shape[2]
+    total, page, kv_heads = key_cache.shape[:3]
+    requests = tables.pages.shape[0]
 
     def loadable(cache):  # 16-byte loads
-        return (cache.dtype == query.dtype and cache.stride(3) == 1 and cache.data_ptr() % 16 == 0
-                and all(s % 8 == 0 for s in cache.stride()[:3]))
+        return (cache.dtype == query.dtype and cache.device == query.device and cache.stride(3) == 1
+                and cache.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in cache.stride()[:3]))
 
     if not (query.dtype in _HALF and loadable(key_cache) and loadable(value_cache)
             and query.stride(2) == 1 and query.stride(0) % 2 == 0 and query.stride(1) % 2 == 0
-            and query.data_ptr() % 4 == 0 and dim % 8 == 0 and dim <= 256 and heads <= 1024
-            and heads % kv_heads == 0 and rows <= 4096 and tables.pages.shape[0] <= 1024):
+            and query.data_ptr() % 4 == 0 and 8 <= dim <= 256 and dim % 8 == 0
+            and key_cache.shape[3] == dim and total and page and kv_heads and 1 <= heads <= 1024
+            and heads % kv_heads == 0 and rows <= 4096 and requests <= 1024
+            and _is_table(tables.pages, query, torch.int32)
+            and _is_list(tables.prefix_pages, tables.prefix_pages.numel(), query, torch.int32)
+            and _is_list(tables.prefix_len, 1, query, torch.int32)
+            and _is_list(tables.own_lens, requests, query, torch.int32)
+            and _is_list(tables.row_start, requests + 1, query, torch.int32)
+            and (tree is None or _is_list(tree, rows, query, torch.int64))
+            and attention_tables_fit(requests, rows, heads, kv_heads, dim,
+                                     tables.prefix_pages.numel() * page, tables.pages.shape[1] * page)):
         return None
     return (ops or _ops()).prefix_attn(query, key_cache, value_cache, tables.prefix_pages,
                                        tables.prefix_len, tables.pages, tables.own_lens,
@@ -182,9 +233,21 @@ def process_logits(logits: torch.Tensor, tokens=None, row_seq=None, prompt_lens=
     request; ``vocab_start`` is a tensor-parallel shard's first token."""
     if logits.dtype not in _FLOATS or logits.dim() != 2 or logits.stride(1) != 1:
         return None
-    if tokens is not None and tokens.shape[1] >= 1 << 20:
+    rows, vocab = logits.shape
+    if not 0 <= vocab_start <= 2**31 - 65 - vocab:
         return None
-    if bias_ids is not None and bias_ids.shape[1] > 2047:
+    lists = ((row_seq, torch.int32), (prompt_lens, torch.int32), (total_lens, torch.int32),
+             (repetition, torch.float32), (frequency, torch.float32), (presence, torch.float32))
+    if not all(t is None or _is_list(t, rows, logits, dtype) for t, dtype in lists):
+        return None
+    if tokens is not None and not (_is_table(tokens, logits, *_INTS) and tokens.shape[1] < 1 << 20):
+        return None
+    for t, dtype in ((bias_ids, torch.int32), (bias_values, torch.float32)):
+        if t is not None and not (_is_table(t, logits, dtype) and t.is_contiguous()
+                                  and t.shape[0] == rows and t.shape[1] <= 2047):
+            return None
+    if mask is not None and not (_is_table(mask, logits, torch.int32) and mask.shape[0] == rows
+                                 and mask.shape[1] * 32 >= vocab_start + vocab):
         return None
     return (ops or _ops()).logits_process(logits, tokens, row_seq, prompt_lens, total_lens,
                                           repetition, frequency, presence, bias_ids, bias_values,

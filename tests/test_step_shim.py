@@ -112,3 +112,91 @@ def test_logits_in_the_samplers_order(shim):
                         ops=r)
     name, args = r.calls[-1]
     assert name == "logits_process" and len(args) == 13 and args[12] is True
+
+
+def test_rotary_leaves_what_the_kernel_does_not_take(shim):
+    """Each of these made the operator raise; the caller has its stock path."""
+    r = Recorder()
+    rot = shim.RotaryPositions(64, 32, device="cpu", ops=r)
+    q, k, v = torch.randn(5, 512).half(), torch.randn(5, 128).half(), torch.randn(5, 128).half()
+    pos, slots, cache = torch.arange(5), torch.arange(5), torch.zeros(2, 3, 16, 2, 64).half()
+    for bad in (pos.float(), pos[:4], pos.view(1, 5), torch.arange(10)[::2]):
+        assert rot.forward(bad, q, k) is None
+        assert rot.forward_and_cache(bad, q, k, v, cache[0], cache[1], slots) is None
+    assert rot.forward(pos, q, k[:4]) is None
+    for bad in (slots[:4], slots.int(), slots.view(5, 1), torch.arange(10)[::2]):
+        assert rot.forward_and_cache(pos, q, k, v, cache[0], cache[1], bad) is None
+    for bad in (cache[0][0], cache[0][:, :, :1], cache[0][..., :32], cache[0][:0], cache[0].transpose(2, 3),
+                cache[0][:2]):
+        assert rot.forward_and_cache(pos, q, k, v, cache[0], bad, slots) is None
+    assert rot.forward_and_cache(pos, q, k, torch.randn(5, 256).half(), cache[0], cache[1], slots) is None
+    wide = shim.RotaryPositions(1026, 32, device="cpu", ops=r)
+    assert wide.forward(pos, torch.randn(5, 1026), torch.randn(5, 1026)) is None
+    assert not r.calls
+    assert rot.forward_and_cache(pos.int(), q, k, v, cache[0], cache[1], slots) is not None
+
+
+def test_prefix_attention_leaves_what_the_kernel_does_not_take(shim):
+    r = Recorder()
+    table = torch.arange(12, dtype=torch.int32).reshape(2, 6)
+    lens, starts = torch.tensor([70, 40]).int(), torch.tensor([0, 1, 4]).int()
+    q, cache = torch.randn(4, 8, 128).half(), torch.zeros(2, 12, 16, 2, 128).half()
+
+    def call(q=q, k=cache[0], v=cache[1], common=32, table=table, lens=lens, starts=starts, tree=None):
+        t = shim.PrefixTables(common, 16, table, lens, starts)
+        return shim.prefix_attention(q, k, v, t, 0.1, tree, ops=r)
+
+    assert call() is not None and call(tree=torch.zeros(4, dtype=torch.int64)) is not None
+    n = len(r.calls)
+    for bad in (dict(q=q.flatten(1)), dict(k=cache[0][0]), dict(v=cache[1][:5]),
+                dict(k=cache[0][..., :64], v=cache[1][..., :64]), dict(table=table.long()),
+                dict(lens=lens.long()), dict(starts=starts.long()), dict(starts=starts[:2]),
+                dict(lens=lens[:1]), dict(tree=torch.zeros(3, dtype=torch.int64)),
+                dict(tree=torch.zeros(4, dtype=torch.int32)), dict(table=table.T, common=0),
+                dict(k=cache[0][:0], v=cache[1][:0]),
+                dict(table=table[:1, :1].expand(2, 1 << 27), common=0)):
+        assert call(**bad) is None, bad.keys()
+    assert len(r.calls) == n
+
+
+@pytest.mark.parametrize("requests,rows,hq,hk,dim", [(256, 256, 32, 8, 128), (1024, 4096, 16, 16, 64),
+                                                     (1, 8, 48, 8, 256), (7, 300, 8, 1, 128)])
+def test_table_limit_is_the_kernels(shim, capi, requests, rows, hq, hk, dim):
+    """On both sides of the limit, of the shared and of the own tables, the call site's rule is that of
+    the C ABI (no workspace is given: a call that is taken ends there)."""
+    at, st = 1 << 20, capi.strides
+
+    def taken(prefix, own):
+        rc = capi.lib().b2_prefix_attn(
+            at, st(hq * dim, dim), at, st(16 * hk * dim, hk * dim, dim), at, st(16 * hk * dim, hk * dim, dim),
+            9, 16, at, prefix // 16, at, at, own // 16, own // 16, at, at, None, requests, rows, hq, hk, dim,
+            0.1, 0, at, at, None, 0, None)
+        assert rc in (capi.B2_ERR_WORKSPACE, capi.B2_ERR_INVALID_ARG)
+        return rc == capi.B2_ERR_WORKSPACE
+
+    for mix in ((1, 0), (0, 1), (1, 1), (3, 1)):
+        lo, hi = 0, 2**27
+        while hi - lo > 1:
+            mid = (lo + hi) // 2
+            p, o = (min(16 * mid * m, 2**32) for m in mix)
+            fits = shim.attention_tables_fit(requests, rows, hq, hk, dim, p, o)
+            assert fits == taken(p, o)
+            lo, hi = (mid, hi) if fits else (lo, mid)
+
+
+def test_logits_leave_what_the_kernel_does_not_take(shim):
+    r = Recorder()
+    x, i32 = torch.randn(3, 100).half(), torch.int32
+    good = dict(tokens=torch.zeros(2, 9, dtype=i32), row_seq=torch.zeros(3, dtype=i32),
+                prompt_lens=torch.zeros(3, dtype=i32), total_lens=torch.zeros(3, dtype=i32),
+                repetition=torch.ones(3), bias_ids=torch.zeros(3, 2, dtype=i32),
+                bias_values=torch.zeros(3, 2), mask=torch.zeros(3, 4, dtype=i32))
+    assert shim.process_logits(x, **good, ops=r) is not None
+    for bad in (dict(tokens=torch.zeros(2, 9)), dict(tokens=good["tokens"][0]),
+                dict(tokens=torch.zeros(2, 18, dtype=i32)[:, ::2]), dict(row_seq=torch.zeros(3).long()),
+                dict(total_lens=torch.zeros(2, dtype=i32)), dict(repetition=torch.ones(3).double()),
+                dict(bias_ids=good["bias_ids"].long()), dict(bias_values=torch.zeros(2, 2)),
+                dict(mask=good["mask"][:, :3]), dict(mask=good["mask"].long()), dict(vocab_start=-1),
+                dict(vocab_start=2**31 - 100)):
+        assert shim.process_logits(x, **{**good, **bad}, ops=r) is None, bad.keys()
+    assert len(r.calls) == 1
