@@ -32,6 +32,7 @@ namespace {
 constexpr int kMaxDim = 1024;
 constexpr int kRopeThreads = 128;
 constexpr int kFewRows = 148;
+constexpr int kMaxGridY = 65535;
 // Items of a thread whose loads are under way together, with many rows; with few, a thread has one.
 // With one, 2048 rows with the cache write take 11.3 us instead of 10.3; with four 11.9, and 4099 rows
 // 16.9 instead of 15.8. Blocks of 64 threads: 9.4 and 16.5; of 256: 13.8 and 19.9. Where a thread has
@@ -49,7 +50,7 @@ struct RopeArgs {
   int64_t n_slots;
   int q_heads, kv_heads, dim, rot, page;
   int units;        // work units per head
-  int items;        // units of a whole row
+  int items;        // units of a whole row, 2^27 at most
   int chunk;        // items per block
   FastDiv by_units;
   int pos64;
@@ -220,8 +221,10 @@ int launch_typed(RopeArgs& p, int rows, bool vec, cudaStream_t stream) {
   p.units = vec ? (p.dim + 15) / 16 : (p.dim + 1) / 2;
   p.items = heads * p.units;
   p.by_units = make_div(p.units);
-  // A block per row, or with few rows an item per thread, so that more SMs take part.
-  p.chunk = rows >= kFewRows ? p.items : std::min(p.items, kRopeThreads);
+  // A block per row, or with few rows an item per thread, so that more SMs take part; more items than
+  // that where a row of very many heads would have more blocks than a grid may along y.
+  const int few = std::max(kRopeThreads, (p.items + kMaxGridY - 1) / kMaxGridY);
+  p.chunk = rows >= kFewRows ? p.items : std::min(p.items, few);
   const dim3 grid((unsigned)rows, (unsigned)((p.items + p.chunk - 1) / p.chunk));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

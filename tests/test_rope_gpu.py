@@ -204,3 +204,14 @@ def test_refusals(ops):
     for call in bad:
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 258), (F16, 256)])
+def test_most_heads(ops, dtype, dim):
+    """As many heads as there may be, in one row: more blocks than a grid has in its second
+    dimension, were each to take one item per thread."""
+    q, k, _ = heads(1, 65536, 64, dim, dtype, 11)
+    pos, inv = torch.tensor([12345], device="cuda"), freqs(dim // 2 // 16 * 16)
+    qo, ko = ops.rope(q, k, pos, inv)
+    check(qo, q, pos, inv, 1.0, False)
+    check(ko, k, pos, inv, 1.0, False)
