@@ -380,7 +380,8 @@ int b2_prefix_attn(const void* q, const int64_t* q_strides, const void* k_cache,
  *   bit (token & 31) of mask[r * mask_stride + token / 32] clear:            x = -inf
  * repetition, frequency, presence, biases and mask may be NULL. tokens holds int32, or int64 when
  * tokens_64 is non-zero, rows tokens_stride apart; ids outside the shard are skipped, a row_seq
- * outside [0, n_seqs) means no history. At most 2^20 - 1 tokens of history and 2047 biases a row.
+ * outside [0, n_seqs) means no history. At most 2^30 columns, 2^20 - 1 tokens of
+ * history and 2047 biases a row.
  * `out` may be `logits` where those are fp32 and contiguous. Results do not depend on timing.
  * ---------------------------------------------------------------------------------------- */
 int b2_logits_process(const void* logits, int64_t row_stride, int dtype, float* out, int rows,

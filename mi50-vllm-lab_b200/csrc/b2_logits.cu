@@ -56,6 +56,7 @@ constexpr int kMaxSlice = kMostThreads * kVec * kSteps;    // words of shared me
 constexpr int kAhead = 8;                              // tokens of the history a thread loads at a time
 constexpr int kMaxBias = 2047;                         // 11 bits of the word
 constexpr int kMaxHistory = (1 << 20) - 1;             // 20 bits
+constexpr int kMaxVocab = 1 << 30;                     // columns, with the rounding to slices, in 31 bits
 constexpr uint32_t kPromptBit = 0x80000000u;
 constexpr uint32_t kMark = 0x40000000u;
 
@@ -431,7 +432,8 @@ int check_and_launch(const void* logits, int64_t row_stride, int dtype, float* o
                      int n_bias, const uint32_t* mask, int64_t mask_stride, int mask_words,
                      bool bias_first, void* stream) {
   const char* op = "logits_process";
-  if (rows < 0 || vocab < 1) return fail(B2_ERR_INVALID_ARG, "%s: %d rows of %d logits", op, rows, vocab);
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab)
+    return fail(B2_ERR_INVALID_ARG, "%s: %d rows of %d logits (at most %d)", op, rows, vocab, kMaxVocab);
   if (vocab_start < 0 || (int64_t)vocab_start + vocab > 0x7fffffff - 64)
     return fail(B2_ERR_INVALID_ARG, "%s: vocab_start=%d", op, vocab_start);
   if (dtype != B2_DTYPE_F16 && dtype != B2_DTYPE_BF16 && dtype != B2_DTYPE_F32)

@@ -234,7 +234,7 @@ def process_logits(logits: torch.Tensor, tokens=None, row_seq=None, prompt_lens=
     if logits.dtype not in _FLOATS or logits.dim() != 2 or logits.stride(1) != 1:
         return None
     rows, vocab = logits.shape
-    if not 0 <= vocab_start <= 2**31 - 65 - vocab:
+    if vocab > 1 << 30 or not 0 <= vocab_start <= 2**31 - 65 - vocab:
         return None
     lists = ((row_seq, torch.int32), (prompt_lens, torch.int32), (total_lens, torch.int32),
              (repetition, torch.float32), (frequency, torch.float32), (presence, torch.float32))

@@ -295,3 +295,11 @@ def test_prefix_attn_takes_wide_tables(capi):
     """256 requests of one row with room for ten million tokens each."""
     kw = dict(requests=256, rows=256, hq=32, hk=8, np=0, max_pages=10_000_000 // 16, ws=None)
     assert attn_call(capi, **kw) == capi.B2_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("vocab", [2**30 + 1, 2**31 - 65 - 2000, 2**31 - 65])
+def test_logits_process_refuses_too_many_columns(capi, vocab):
+    """Their number rounded up to slices would pass 31 bits (no row is given: a call that is taken ends
+    there)."""
+    assert logits_call(capi, rows=0, vocab=2**30) == 0
+    assert logits_call(capi, rows=0, vocab=vocab) == capi.B2_ERR_INVALID_ARG
