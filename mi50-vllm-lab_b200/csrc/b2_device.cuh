@@ -416,14 +416,13 @@ struct UnitCursor {
 // Division of 0 <= n < 2^31 by a number fixed for the launch, as a product and a shift (Granlund and
 // Montgomery, Division by Invariant Integers using Multiplication, 1994).
 struct FastDiv {
-  uint32_t d, mul, shift;
+  uint32_t mul, shift;
   __device__ __forceinline__ int div(int n) const {
     return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
   }
 };
 inline FastDiv make_div(int d) {
   FastDiv f;
-  f.d = (uint32_t)d;
   f.shift = 0;
   while ((1ll << f.shift) < d) ++f.shift;
   f.mul = (uint32_t)((((1ull << f.shift) - (uint64_t)d) << 32) / (uint64_t)d + 1);

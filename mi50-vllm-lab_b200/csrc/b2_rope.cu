@@ -31,7 +31,6 @@ namespace {
 
 constexpr int kMaxDim = 1024;
 constexpr int kRopeThreads = 128;
-constexpr int kFewRows = 148;
 constexpr int kMaxGridY = 65535;
 // Items of a thread whose loads are under way together, with many rows; with few, a thread has one.
 // With one, 2048 rows with the cache write take 11.3 us instead of 10.3; with four 11.9, and 4099 rows
@@ -216,15 +215,15 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs p) {
 }
 
 template <typename T, bool kInterleaved, bool kCache>
-int launch_typed(RopeArgs& p, int rows, bool vec, cudaStream_t stream) {
+int launch_typed(RopeArgs& p, int rows, bool vec, bool few, cudaStream_t stream) {
   const int heads = p.q_heads + p.kv_heads * (kCache ? 2 : 1);
   p.units = vec ? (p.dim + 15) / 16 : (p.dim + 1) / 2;
   p.items = heads * p.units;
   p.by_units = make_div(p.units);
-  // A block per row, or with few rows an item per thread, so that more SMs take part; more items than
-  // that where a row of very many heads would have more blocks than a grid may along y.
-  const int few = std::max(kRopeThreads, (p.items + kMaxGridY - 1) / kMaxGridY);
-  p.chunk = rows >= kFewRows ? p.items : std::min(p.items, few);
+  // A block per row, or with fewer rows than SMs an item per thread, so that more of them take part;
+  // more items than that where a row of very many heads would have more blocks than a grid may along y.
+  const int least = std::max(kRopeThreads, (p.items + kMaxGridY - 1) / kMaxGridY);
+  p.chunk = few ? std::min(p.items, least) : p.items;
   const dim3 grid((unsigned)rows, (unsigned)((p.items + p.chunk - 1) / p.chunk));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -269,6 +268,7 @@ int launch_rope(RopeArgs& p, int rows, int interleaved, int dtype, cudaStream_t 
   DeviceInfo di;
   const int rc = device_info(&di);
   if (rc) return rc;
+  const bool few = rows < di.sm_count;
   bool vec = dtype != B2_DTYPE_F32 && p.dim % 8 == 0 && p.rot % 16 == 0 && aligned16(p.q) &&
              aligned16(p.k) && aligned16(p.q_out);
   for (int64_t s : {p.q_row, p.q_head, p.k_row, p.k_head}) vec = vec && s % 8 == 0;
@@ -280,13 +280,13 @@ int launch_rope(RopeArgs& p, int rows, int interleaved, int dtype, cudaStream_t 
     vec = vec && aligned16(p.k_out);
   }
   switch (dtype * 2 + (interleaved ? 1 : 0)) {
-    case B2_DTYPE_F16 * 2: return launch_typed<__half, false, kCache>(p, rows, vec, stream);
-    case B2_DTYPE_F16 * 2 + 1: return launch_typed<__half, true, kCache>(p, rows, vec, stream);
-    case B2_DTYPE_BF16 * 2: return launch_typed<__nv_bfloat16, false, kCache>(p, rows, vec, stream);
+    case B2_DTYPE_F16 * 2: return launch_typed<__half, false, kCache>(p, rows, vec, few, stream);
+    case B2_DTYPE_F16 * 2 + 1: return launch_typed<__half, true, kCache>(p, rows, vec, few, stream);
+    case B2_DTYPE_BF16 * 2: return launch_typed<__nv_bfloat16, false, kCache>(p, rows, vec, few, stream);
     case B2_DTYPE_BF16 * 2 + 1:
-      return launch_typed<__nv_bfloat16, true, kCache>(p, rows, vec, stream);
-    case B2_DTYPE_F32 * 2: return launch_typed<float, false, kCache>(p, rows, vec, stream);
-    default: return launch_typed<float, true, kCache>(p, rows, vec, stream);
+      return launch_typed<__nv_bfloat16, true, kCache>(p, rows, vec, few, stream);
+    case B2_DTYPE_F32 * 2: return launch_typed<float, false, kCache>(p, rows, vec, few, stream);
+    default: return launch_typed<float, true, kCache>(p, rows, vec, few, stream);
   }
 }
 
