@@ -9,9 +9,10 @@
 //
 // Angles: the product p * inv_freq is formed in fp64 and reduced there to a fraction of a turn in
 // [-1/2, 1/2], whose sine and cosine are taken in fp32. A fp32 product would be off by p * 2^-24
-// radians, 0.06 at position 10^6; the reduced fraction is off by at most 2^-26 turns. The fp64
-// work is three operations per frequency and row, shared by all heads of the row through a table
-// in shared memory.
+// radians, 0.06 at position 10^6; the reduced fraction is off by 2^-26 turns, its rounding to fp32,
+// and by 2.5 * 2^-53 of the turns themselves, which is a tenth of that at 2^25 radians. The fp64 work
+// is three operations per frequency and row, shared by all heads of the row through a table in shared
+// memory.
 //
 // Bound: memory. A row's heads are read and written once, 16 bytes per access; a thread owns both
 // members of its pairs, so outputs may alias inputs. The table is built behind the loads of the

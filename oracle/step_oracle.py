@@ -31,7 +31,9 @@ def rope_ref(x, positions, inv_freq, scale=1.0, interleaved=False):
     """x [rows, heads, dim] turned, and the bound on a kernel's error per element.
 
     The bound: half a step of the type, plus what fp32 arithmetic adds. The reduced angle is off by
-    at most 2^-26 turns (its rounding to fp32, |fraction| <= 1/2) = 9.4e-8 rad; sincospi is good to
+    at most 2^-26 turns (its rounding to fp32, |fraction| <= 1/2) = 9.4e-8 rad, beside 2.5 * 2^-53 of
+    the turns for the fp64 products, which is under 2^-26 up to 2^28 radians (the angle here is such a
+    product, too); sincospi is good to
     2^-22 (2 units in the last place); factor, two products and their sum round by 2^-24 each:
     under 6e-7 (|a| + |b|) scale in all."""
     x = x.detach().cpu()
