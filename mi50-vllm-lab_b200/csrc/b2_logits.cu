@@ -48,8 +48,10 @@ namespace {
 
 constexpr int kMostThreads = 512;
 constexpr int kVec = 8;                                // tokens per thread and step
-// Steps of a slice. Five at two CTAs per SM (64 registers) keep 128 rows' stream at 19.1 us; four at
-// three CTAs spill at 40 registers, 23.7 us. Smaller CTAs read the history more often: 256 threads
+// Steps of a slice, chosen for 16-bit logits: five at two CTAs per SM (64 registers) keep 128 rows'
+// stream at 19.1 us; four at three CTAs spill at 40 registers, 23.7 us. With fp32 logits, twice the
+// registers for a step, five spill: 128 rows of 151936 with one token of history 35.8 us of 23.8 that
+// their bytes take, with long histories, biases and mask 63. Smaller CTAs read the history more often: 256 threads
 // took 73 us for the long histories where 512 took 56.
 constexpr int kSteps = 5;
 constexpr int kMaxSlice = kMostThreads * kVec * kSteps;    // words of shared memory per CTA
@@ -93,8 +95,8 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* row, int words, in
 
 // A row's penalties. The division by `rep` is a product with its reciprocal and one correction by
 // the residual (Markstein, IBM J. Res. Dev. 34, 1990), which gives the rounded quotient in a few
-// instructions without a branch: a warp works on 32 tokens of which some are divided and others
-// multiplied. Where the residual is no number (infinite x) the product stands. `plain`: the row's
+// instructions without a branch (for |x| of 2^-102 and more, where the residual is exact): a warp works
+// on 32 tokens of which some are divided and others multiplied. Where the residual is no number (infinite x) the product stands. `plain`: the row's
 // `rep` is too small or too large for that, or 0 or infinite, and the row divides.
 struct RowParams {
   float rep, inv, freq, pres;
